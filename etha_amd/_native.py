@@ -7,14 +7,14 @@ from __future__ import annotations
 
 import ctypes
 import os
-from ctypes import POINTER, byref, c_char_p, c_int, c_uint32, c_uint64, c_void_p
+from ctypes import POINTER, byref, c_char_p, c_float, c_int, c_int64, c_uint32, c_uint64, c_void_p
 
 import numpy as np
 
 from .build import LIB_PATH
 
 ETHA_MAX_NDIM = 8
-ABI_VERSION = 6
+ABI_VERSION = 7
 LAUNCH_UNORDERED = 1  # ETHA_LAUNCH_UNORDERED
 SEG_PACK, SEG_UNPACK, SEG_REDUCE_PACK, SEG_SELFCOPY = 0, 1, 2, 3  # ETHA_SEG_*
 MAX_SEGMENTS = 16
@@ -145,6 +145,18 @@ _SIGNATURES = {
     "etha_ipc_export": (c_int, [c_void_p, POINTER(IpcHandle)]),
     "etha_ipc_open": (c_int, [POINTER(IpcHandle), POINTER(c_void_p)]),
     "etha_ipc_close": (c_int, [c_void_p]),
+    "etha_embedding": (c_int, [c_void_p, c_uint32, c_uint64, c_void_p, c_uint32, c_uint64, c_uint64, c_int64, c_int64, c_float,
+                               c_void_p, c_uint32, c_int64, c_void_p]),
+    "etha_embedding_grad_workspace": (c_int, [c_uint64, c_uint64, c_uint64, c_uint32, POINTER(c_uint64)]),
+    "etha_embedding_grad": (c_int, [c_void_p, c_uint32, c_int64, c_void_p, c_uint32, c_uint64, c_uint64, c_uint64, c_int64, c_float,
+                                    c_void_p, c_uint32, c_int64, c_int, c_void_p, c_uint64, c_void_p]),
+    "etha_quantize_rows": (c_int, [c_void_p, c_uint32, c_uint64, c_uint64, c_int64, c_void_p, c_int64, c_void_p, c_void_p]),
+    "etha_int8_matmul": (c_int, [c_void_p, c_void_p, c_uint64, c_int64, c_void_p, c_void_p, c_uint64, c_int64, c_uint64, c_void_p,
+                                 c_void_p, c_uint32, c_int64, c_void_p]),
+    "etha_grouped_matmul": (c_int, [c_void_p, c_uint32, c_uint64, c_int64, c_void_p, c_uint64, c_uint64, c_uint64, c_int64, c_int64,
+                                    c_int, c_void_p, c_void_p, c_uint32, c_int64, c_int, c_void_p]),
+    "etha_grouped_matmul_reduce": (c_int, [c_void_p, c_void_p, c_uint32, c_uint64, c_int64, c_int64, c_uint64, c_uint64, c_uint64,
+                                           c_void_p, c_void_p, c_uint32, c_int64, c_int64, c_void_p]),
 }
 
 _lib = None
@@ -407,6 +419,14 @@ class Schedule:
             self.close()
         except Exception:
             pass
+
+
+def embedding_grad_workspace(n_tokens: int, n_rows: int, width: int, grad_dtype: int) -> int:
+    """Bytes of workspace that ``etha_embedding_grad`` needs for these sizes."""
+    out = c_uint64()
+    _check("etha_embedding_grad_workspace",
+           lib().etha_embedding_grad_workspace(n_tokens, n_rows, width, grad_dtype, byref(out)))
+    return out.value
 
 
 def ipc_open(handle_bytes: bytes) -> int:

@@ -1,0 +1,114 @@
+"""Checks and addressing shared by the operators on local shards (:mod:`etha_amd.embedding`, :mod:`etha_amd.int8`,
+:mod:`etha_amd.experts`): device tensors in, one call of the C ABI out."""
+
+from __future__ import annotations
+
+import torch
+
+from . import _native
+
+DTYPE_CODES = {torch.float32: _native.F32, torch.bfloat16: _native.BF16, torch.float16: _native.F16}
+TOKEN_CODES = {torch.int32: _native.I32, torch.int64: _native.I64}
+
+
+def check_device(what: str, first: torch.Tensor, *others: torch.Tensor | None) -> torch.device:
+    """The one GPU that all operands live on."""
+    device = first.device
+    if device.type != "cuda":
+        raise RuntimeError(f"{what}: tensors live on {device}; this operator only runs on a GPU (there is no CPU path)")
+    for t in others:
+        if t is not None and t.device != device:
+            raise ValueError(f"{what}: operands live on {device} and {t.device}")
+    return device
+
+
+def code_of(what: str, dtype: torch.dtype) -> int:
+    code = DTYPE_CODES.get(dtype)
+    if code is None:
+        raise ValueError(f"{what}: element type {dtype}; float32, bfloat16 and float16 are supported")
+    return code
+
+
+def row_stride(t: torch.Tensor) -> int | None:
+    """Distance, in elements, between consecutive rows (all leading dims flattened) of a tensor whose last dim is
+    contiguous; None if the rows do not lie at one distance."""
+    dim = t.dim()
+    if dim == 2:  # the usual case first
+        return t.stride(0) if t.stride(1) == 1 or t.shape[1] <= 1 else None
+    if dim == 0 or (t.stride(-1) != 1 and t.shape[-1] > 1):
+        return None
+    stride, expect = None, None
+    for size, step in zip(reversed(t.shape[:-1]), reversed(t.stride()[:-1])):
+        if size == 1:
+            continue
+        if stride is None:
+            stride = step
+        elif step != expect:
+            return None
+        expect = step * size
+    return t.shape[-1] if stride is None else stride
+
+
+def readable_rows(t: torch.Tensor) -> tuple[torch.Tensor, int]:
+    """``t`` or, where its rows do not lie at one distance, a contiguous copy; and that distance."""
+    stride = row_stride(t)
+    if stride is None:
+        t = t.contiguous()
+        stride = row_stride(t)
+    return t, stride
+
+
+def _byte_range(t: torch.Tensor) -> tuple[int, int]:
+    """First byte and the byte behind the last that the elements of ``t`` lie in."""
+    lo = hi = 0
+    for size, step in zip(t.shape, t.stride()):
+        lo += min(0, (size - 1) * step)
+        hi += max(0, (size - 1) * step)
+    es = t.element_size()
+    return t.data_ptr() + lo * es, t.data_ptr() + (hi + 1) * es
+
+
+def check_out(what: str, out: torch.Tensor, shape, dtypes, *inputs: torch.Tensor | None) -> int:
+    """Checks an output that the caller passes; returns its row stride."""
+    if tuple(out.shape) != tuple(shape):
+        raise ValueError(f"{what}: out has shape {tuple(out.shape)}, not {tuple(shape)}")
+    if out.dtype not in dtypes:
+        raise ValueError(f"{what}: out is {out.dtype}")
+    if out.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{what}: out requires a gradient")
+    stride = row_stride(out)
+    rows = out.numel() // out.shape[-1] if out.dim() and out.shape[-1] else 0
+    if stride is None or (rows > 1 and stride < out.shape[-1]):
+        raise ValueError(f"{what}: the rows of out have to be contiguous, apart and at one distance")
+    if out.numel():
+        lo, hi = _byte_range(out)
+        for t in inputs:
+            if t is not None and t.numel():
+                a, b = _byte_range(t)
+                if a < hi and lo < b:
+                    raise ValueError(f"{what}: out overlaps an input")
+    return stride
+
+
+def refuse_grad(what: str, *inputs: torch.Tensor | None) -> None:
+    """For operators without a gradient: a silent cut of the graph would train on nothing."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in inputs):
+        raise RuntimeError(f"{what} has no gradient: call it under torch.no_grad() or detach its inputs")
+
+
+def refuse_captured_backward(what: str) -> None:
+    """Autograd's accumulation into a leaf runs on the stream of the leaf's first graph; under capture on another stream
+    that ends the process, so a backward pass is captured by calling the gradient functions themselves."""
+    if torch.cuda.is_current_stream_capturing():
+        raise RuntimeError(f"the backward pass of {what} cannot be captured into a graph: capture a call of its gradient function")
+
+
+def call(device: torch.device, func, name: str, *args) -> None:
+    """``func(*args, stream)`` on the current stream of ``device``, which becomes the current device for the call."""
+    if device.index != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            rc = func(*args, torch.cuda.current_stream(device).cuda_stream)
+    else:
+        rc = func(*args, torch.cuda.current_stream(device).cuda_stream)
+    if rc != 0:
+        _native._check(name, rc)

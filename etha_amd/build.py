@@ -1,6 +1,6 @@
 """Build recipe for the HIP library (gfx950 only).
 
-``python -m etha_amd.build`` compiles ``csrc/etha_reshard.hip`` into
+``python -m etha_amd.build`` compiles the ``csrc/*.hip`` files into
 ``etha_amd/libetha_reshard.so`` next to this file.  hipcc cross-compiles, so no GPU is needed.
 """
 
@@ -11,10 +11,13 @@ import os
 import shutil
 import subprocess
 import sys
+import tempfile
 
 PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 REPO_DIR = os.path.dirname(PKG_DIR)
-SOURCE = os.path.join(PKG_DIR, "csrc", "etha_reshard.hip")
+CSRC_DIR = os.path.join(PKG_DIR, "csrc")
+SOURCES = [os.path.join(CSRC_DIR, name) for name in ("etha_reshard.hip", "etha_rows.hip", "etha_matmul.hip", "etha_digest.hip")]
+INTERNAL_HEADERS = [os.path.join(CSRC_DIR, name) for name in ("etha_internal.h", "etha_device.h")]
 INCLUDE_DIR = os.path.join(REPO_DIR, "include")
 # ETHA_AMD_LIB selects another build of the same library (kernel tuning experiments)
 LIB_PATH = os.environ.get("ETHA_AMD_LIB") or os.path.join(PKG_DIR, "libetha_reshard.so")
@@ -28,7 +31,6 @@ HIPCC_FLAGS = [
     # workgroup here lives only a few microseconds, and that load is on its critical path (measured +0.3 %)
     "-mllvm", "-amdgpu-kernarg-preload-count=8",
     "-fPIC",
-    "-shared",
     "-std=c++17",
 ]
 
@@ -47,7 +49,7 @@ def source_hash() -> str:
     """Digest of the sources and compiler flags the library is built from; the library carries the one it was
     built with."""
     h = hashlib.sha256(" ".join(HIPCC_FLAGS).encode())
-    for path in (SOURCE, HEADER):
+    for path in (*SOURCES, *INTERNAL_HEADERS, HEADER):
         with open(path, "rb") as f:
             h.update(f.read())
     return h.hexdigest()[:32]
@@ -73,12 +75,22 @@ def build_library(verbose: bool = False, defines: tuple[str, ...] = (), out_path
     """Compile the shared library (always recompiles) and return its path."""
     out_path = out_path or LIB_PATH
     defines = (*defines, f'ETHA_SOURCE_HASH="{source_hash()}"')
-    cmd = [hipcc_path(), *HIPCC_FLAGS, *[f"-D{d}" for d in defines], f"-I{INCLUDE_DIR}", "-o", out_path + ".tmp", SOURCE]
-    proc = subprocess.run(cmd, capture_output=True, text=True)
-    if proc.returncode != 0:
-        raise RuntimeError(f"hipcc failed ({proc.returncode}):\n{' '.join(cmd)}\n{proc.stdout}\n{proc.stderr}")
-    if verbose and proc.stderr:
-        sys.stderr.write(proc.stderr)
+    with tempfile.TemporaryDirectory() as tmp:  # one object per source file, compiled side by side
+        jobs = []
+        for source in SOURCES:
+            obj = os.path.join(tmp, os.path.basename(source) + ".o")
+            cmd = [hipcc_path(), *HIPCC_FLAGS, *[f"-D{d}" for d in defines], f"-I{INCLUDE_DIR}", "-c", "-o", obj, source]
+            jobs.append((cmd, obj, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)))
+        outputs = [(cmd, proc.communicate()[0], proc.returncode) for cmd, _, proc in jobs]
+        link = [hipcc_path(), "-shared", "-fPIC", "--offload-arch=gfx950", "-o", out_path + ".tmp", *[obj for _, obj, _ in jobs]]
+        if all(rc == 0 for _, _, rc in outputs):
+            proc = subprocess.run(link, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
+            outputs.append((link, proc.stdout, proc.returncode))
+        for cmd, text, rc in outputs:
+            if rc != 0:
+                raise RuntimeError(f"hipcc failed ({rc}):\n{' '.join(cmd)}\n{text}")
+            if verbose and text:
+                sys.stderr.write(text)
     os.replace(out_path + ".tmp", out_path)
     return out_path
 

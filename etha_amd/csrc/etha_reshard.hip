@@ -28,7 +28,13 @@
 #include <string>
 #include <vector>
 
+#include "etha_internal.h"
 #include "etha_reshard.h"
+
+using etha_internal::fail;
+using etha_internal::g_err;
+using etha_internal::g_kernel_launches;
+using etha_internal::guarded;
 
 namespace {
 
@@ -1446,9 +1452,6 @@ __global__ __launch_bounds__(ETHA_TRANS_THREADS, 8) void etha_transpose_reduce_k
 // =================================================================================================
 // Host side: validation and the tile compiler.
 // =================================================================================================
-// message of the calling thread's last failure; a fixed buffer, so that reporting a failure (out of host memory
-// among them) allocates nothing
-thread_local char g_err[512] = "";
 // An allocation may be opened once per process; several tensors usually share one allocation, so
 // mappings are cached per handle and reference-counted.
 struct IpcMapping {
@@ -1461,35 +1464,6 @@ std::map<IpcKey, IpcMapping> g_ipc_open;
 std::map<void*, IpcKey> g_ipc_ptrs;  // pointer handed out by etha_ipc_open -> its handle (multimap not needed:
                                      // equal pointers come from equal handles and share the count)
 std::map<void*, int> g_ipc_ptr_refs;
-
-int fail(int code, const char* fmt, ...) {
-  va_list ap;
-  va_start(ap, fmt);
-  vsnprintf(g_err, sizeof(g_err), fmt, ap);
-  va_end(ap);
-  return code;
-}
-
-// Body of an entry point that builds host-side containers: no C++ exception leaves the library (the ABI is
-// plain C); running out of host memory becomes ETHA_ERR_NOMEM.
-template <typename F>
-int guarded(const char* what, F&& body) {
-  try {
-    return body();
-  } catch (const std::bad_alloc&) {
-    return fail(ETHA_ERR_NOMEM, "%s: out of host memory", what);
-  } catch (const std::exception& e) {
-    return fail(ETHA_ERR_INVALID, "%s: %s", what, e.what());
-  } catch (...) {
-    return fail(ETHA_ERR_INVALID, "%s: unexpected exception", what);
-  }
-}
-
-#define HIP_TRY(expr)                                                                      \
-  do {                                                                                     \
-    hipError_t e_ = (expr);                                                                \
-    if (e_ != hipSuccess) return fail(ETHA_ERR_HIP, "%s: %s", #expr, hipGetErrorString(e_)); \
-  } while (0)
 
 int dtype_size(uint32_t dt) {
   switch (dt) {
@@ -2107,8 +2081,6 @@ int check_range(const EthaTable* t, uint32_t first, uint32_t count, int kind) {
 // clears that wait for this one dispatch: the kernel may start while earlier launches are still running,
 // which removes the drain/ramp bubble between launches that do not depend on each other.  The next
 // ordinary launch on the stream again waits for everything before it, unordered launches included.
-std::atomic<uint64_t> g_kernel_launches{0};
-
 template <typename... Args, typename F>
 void launch_kernel(F kernel, dim3 grid, dim3 block, size_t lds, void* stream, uint32_t flags, Args... args) {
   g_kernel_launches.fetch_add(1, std::memory_order_relaxed);
@@ -2590,14 +2562,8 @@ struct EthaSchedule {
 
 extern "C" {
 
-#ifndef ETHA_SOURCE_HASH
-#define ETHA_SOURCE_HASH "unknown"
-#endif
 int etha_abi_version(void) { return ETHA_ABI_VERSION; }
 uint64_t etha_kernel_launches(void) { return g_kernel_launches.load(std::memory_order_relaxed); }
-// the marker lets a build script find the digest in the file without loading the library
-static const char kSourceDigest[] = "etha-source-digest:" ETHA_SOURCE_HASH;
-const char* etha_source_hash(void) { return kSourceDigest + sizeof("etha-source-digest:") - 1; }
 const char* etha_last_error(void) { return g_err; }
 
 int etha_table_create(const EthaChunkDesc* descs, uint32_t n_chunks, const uint64_t* partial_ptrs,

@@ -32,7 +32,7 @@
 extern "C" {
 #endif
 
-#define ETHA_ABI_VERSION 6
+#define ETHA_ABI_VERSION 7
 #define ETHA_MAX_NDIM 8
 
 /* status codes */
@@ -319,6 +319,72 @@ int etha_arena_destroy(void* ptr);
 int etha_ipc_export(const void* dev_ptr, EthaIpcHandle* out);
 int etha_ipc_open(const EthaIpcHandle* handle, void** out_ptr); /* returns base + offset */
 int etha_ipc_close(void* opened_ptr);
+
+/*
+ * Operators on local shards: what reads or feeds the shards that a redistribute delivers.  No counterpart in the
+ * reference, which leaves them to the framework on either side of it.
+ *  - tensors are given by address and strides in elements of their own type; the last dimension is contiguous; rows
+ *    may start at any multiple of the element size.  Types are ETHA_F32, ETHA_BF16 and ETHA_F16 unless said otherwise.
+ *  - sums are held in fp32 (32-bit integers for 8-bit products) and rounded once.
+ *  - results do not depend on timing: the same call on the same values gives the same bits.
+ *  - launches are asynchronous on `stream` of the current device and can be captured into a graph; nothing is allocated.
+ *    An output must not overlap an input.
+ */
+
+/*
+ * Embedding lookup in a shard of rows [first_row, first_row + n_rows): out[t,:] = scale * weight[tokens[t] - first_row,:],
+ * zeros for a token of another shard (the results of all shards of a vocabulary are then a Partial sum).
+ * tokens: ETHA_I32 or ETHA_I64, any value.
+ */
+int etha_embedding(const void* tokens, uint32_t token_dtype, uint64_t n_tokens, const void* weight, uint32_t weight_dtype,
+                   uint64_t n_rows, uint64_t width, int64_t weight_stride, int64_t first_row, float scale, void* out,
+                   uint32_t out_dtype, int64_t out_stride, void* stream);
+
+/*
+ * Gradient of the lookup: out[r,:] = scale * sum of grad[t,:] over the tokens of row r, in the order of t (pieces of a
+ * frequent row are summed apart and joined in order); zeros for a row without tokens.  With accumulate the sum is added
+ * to out (one rounding) and rows without tokens are left as they are.  The workspace (16-byte aligned, at least the
+ * bytes that etha_embedding_grad_workspace names) may be used again once the launches have finished.
+ */
+int etha_embedding_grad_workspace(uint64_t n_tokens, uint64_t n_rows, uint64_t width, uint32_t grad_dtype, uint64_t* bytes);
+int etha_embedding_grad(const void* grad, uint32_t grad_dtype, int64_t grad_stride, const void* tokens, uint32_t token_dtype,
+                        uint64_t n_tokens, uint64_t n_rows, uint64_t width, int64_t first_row, float scale, void* out,
+                        uint32_t out_dtype, int64_t out_stride, int accumulate, void* workspace, uint64_t workspace_bytes,
+                        void* stream);
+
+/*
+ * Rows to 8 bits: scales[r] = max |x[r,:]| / 127, values[r,k] = x[r,k] / scales[r] rounded half to even (the exact
+ * quotient; within +-127), 0 where the scale is 0.  A row that holds a NaN or an infinity gets that as its scale and
+ * zeros as its values.
+ */
+int etha_quantize_rows(const void* x, uint32_t dtype, uint64_t rows, uint64_t width, int64_t x_stride, int8_t* values,
+                       int64_t values_stride, float* scales, void* stream);
+
+/*
+ * Product of 8-bit rows with a scale each: out[m,n] = x_scale[m] * w_scale[n] * sum_k x[m,k] * w[n,k] + bias[n] (bias:
+ * fp32, may be NULL).  The sum is exact; width is at most ETHA_INT8_MAX_WIDTH, so that it stays within 32 bits.
+ */
+#define ETHA_INT8_MAX_WIDTH 131071u
+int etha_int8_matmul(const int8_t* x, const float* x_scale, uint64_t rows, int64_t x_stride, const int8_t* w, const float* w_scale,
+                     uint64_t cols, int64_t w_stride, uint64_t width, const float* bias, void* out, uint32_t out_dtype,
+                     int64_t out_stride, void* stream);
+
+/*
+ * Products grouped by expert.  Rows [offsets[e], offsets[e+1]) of x belong to expert e (offsets: n_groups + 1 entries on
+ * the device; an entry outside [0, rows] or below an earlier one is taken as the nearest that is not).
+ * etha_grouped_matmul: out[t,:] = x[t,:] * w[e]^T with w[e] a [cols, red] matrix, or x[t,:] * w[e] with w[e] a [red, cols]
+ * one (w_transposed): the forward product and the gradient of its rows.  Rows of no expert become zeros with zero_rest
+ * and are left as they are without.
+ * etha_grouped_matmul_reduce: out[e] = grad[rows of e]^T * x[rows of e], the gradient of the weights, [out_rows, out_cols]
+ * for each expert; zeros for an expert without rows.
+ * Operands are ETHA_BF16 or ETHA_F16.
+ */
+int etha_grouped_matmul(const void* x, uint32_t dtype, uint64_t rows, int64_t x_stride, const void* w, uint64_t n_groups,
+                        uint64_t cols, uint64_t red, int64_t w_stride, int64_t w_group_stride, int w_transposed,
+                        const int32_t* offsets, void* out, uint32_t out_dtype, int64_t out_stride, int zero_rest, void* stream);
+int etha_grouped_matmul_reduce(const void* grad, const void* x, uint32_t dtype, uint64_t rows, int64_t grad_stride, int64_t x_stride,
+                               uint64_t n_groups, uint64_t out_rows, uint64_t out_cols, const int32_t* offsets, void* out,
+                               uint32_t out_dtype, int64_t out_stride, int64_t out_group_stride, void* stream);
 
 #ifdef __cplusplus
 }
