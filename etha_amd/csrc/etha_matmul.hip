@@ -1,10 +1,8 @@
 // Matrix products on local shards, MI355X (gfx950): 8-bit integers with scales, and products grouped by expert.
 //
 // One tile kernel serves every product here: an output tile out[r, c] = sum_k P(r, k) * Q(c, k), where either operand may
-// lie k-contiguous in memory or transposed (k as the memory row).  Tiles of both operands are staged through LDS as rows
-// of 128 bytes of k (64 elements of 16 bits, 128 of 8 bits) and go through the matrix units, which need 16 bytes of k a
-// lane for either type, so both share one layout.  The eight 16-byte pieces of LDS row r are stored at piece ^ (r & 7):
-// the 16 lanes that read the same piece of 16 rows then touch all banks.
+// lie k-contiguous in memory or transposed (k as the memory row).  The matrix instructions take 16 bytes of k a lane for
+// 16-bit and for 8-bit elements alike, so both types share every layout.
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
@@ -144,8 +142,96 @@ __device__ inline void group_bounds(const MatmulArgs& a, uint32_t group, uint32_
   *hi = (uint32_t)(end > top ? end : top);
 }
 
-// ---- staging through registers: any stride, any alignment --------------------------------------------------------
-constexpr int kStageBytes = 128;  // of k, a row
+// ---- staging -------------------------------------------------------------------------------------------------------
+// A stage holds BKB bytes of k of both operands.  Where an operand lies k-contiguous in memory its LDS tile is ROWS rows of
+// BKB bytes, read 16 bytes of k a lane; where it lies transposed (16-bit elements) the tile is the memory's own [k][ROWS],
+// read with the transposing LDS load, which hands each of 16 lanes four k of one column.  Either tile is a sequence of
+// 16-byte slots; which piece of memory a slot holds is permuted so that the lanes of one read touch all banks: by the row
+// where 16 rows are read at one k, in 32-byte column groups by (k & 3, k >> 3) where 8 rows of k are read at one column.
+constexpr uint32_t kOutside = 0x80000000u;  // an offset that no operand's tile reaches: reads there give zeros
+
+template <typename E, bool TRANS_, int ROWS, int BKB, int THREADS_>
+struct Operand {
+  static constexpr bool kTrans = TRANS_;
+  static constexpr int kEs = E::kEs, kThreads = THREADS_;
+  static constexpr int kStageK = BKB / kEs;
+  static constexpr int kBytes = ROWS * BKB, kSlots = kBytes / 16, kPer = kSlots / kThreads;
+  static constexpr int kPieces = kTrans ? ROWS / 8 : BKB / 16;  // slots of an LDS row
+  static_assert(kSlots % kThreads == 0 && kPer > 0, "every work-item stages the same number of slots");
+
+  static __device__ uint32_t row_of(uint32_t slot) { return slot / kPieces; }
+  static __device__ uint32_t swizzle(uint32_t row, uint32_t piece) {
+    if constexpr (kTrans) return piece ^ ((((row & 3) | ((row >> 1) & 4)) << 1) & (kPieces - 1));
+    else if constexpr (kPieces == 8) return piece ^ (row & 7);
+    else return piece ^ ((row >> 2) & 3);
+  }
+  static __device__ uint32_t piece_of(uint32_t slot) { return swizzle(row_of(slot), slot % kPieces); }
+
+  // The 16 bytes of k that this lane needs of tile row r0 + (lane & 15), from k piece kp0 + (lane >> 4) of the stage.
+  static __device__ u32x4 fragment(const char* lds, uint32_t r0, uint32_t kp0) {
+    const uint32_t lane = threadIdx.x & 63;
+    if constexpr (!kTrans) {
+      const uint32_t r = r0 + (lane & 15);
+      return *(const u32x4*)(lds + r * BKB + swizzle(r, kp0 + (lane >> 4)) * 16);
+    } else {
+      typedef short s16x4 __attribute__((ext_vector_type(4)));
+      typedef __attribute__((address_space(3))) s16x4* lds_ptr;
+      const uint32_t k = (kp0 + (lane >> 4)) * 8 + ((lane & 15) >> 2), col = r0 + (lane & 3) * 4;
+      const char* p = lds + k * (ROWS * 2) + swizzle(k, col >> 3) * 16 + (col & 7) * 2;
+      // rows k and k + 4 have the same permutation
+      const u32x2 a = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)p));
+      const u32x2 b = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(p + 4 * ROWS * 2)));
+      return u32x4{a.x, a.y, b.x, b.y};
+    }
+  }
+};
+
+__device__ inline uint32_t lds_address(const char* p) { return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) char*)p; }
+
+// Straight from memory into LDS, 16 bytes a lane: for operands whose rows start at 16-byte addresses and, k-contiguous
+// ones, hold whole 16-byte pieces of k.  The buffer descriptor ends with the operand tile's last byte, so that whatever
+// the tile reaches over reads as zero.  The loads write no registers; the kernel waits for them by count.
+template <typename OP>
+struct DirectStage {
+  static constexpr bool kDirect = true;
+  uint32_t at[OP::kPer];
+  uint32_t k_byte;   // where in the stage's k this lane's pieces lie (one place for all of them)
+  const char* base;
+  int64_t left;      // bytes from base to the end of the operand's tile
+  uint32_t stride;
+  uint32_t wave_at;  // where this wave's first slot lies in a stage
+
+  __device__ void init(const char* tile, int64_t row_stride, uint32_t n_rows, uint32_t red) {
+    base = tile;
+    stride = (uint32_t)row_stride;
+    left = OP::kTrans ? (int64_t)((int)red - 1) * row_stride + (int64_t)n_rows * 2
+                      : (int64_t)((int)n_rows - 1) * row_stride + (int64_t)red * OP::kEs;
+    #pragma unroll
+    for (int i = 0; i < OP::kPer; i++) {
+      const uint32_t slot = threadIdx.x + i * OP::kThreads;
+      at[i] = OP::row_of(slot) * stride + OP::piece_of(slot) * 16;
+    }
+    k_byte = OP::piece_of(threadIdx.x) * 16;
+    wave_at = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * 1024;
+  }
+  // The stage that begins at k0, into LDS; past the end of k it brings zeros.
+  __device__ void load(char* lds, uint32_t k0, uint32_t red) {
+    const uint64_t b = (uint64_t)base;
+    const uint32_t size = left > 0x7fffffff ? 0x7fffffffu : left < 0 ? 0u : (uint32_t)left;
+    const u32x4 rsrc = {(uint32_t)b, (uint32_t)(b >> 32) & 0xffffu, size, 0x00020000u};
+    const uint32_t to = lds_address(lds) + wave_at;
+    uint32_t outside = 0;
+    if constexpr (!OP::kTrans) outside = (int64_t)k_byte >= ((int64_t)red - (int64_t)k0) * OP::kEs ? kOutside : 0;
+    #pragma unroll
+    for (int i = 0; i < OP::kPer; i++)
+      asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+                   :: "s"(to + i * OP::kThreads * 16), "v"(at[i] | outside), "s"(rsrc) : "memory");
+    const int64_t step = OP::kTrans ? (int64_t)OP::kStageK * stride : (int64_t)OP::kStageK * OP::kEs;
+    base += step;
+    left -= step;
+  }
+  __device__ void store(char*) const {}
+};
 
 // 16 bytes at p of which `left` exist; the others read as zero
 template <int ES>
@@ -165,43 +251,36 @@ __device__ inline u32x4 load_part(const char* p, int64_t left) {
   return v;
 }
 
-__device__ inline uint32_t lds_at(uint32_t row, uint32_t piece) { return row * kStageBytes + ((piece ^ (row & 7)) << 4); }
+// Through registers: any start, any distance, any length of k.  The next stage's loads are in flight during a stage.
+template <typename OP>
+struct RegisterStage {
+  static constexpr bool kDirect = false;
+  u32x4 v[OP::kPer];
+  const char* base;
+  int64_t stride;
+  uint32_t n_rows;
 
-// One operand's tile of ROWS rows, THREADS work-items.  `n_rows` rows exist from `base` on; k0 is in elements.
-template <int ES, bool TRANS, int ROWS, int THREADS>
-struct Stage {
-  static constexpr int kPer = ROWS * 8 / THREADS;
-  u32x4 v[kPer];
-
-  __device__ void load(const char* base, int64_t stride, uint32_t n_rows, uint32_t k0, uint32_t red) {
+  __device__ void init(const char* tile, int64_t row_stride, uint32_t n_rows_, uint32_t) {
+    base = tile;
+    stride = row_stride;
+    n_rows = n_rows_;
+  }
+  __device__ void load(char*, uint32_t k0, uint32_t red) {
+    const bool whole = k0 + OP::kStageK <= red;
     #pragma unroll
-    for (int i = 0; i < kPer; i++) {
-      const uint32_t id = threadIdx.x + i * THREADS;
-      if constexpr (!TRANS) {
-        const uint32_t row = id >> 3, piece = id & 7;
-        const int64_t at = (int64_t)k0 * ES + piece * 16;
-        v[i] = load_part<ES>(base + (int64_t)row * stride + at, row < n_rows ? (int64_t)red * ES - at : 0);
-      } else {  // memory row = k, 8 tile rows a piece
-        constexpr uint32_t kPieces = ROWS / 8;
-        const uint32_t k = id / kPieces, piece = id % kPieces;
-        v[i] = load_part<ES>(base + (int64_t)(k0 + k) * stride + piece * 16, k0 + k < red ? ((int64_t)n_rows - piece * 8) * 2 : 0);
+    for (int i = 0; i < OP::kPer; i++) {
+      const uint32_t slot = threadIdx.x + i * OP::kThreads, row = OP::row_of(slot), piece = OP::piece_of(slot);
+      if constexpr (!OP::kTrans) {
+        const char* p = base + (int64_t)(row < n_rows ? row : n_rows - 1) * stride + (int64_t)k0 * OP::kEs + piece * 16;
+        v[i] = whole ? load_raw<16>(p) : load_part<OP::kEs>(p, ((int64_t)red - k0) * OP::kEs - piece * 16);
+      } else {  // memory row = k, a piece holds 8 tile rows
+        v[i] = load_part<OP::kEs>(base + (int64_t)(k0 + row) * stride + piece * 16, k0 + row < red ? ((int64_t)n_rows - piece * 8) * 2 : 0);
       }
     }
   }
   __device__ void store(char* lds) const {
     #pragma unroll
-    for (int i = 0; i < kPer; i++) {
-      const uint32_t id = threadIdx.x + i * THREADS;
-      if constexpr (!TRANS) {
-        *(u32x4*)(lds + lds_at(id >> 3, id & 7)) = v[i];
-      } else {
-        constexpr uint32_t kPieces = ROWS / 8;
-        const uint32_t k = id / kPieces, piece = id % kPieces;
-        #pragma unroll
-        for (int j = 0; j < 8; j++)
-          *(uint16_t*)(lds + lds_at(piece * 8 + j, k >> 3) + (k & 7) * 2) = (uint16_t)(v[i][j >> 1] >> (16 * (j & 1)));
-      }
-    }
+    for (int i = 0; i < OP::kPer; i++) *(u32x4*)(lds + (threadIdx.x + i * OP::kThreads) * 16) = v[i];
   }
 };
 
@@ -228,88 +307,129 @@ __device__ inline void store_four(const MatmulArgs& a, typename D::bits* out, ui
 }
 
 // ---- the tile kernel -----------------------------------------------------------------------------------------------
-constexpr int kTile = 128;
+// A tile of BM rows and BN columns, WM x WN waves, STAGES stages of BKB bytes of k in LDS.  One barrier a stage: behind it
+// every wave has finished the stage before, whose LDS the stage STAGES - 1 ahead may then take.
+template <int BM_, int BN_, int WM_, int WN_, int BKB_, int STAGES_>
+struct Shape {
+  static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, BKB = BKB_, STAGES = STAGES_;
+  static constexpr int kThreads = WM * WN * 64;
+};
 
-template <typename E, uint32_t KIND, typename D>
-__global__ __launch_bounds__(256) void etha_matmul_kernel(const MatmulArgs a) {
-  constexpr bool kTransP = KIND == kGroupReduce, kTransQ = KIND == kGroupReduce || KIND == kGroupRowsT;
-  constexpr uint32_t kStageK = kStageBytes / E::kEs;
-  __shared__ __align__(16) char s_p[kTile * kStageBytes];
-  __shared__ __align__(16) char s_q[kTile * kStageBytes];
-  const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const uint32_t col_tiles = (a.cols + kTile - 1) / kTile;
-  const uint32_t tile_col = blockIdx.x % col_tiles, rest = blockIdx.x / col_tiles;
-  const uint32_t col0 = tile_col * kTile;
+template <int N>
+__device__ inline void wait_stage() {  // at most N loads into LDS outstanding; this wave's LDS reads done
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" :: "n"(N) : "memory");
+}
+
+template <typename E, uint32_t KIND, typename D, typename S, template <typename> class STAGE>
+__global__ __launch_bounds__(S::kThreads) void etha_matmul_kernel(const MatmulArgs a) {
+  typedef Operand<E, KIND == kGroupReduce, S::BM, S::BKB, S::kThreads> OpP;
+  typedef Operand<E, KIND == kGroupReduce || KIND == kGroupRowsT, S::BN, S::BKB, S::kThreads> OpQ;
+  constexpr bool kDirect = STAGE<OpP>::kDirect;
+  constexpr int kStages = kDirect ? S::STAGES : 2, kFm = S::BM / S::WM / 16, kFn = S::BN / S::WN / 16;
+  constexpr uint32_t kStageK = OpP::kStageK;
+  __shared__ __align__(1024) char lds[kStages * (OpP::kBytes + OpQ::kBytes)];
+  const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t col_tiles = (a.cols + S::BN - 1) / S::BN;
+  // Workgroups go to the 8 XCDs in turn: each XCD takes a run of the tiles, so that its L2 sees operands again.  In a run
+  // the tiles go down bands of kBand row tiles.
+  constexpr uint32_t kBand = 4;
+  uint32_t id = blockIdx.x;
+  {
+    const uint32_t n = gridDim.x, xcd = id & 7, each = n >> 3, more = n & 7;
+    id = xcd * each + (xcd < more ? xcd : more) + (id >> 3);
+  }
+  const uint32_t row_tiles_all = gridDim.x / col_tiles, band = id / (kBand * col_tiles);
+  const uint32_t in_band = row_tiles_all - band * kBand < kBand ? row_tiles_all - band * kBand : kBand;
+  const uint32_t row_id = band * kBand + (id - band * kBand * col_tiles) % in_band;
+  const uint32_t col0 = (id - band * kBand * col_tiles) / in_band * S::BN;
   uint32_t row0, row_end, red = a.red;
   const char *p = a.p, *q = a.q;
   typename D::bits* out = (typename D::bits*)a.out;
   bool zero = false;
   if constexpr (KIND == kPlain) {
-    row0 = rest * kTile;
+    row0 = row_id * S::BM;
     row_end = a.rows;
   } else if constexpr (KIND == kGroupReduce) {
-    const uint32_t row_tiles = (a.rows + kTile - 1) / kTile, group = rest / row_tiles;
+    const uint32_t row_tiles = (a.rows + S::BM - 1) / S::BM, group = row_id / row_tiles;
     uint32_t lo, hi;
     group_bounds(a, group, &lo, &hi);
     red = hi - lo;
     p += (int64_t)lo * a.p_stride;
     q += (int64_t)lo * a.q_stride;
     out += (int64_t)group * a.out_group_stride;
-    row0 = rest % row_tiles * kTile;
+    row0 = row_id % row_tiles * S::BM;
     row_end = a.rows;
   } else {
-    const GroupTile t = find_tile<kTile>(a, rest);
+    const GroupTile t = find_tile<S::BM>(a, row_id);
     if (!t.found) return;
-    row0 = t.lo + t.tile * kTile;
+    row0 = t.lo + t.tile * S::BM;
     row_end = t.hi;
     zero = t.group == a.n_groups;
     if (!zero) q += (int64_t)t.group * a.q_group_stride;
   }
-  const uint32_t n_rows = row_end - row0 < kTile ? row_end - row0 : kTile;
-  const uint32_t n_cols = a.cols - col0 < kTile ? a.cols - col0 : kTile;
-  p += kTransP ? (int64_t)row0 * E::kEs : (int64_t)row0 * a.p_stride;
-  q += kTransQ ? (int64_t)col0 * E::kEs : (int64_t)col0 * a.q_stride;
+  const uint32_t n_rows = row_end - row0 < S::BM ? row_end - row0 : S::BM;
+  const uint32_t n_cols = a.cols - col0 < S::BN ? a.cols - col0 : S::BN;
+  p += OpP::kTrans ? (int64_t)row0 * E::kEs : (int64_t)row0 * a.p_stride;
+  q += OpQ::kTrans ? (int64_t)col0 * E::kEs : (int64_t)col0 * a.q_stride;
 
-  typename E::acc acc[4][4] = {};
-  const uint32_t wr = (wave >> 1) * 64, wc = (wave & 1) * 64;
-  if (!zero) {
-    Stage<E::kEs, kTransP, kTile, 256> sp;
-    Stage<E::kEs, kTransQ, kTile, 256> sq;
-    if (red) {
-      sp.load(p, a.p_stride, n_rows, 0, red);
-      sq.load(q, a.q_stride, n_cols, 0, red);
+  typename E::acc acc[kFm][kFn] = {};
+  const uint32_t wr = wave / S::WN * (S::BM / S::WM), wc = wave % S::WN * (S::BN / S::WN);
+  const uint32_t stages = zero ? 0 : (red + kStageK - 1) / kStageK;
+  if (stages) {
+    STAGE<OpP> sp;
+    STAGE<OpQ> sq;
+    sp.init(p, a.p_stride, n_rows, red);
+    sq.init(q, a.q_stride, n_cols, red);
+    constexpr int kAhead = kDirect ? kStages - 1 : 1;
+    #pragma unroll
+    for (int s = 0; s < kAhead; s++) {
+      char* to = lds + s * (OpP::kBytes + OpQ::kBytes);
+      sp.load(to, s * kStageK, red);
+      sq.load(to + OpP::kBytes, s * kStageK, red);
     }
-    for (uint32_t k0 = 0; k0 < red; k0 += kStageK) {
-      __syncthreads();
-      sp.store(s_p);
-      sq.store(s_q);
-      __syncthreads();
-      if (k0 + kStageK < red) {
-        sp.load(p, a.p_stride, n_rows, k0 + kStageK, red);
-        sq.load(q, a.q_stride, n_cols, k0 + kStageK, red);
+    if constexpr (!kDirect) {
+      sp.store(lds);
+      sq.store(lds + OpP::kBytes);
+    }
+    uint32_t use = 0, fill = kAhead * (OpP::kBytes + OpQ::kBytes);
+    for (uint32_t s = 0; s < stages; s++) {
+      if constexpr (kDirect) wait_stage<(kStages - 2) * (OpP::kPer + OpQ::kPer)>();
+      else __syncthreads();
+      // past the last stage these bring zeros that nobody reads: the count of loads stays the same
+      if (kDirect || s + 1 < stages) {
+        sp.load(lds + fill, (s + kAhead) * kStageK, red);
+        sq.load(lds + fill + OpP::kBytes, (s + kAhead) * kStageK, red);
       }
+      const char* lp = lds + use;
+      const char* lq = lp + OpP::kBytes;
       #pragma unroll
-      for (int s = 0; s < 2; s++) {
-        u32x4 fp[4], fq[4];
+      for (int h = 0; h < S::BKB / 64; h++) {
+        u32x4 fp[kFm], fq[kFn];
         #pragma unroll
-        for (int i = 0; i < 4; i++) {
-          fp[i] = *(const u32x4*)(s_p + lds_at(wr + i * 16 + (lane & 15), s * 4 + (lane >> 4)));
-          fq[i] = *(const u32x4*)(s_q + lds_at(wc + i * 16 + (lane & 15), s * 4 + (lane >> 4)));
-        }
+        for (int i = 0; i < kFm; i++) fp[i] = OpP::fragment(lp, wr + i * 16, h * 4);
         #pragma unroll
-        for (int i = 0; i < 4; i++)
+        for (int j = 0; j < kFn; j++) fq[j] = OpQ::fragment(lq, wc + j * 16, h * 4);
+        #pragma unroll
+        for (int i = 0; i < kFm; i++)
           #pragma unroll
-          for (int j = 0; j < 4; j++) acc[i][j] = E::mfma(fq[j], fp[i], acc[i][j]);
+          for (int j = 0; j < kFn; j++) acc[i][j] = E::mfma(fq[j], fp[i], acc[i][j]);
       }
+      if (!kDirect && s + 1 < stages) {
+        sp.store(lds + fill);
+        sq.store(lds + fill + OpP::kBytes);
+      }
+      use = use + OpP::kBytes + OpQ::kBytes == sizeof(lds) ? 0 : use + OpP::kBytes + OpQ::kBytes;
+      fill = fill + OpP::kBytes + OpQ::kBytes == sizeof(lds) ? 0 : fill + OpP::kBytes + OpQ::kBytes;
     }
+    if constexpr (kDirect) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no load into this LDS outlives the workgroup
   }
   // a lane holds row (lane & 15) and four consecutive columns of each 16 x 16 block
   #pragma unroll
-  for (int i = 0; i < 4; i++) {
+  for (int i = 0; i < kFm; i++) {
     const uint32_t row = row0 + wr + i * 16 + (lane & 15);
     if (row >= row_end) continue;
     #pragma unroll
-    for (int j = 0; j < 4; j++) store_four<E, D>(a, out, row, col0 + wc + j * 16 + (lane >> 4) * 4, a.cols, acc[i][j]);
+    for (int j = 0; j < kFn; j++) store_four<E, D>(a, out, row, col0 + wc + j * 16 + (lane >> 4) * 4, a.cols, acc[i][j]);
   }
 }
 
@@ -328,25 +448,71 @@ int check_sizes(const char* what, uint64_t rows, uint64_t cols, uint64_t red, ui
   return ETHA_OK;
 }
 
-template <typename E, uint32_t KIND>
-int run_matmul(const char* what, const MatmulArgs& a, uint64_t row_tiles, uint32_t out_dtype, void* stream) {
-  const uint64_t col_tiles = ((uint64_t)a.cols + kTile - 1) / kTile;
-  const uint64_t blocks = row_tiles * col_tiles;
-  if (blocks >= 1ull << 24) return fail(ETHA_ERR_UNSUPPORTED, "%s: the product is too large for one call", what);
+// Whether an operand's tiles can be brought straight into LDS, see DirectStage.
+bool is_direct(const void* base, int64_t stride, int64_t group_stride, uint64_t k_bytes, bool trans) {
+  return !(((uintptr_t)base | (uint64_t)stride | (uint64_t)group_stride) & 15) && (trans || !(k_bytes & 15)) && stride >= 0 &&
+         stride < 1 << 22;
+}
+
+template <typename E, uint32_t KIND, typename D, typename S>
+int launch_matmul(const char* what, const MatmulArgs& a, uint64_t row_tiles, bool direct, void* stream) {
+  const uint64_t col_tiles = ((uint64_t)a.cols + S::BN - 1) / S::BN, blocks = row_tiles * col_tiles;
+  if (blocks >= 1ull << 22) return fail(ETHA_ERR_UNSUPPORTED, "%s: the product is too large for one call", what);
   if (!blocks) return ETHA_OK;
-  const dim3 grid((uint32_t)blocks), block(256);
-  if (out_dtype == ETHA_F32) hipLaunchKernelGGL((etha_matmul_kernel<E, KIND, F32>), grid, block, 0, (hipStream_t)stream, a);
-  else if (out_dtype == ETHA_BF16) hipLaunchKernelGGL((etha_matmul_kernel<E, KIND, BF16>), grid, block, 0, (hipStream_t)stream, a);
-  else hipLaunchKernelGGL((etha_matmul_kernel<E, KIND, F16>), grid, block, 0, (hipStream_t)stream, a);
+  const dim3 grid((uint32_t)blocks), block(S::kThreads);
+  if (direct) hipLaunchKernelGGL((etha_matmul_kernel<E, KIND, D, S, DirectStage>), grid, block, 0, (hipStream_t)stream, a);
+  else hipLaunchKernelGGL((etha_matmul_kernel<E, KIND, D, S, RegisterStage>), grid, block, 0, (hipStream_t)stream, a);
   return launched("etha_matmul_kernel");
+}
+
+#ifndef SHAPE_L
+#define SHAPE_L 256, 256, 2, 4, 128, 2
+#endif
+#ifndef SHAPE_M
+#define SHAPE_M 128, 128, 2, 2, 128, 3
+#endif
+#ifndef SHAPE_S
+#define SHAPE_S 32, 64, 1, 4, 128, 6
+#endif
+typedef Shape<SHAPE_L> ShapeL;
+typedef Shape<SHAPE_M> ShapeM;
+typedef Shape<SHAPE_S> ShapeS;
+
+// No group wastes more than one row tile, and a group with rows has at least one.
+uint64_t row_tiles_of(const MatmulArgs& a, uint32_t kind, int bm) {
+  if (kind == kPlain) return ((uint64_t)a.rows + bm - 1) / bm;
+  if (kind == kGroupReduce) return ((uint64_t)a.rows + bm - 1) / bm * a.n_groups;
+  const uint64_t groups = (uint64_t)a.n_groups + 2 < a.rows ? a.n_groups + 2 : a.rows;
+  return (a.rows - groups) / bm + groups;
+}
+
+template <typename E, uint32_t KIND, typename D>
+int shaped_matmul(const char* what, const MatmulArgs& a, bool direct, void* stream) {
+  // rows a group has on average: the height of the tiles that it fills
+  const uint64_t rows = KIND == kGroupRows || KIND == kGroupRowsT ? a.rows / (a.n_groups ? a.n_groups : 1) : a.rows;
+  const auto tiles = [&](int bm, int bn) { return row_tiles_of(a, KIND, bm) * (((uint64_t)a.cols + bn - 1) / bn); };
+  if (rows <= 32 && KIND != kGroupReduce)
+    return launch_matmul<E, KIND, D, ShapeS>(what, a, row_tiles_of(a, KIND, ShapeS::BM), direct, stream);
+  if (rows > 128 && tiles(ShapeL::BM, ShapeL::BN) >= 192)
+    return launch_matmul<E, KIND, D, ShapeL>(what, a, row_tiles_of(a, KIND, ShapeL::BM), direct, stream);
+  return launch_matmul<E, KIND, D, ShapeM>(what, a, row_tiles_of(a, KIND, ShapeM::BM), direct, stream);
+}
+
+template <typename E, uint32_t KIND>
+int run_matmul(const char* what, const MatmulArgs& a, uint32_t out_dtype, void* stream) {
+  constexpr bool kTransP = KIND == kGroupReduce, kTransQ = KIND == kGroupReduce || KIND == kGroupRowsT;
+  const uint64_t k_bytes = (uint64_t)a.red * E::kEs;
+  const bool direct = is_direct(a.p, a.p_stride, 0, k_bytes, kTransP) && is_direct(a.q, a.q_stride, a.q_group_stride, k_bytes, kTransQ);
+  if (out_dtype == ETHA_F32) return shaped_matmul<E, KIND, F32>(what, a, direct, stream);
+  if (out_dtype == ETHA_BF16) return shaped_matmul<E, KIND, BF16>(what, a, direct, stream);
+  return shaped_matmul<E, KIND, F16>(what, a, direct, stream);
 }
 
 bool is_out(uint32_t dtype) { return dtype == ETHA_F32 || dtype == ETHA_BF16 || dtype == ETHA_F16; }
 
 template <uint32_t KIND>
-int run_grouped(const char* what, const MatmulArgs& a, uint64_t row_tiles, uint32_t dtype, uint32_t out_dtype, void* stream) {
-  return dtype == ETHA_BF16 ? run_matmul<ElemBF16, KIND>(what, a, row_tiles, out_dtype, stream)
-                            : run_matmul<ElemF16, KIND>(what, a, row_tiles, out_dtype, stream);
+int run_grouped(const char* what, const MatmulArgs& a, uint32_t dtype, uint32_t out_dtype, void* stream) {
+  return dtype == ETHA_BF16 ? run_matmul<ElemBF16, KIND>(what, a, out_dtype, stream) : run_matmul<ElemF16, KIND>(what, a, out_dtype, stream);
 }
 
 int check_groups(const char* what, const void* offsets, uint64_t n_groups, uint32_t dtype, uint32_t out_dtype) {
@@ -382,7 +548,7 @@ int etha_int8_matmul(const int8_t* x, const float* x_scale, uint64_t rows, int64
   a.row_scale = x_scale;
   a.col_scale = w_scale;
   a.bias = bias;
-  return run_matmul<ElemI8, kPlain>("etha_int8_matmul", a, (rows + kTile - 1) / kTile, out_dtype, stream);
+  return run_matmul<ElemI8, kPlain>("etha_int8_matmul", a, out_dtype, stream);
 }
 
 int etha_grouped_matmul(const void* x, uint32_t dtype, uint64_t rows, int64_t x_stride, const void* w, uint64_t n_groups,
@@ -407,11 +573,8 @@ int etha_grouped_matmul(const void* x, uint32_t dtype, uint64_t rows, int64_t x_
   a.offsets = offsets;
   a.n_groups = (uint32_t)n_groups;
   a.zero_rest = zero_rest != 0;
-  // no group wastes more than one tile, and a group with rows has at least one
-  const uint64_t groups = n_groups + 2 < rows ? n_groups + 2 : rows;
-  const uint64_t tiles = (rows - groups) / kTile + groups;
-  return w_transposed ? run_grouped<kGroupRowsT>("etha_grouped_matmul", a, tiles, dtype, out_dtype, stream)
-                      : run_grouped<kGroupRows>("etha_grouped_matmul", a, tiles, dtype, out_dtype, stream);
+  return w_transposed ? run_grouped<kGroupRowsT>("etha_grouped_matmul", a, dtype, out_dtype, stream)
+                      : run_grouped<kGroupRows>("etha_grouped_matmul", a, dtype, out_dtype, stream);
 }
 
 int etha_grouped_matmul_reduce(const void* grad, const void* x, uint32_t dtype, uint64_t rows, int64_t grad_stride, int64_t x_stride,
@@ -435,8 +598,7 @@ int etha_grouped_matmul_reduce(const void* grad, const void* x, uint32_t dtype, 
   a.red = (uint32_t)rows;
   a.offsets = offsets;
   a.n_groups = (uint32_t)n_groups;
-  const uint64_t tiles = (out_rows + kTile - 1) / kTile * n_groups;
-  return run_grouped<kGroupReduce>("etha_grouped_matmul_reduce", a, tiles, dtype, out_dtype, stream);
+  return run_grouped<kGroupReduce>("etha_grouped_matmul_reduce", a, dtype, out_dtype, stream);
 }
 
 }  // extern "C"

@@ -412,7 +412,7 @@ __global__ __launch_bounds__(kGradWaves* kWave) void etha_embedding_join_kernel(
 }
 
 // ---- rows to 8 bits --------------------------------------------------------------------------------------------
-// scale = max|x| / 127 (one correctly rounded division), q = x / scale rounded half to even - of the exact quotient:
+// scale = max|x| * (1 / 127) in fp32, q = x / scale rounded half to even - of the exact quotient:
 // with q0 next to it, r = x - q0 * scale is a multiple of ulp(scale) / 2 below 2 * scale and so an fp32 number, which
 // the fused multiply-add gives exactly; comparing |r| with scale / 2 then settles the rounding.  The row stays in
 // registers between its maximum and its conversion, so it is read once.
@@ -469,7 +469,7 @@ __global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS) void etha_quantize_r
     for (int w = 0; w < kWaves; w++) top = s_max[w] > top ? s_max[w] : top;
   }
   if (!there) return;
-  const float scale = __builtin_bit_cast(float, top) / 127.f;
+  const float scale = __builtin_bit_cast(float, top) * (1.f / 127.f);
   const bool none = !(scale > 0.f) || top >= 0x7f800000u;  // a row of zeros, or one that holds an infinity or NaN
   // a scale below the smallest normal number may have no finite inverse: the quotient is formed by division there
   const bool tiny = scale < 1.2e-38f;

@@ -19,7 +19,7 @@ def quantize_rows(x: torch.Tensor, *, values: torch.Tensor | None = None,
                   scales: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """Rows of ``x`` (its last dim) in 8 bits: ``(values int8, scales fp32)`` with ``x ~ values * scales[..., None]``.
 
-    ``scales`` is the row's largest magnitude over 127; values are rounded half to even and lie within +-127.  A row of
+    ``scales`` is the row's largest magnitude times 1 / 127 in fp32; values are rounded half to even and lie within +-127.  A row of
     zeros has scale 0; a row that holds a NaN or an infinity has that as its scale and zeros as values.  ``values`` and
     ``scales`` may be given to be written.
     """

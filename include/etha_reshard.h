@@ -353,7 +353,7 @@ int etha_embedding_grad(const void* grad, uint32_t grad_dtype, int64_t grad_stri
                         void* stream);
 
 /*
- * Rows to 8 bits: scales[r] = max |x[r,:]| / 127, values[r,k] = x[r,k] / scales[r] rounded half to even (the exact
+ * Rows to 8 bits: scales[r] = max |x[r,:]| * (1 / 127) in fp32, values[r,k] = x[r,k] / scales[r] rounded half to even (the exact
  * quotient; within +-127), 0 where the scale is 0.  A row that holds a NaN or an infinity gets that as its scale and
  * zeros as its values.
  */

@@ -1,6 +1,6 @@
 """Rows in 8 bits and the product of 8-bit rows, against plain forms in 64 bits.
 
-Tolerances.  Values in 8 bits are integers and compared as such; a scale is one correctly rounded division.  The product's
+Tolerances.  Values in 8 bits are integers and compared as such; a scale is one fp32 product.  The product's
 integer sum is exact; fp32 rounds it, the product of the two scales, their product and the sum with the bias: four
 roundings of at most 2^-24 of |product| + |bias|, then half a step of the result's type.
 """
@@ -16,7 +16,7 @@ DTYPES = [torch.float32, torch.bfloat16, torch.float16]
 
 def plain_rows(x):
     x = x.cpu()
-    scale = x.abs().amax(-1).float() / 127
+    scale = x.abs().amax(-1).float() * (torch.ones(()) / 127)
     fine = scale.isfinite() & (scale > 0)
     quotient = x.double() / torch.where(fine, scale, torch.ones(())).double()[..., None]
     q = torch.where(fine[..., None], quotient.nan_to_num().round().clamp(-127, 127), 0.0)
@@ -113,7 +113,7 @@ def test_rows(gpu_device, rows, width, dtype):
 def test_rounding_of_halves(gpu_device):
     """Quotients at and next to a half: with a scale that is a power of two halves are exact, with others they are near."""
     for top in (127.0, 254.0, 63.5, 127.0 * 1.0009765625, 100.0, 3e-37, 127 * 2.0 ** -126, 3e-40, 127 * 2.0 ** -149, 2.0 ** -149, 3e38):
-        scale = torch.tensor(top, dtype=torch.float32) / 127
+        scale = torch.tensor(top, dtype=torch.float32) * (torch.ones(()) / 127)
         n = torch.arange(-127, 127, dtype=torch.float64) + 0.5
         near = (n * scale.double()).float()
         x = torch.cat([near, torch.nextafter(near, torch.tensor(1e30)), torch.nextafter(near, torch.tensor(-1e30)), torch.tensor([top, -top])])
