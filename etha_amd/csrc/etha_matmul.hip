@@ -6,6 +6,7 @@
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
+#include <type_traits>
 
 #include "etha_device.h"
 #include "etha_internal.h"
@@ -214,21 +215,23 @@ struct DirectStage {
     k_byte = OP::piece_of(threadIdx.x) * 16;
     wave_at = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * 1024;
   }
-  // The stage that begins at k0, into LDS; past the end of k it brings zeros.
-  __device__ void load(char* lds, uint32_t k0, uint32_t red) {
+  // The stage that begins at k0, into LDS, in kPer parts; past the end of k it brings zeros.
+  u32x4 rsrc;
+  uint32_t to, outside;
+  __device__ void begin(char* lds, uint32_t k0, uint32_t red) {
     const uint64_t b = (uint64_t)base;
     const uint32_t size = left > 0x7fffffff ? 0x7fffffffu : left < 0 ? 0u : (uint32_t)left;
-    const u32x4 rsrc = {(uint32_t)b, (uint32_t)(b >> 32) & 0xffffu, size, 0x00020000u};
-    const uint32_t to = lds_address(lds) + wave_at;
-    uint32_t outside = 0;
+    rsrc = u32x4{(uint32_t)b, (uint32_t)(b >> 32) & 0xffffu, size, 0x00020000u};
+    to = lds_address(lds) + wave_at;
+    outside = 0;
     if constexpr (!OP::kTrans) outside = (int64_t)k_byte >= ((int64_t)red - (int64_t)k0) * OP::kEs ? kOutside : 0;
-    #pragma unroll
-    for (int i = 0; i < OP::kPer; i++)
-      asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
-                   :: "s"(to + i * OP::kThreads * 16), "v"(at[i] | outside), "s"(rsrc) : "memory");
     const int64_t step = OP::kTrans ? (int64_t)OP::kStageK * stride : (int64_t)OP::kStageK * OP::kEs;
     base += step;
     left -= step;
+  }
+  __device__ void part(int i) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+                 :: "s"(to + i * OP::kThreads * 16), "v"(at[i] | outside), "s"(rsrc) : "memory");
   }
   __device__ void store(char*) const {}
 };
@@ -265,17 +268,18 @@ struct RegisterStage {
     stride = row_stride;
     n_rows = n_rows_;
   }
-  __device__ void load(char*, uint32_t k0, uint32_t red) {
-    const bool whole = k0 + OP::kStageK <= red;
-    #pragma unroll
-    for (int i = 0; i < OP::kPer; i++) {
-      const uint32_t slot = threadIdx.x + i * OP::kThreads, row = OP::row_of(slot), piece = OP::piece_of(slot);
-      if constexpr (!OP::kTrans) {
-        const char* p = base + (int64_t)(row < n_rows ? row : n_rows - 1) * stride + (int64_t)k0 * OP::kEs + piece * 16;
-        v[i] = whole ? load_raw<16>(p) : load_part<OP::kEs>(p, ((int64_t)red - k0) * OP::kEs - piece * 16);
-      } else {  // memory row = k, a piece holds 8 tile rows
-        v[i] = load_part<OP::kEs>(base + (int64_t)(k0 + row) * stride + piece * 16, k0 + row < red ? ((int64_t)n_rows - piece * 8) * 2 : 0);
-      }
+  uint32_t k0, red;
+  __device__ void begin(char*, uint32_t k0_, uint32_t red_) {
+    k0 = k0_;
+    red = red_;
+  }
+  __device__ void part(int i) {
+    const uint32_t slot = threadIdx.x + i * OP::kThreads, row = OP::row_of(slot), piece = OP::piece_of(slot);
+    if constexpr (!OP::kTrans) {
+      const char* p = base + (int64_t)(row < n_rows ? row : n_rows - 1) * stride + (int64_t)k0 * OP::kEs + piece * 16;
+      v[i] = k0 + OP::kStageK <= red ? load_raw<16>(p) : load_part<OP::kEs>(p, ((int64_t)red - k0) * OP::kEs - piece * 16);
+    } else {  // memory row = k, a piece holds 8 tile rows
+      v[i] = load_part<OP::kEs>(base + (int64_t)(k0 + row) * stride + piece * 16, k0 + row < red ? ((int64_t)n_rows - piece * 8) * 2 : 0);
     }
   }
   __device__ void store(char* lds) const {
@@ -284,31 +288,10 @@ struct RegisterStage {
   }
 };
 
-// ---- one element of the result -----------------------------------------------------------------------------------
-template <typename E, typename D>
-__device__ inline void store_four(const MatmulArgs& a, typename D::bits* out, uint32_t row, uint32_t col, uint32_t cols,
-                                  typename E::acc acc) {
-  float v[4];
-  if constexpr (E::kEs == 1) {  // the integer sum is exact; one product of scales, as the definition has it
-    const float rs = a.row_scale[row];
-    #pragma unroll
-    for (int i = 0; i < 4; i++) {
-      v[i] = 0.f;
-      if (col + i < cols) {
-        v[i] = (float)acc[i] * (rs * a.col_scale[col + i]);
-        if (a.bias) v[i] += a.bias[col + i];
-      }
-    }
-  } else {
-    #pragma unroll
-    for (int i = 0; i < 4; i++) v[i] = acc[i];
-  }
-  if (col < cols) store_f32<D, 4>(out + (int64_t)row * a.out_stride + col, v, (int64_t)cols - col);
-}
-
 // ---- the tile kernel -----------------------------------------------------------------------------------------------
-// A tile of BM rows and BN columns, WM x WN waves, STAGES stages of BKB bytes of k in LDS.  One barrier a stage: behind it
-// every wave has finished the stage before, whose LDS the stage STAGES - 1 ahead may then take.
+// A tile of BM rows and BN columns, WM x WN waves, STAGES stages of BKB bytes of k in LDS.  The fragments of the next half
+// of a stage are read while the matrix units work on this one's.  One barrier a stage, in front of its last half: every
+// wave then has all it needs of the stage in registers, so that its LDS can take a stage further on.
 template <int BM_, int BN_, int WM_, int WN_, int BKB_, int STAGES_>
 struct Shape {
   static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, BKB = BKB_, STAGES = STAGES_;
@@ -380,57 +363,122 @@ __global__ __launch_bounds__(S::kThreads) void etha_matmul_kernel(const MatmulAr
     STAGE<OpQ> sq;
     sp.init(p, a.p_stride, n_rows, red);
     sq.init(q, a.q_stride, n_cols, red);
-    constexpr int kAhead = kDirect ? kStages - 1 : 1;
-    #pragma unroll
-    for (int s = 0; s < kAhead; s++) {
-      char* to = lds + s * (OpP::kBytes + OpQ::kBytes);
-      sp.load(to, s * kStageK, red);
-      sq.load(to + OpP::kBytes, s * kStageK, red);
-    }
-    if constexpr (!kDirect) {
+    constexpr uint32_t kStageBytes = OpP::kBytes + OpQ::kBytes;
+    constexpr int kHalves = S::BKB / 64;
+    uint32_t next = 0;  // the first stage that is not on its way yet
+    const auto begin = [&](char* to) {
+      sp.begin(to, next * kStageK, red);
+      sq.begin(to + OpP::kBytes, next * kStageK, red);
+      next++;
+    };
+    constexpr int kParts = OpP::kPer + OpQ::kPer;
+    const auto part = [&](int t) {
+      if (t < OpP::kPer) sp.part(t);
+      else sq.part(t - OpP::kPer);
+    };
+    const auto load = [&](char* to) {
+      begin(to);
+      #pragma unroll
+      for (int t = 0; t < kParts; t++) part(t);
+    };
+    u32x4 fp[2][kFm], fq[2][kFn];
+    constexpr int kReads = kFm + kFn;
+    const auto read = [&](int set, const char* from, int half, int t) {
+      if (t < kFn) fq[set][t] = OpQ::fragment(from + OpP::kBytes, wc + t * 16, half * 4);
+      else fp[set][t - kFn] = OpP::fragment(from, wr + (t - kFn) * 16, half * 4);
+    };
+    load(lds);
+    if constexpr (kDirect) {
+      #pragma unroll
+      for (int s = 1; s < kStages; s++) load(lds + s * kStageBytes);
+      wait_stage<(kStages - 1) * kParts>();
+    } else {
       sp.store(lds);
       sq.store(lds + OpP::kBytes);
+      load(nullptr);
+      __syncthreads();
     }
-    uint32_t use = 0, fill = kAhead * (OpP::kBytes + OpQ::kBytes);
+    #pragma unroll
+    for (int t = 0; t < kReads; t++) read(0, lds, 0, t);
+    uint32_t use = 0;
     for (uint32_t s = 0; s < stages; s++) {
-      if constexpr (kDirect) wait_stage<(kStages - 2) * (OpP::kPer + OpQ::kPer)>();
-      else __syncthreads();
-      // past the last stage these bring zeros that nobody reads: the count of loads stays the same
-      if (kDirect || s + 1 < stages) {
-        sp.load(lds + fill, (s + kAhead) * kStageK, red);
-        sq.load(lds + fill + OpP::kBytes, (s + kAhead) * kStageK, red);
-      }
-      const char* lp = lds + use;
-      const char* lq = lp + OpP::kBytes;
+      const uint32_t then = use + kStageBytes == sizeof(lds) ? 0 : use + kStageBytes;
+      static_assert(kHalves % 2 == 0, "an odd number of halves would change the sets' places every stage");
       #pragma unroll
-      for (int h = 0; h < S::BKB / 64; h++) {
-        u32x4 fp[kFm], fq[kFn];
+      for (int h = 0; h < kHalves; h++) {
+        const bool last = h + 1 == kHalves;
+        if (last) {
+          if constexpr (kDirect) {
+            wait_stage<(kStages - 2) * kParts>();
+            begin(lds + use);  // past the end of k it brings zeros: the count of loads stays the same
+          } else {
+            sp.store(lds + then);
+            sq.store(lds + then + OpP::kBytes);
+            __syncthreads();
+            begin(nullptr);
+          }
+        }
+        // a row of matrix instructions, the next half's fragments and the loads of a stage further on, in turn: issued in
+        // a row each of them would hold up the others
         #pragma unroll
-        for (int i = 0; i < kFm; i++) fp[i] = OpP::fragment(lp, wr + i * 16, h * 4);
-        #pragma unroll
-        for (int j = 0; j < kFn; j++) fq[j] = OpQ::fragment(lq, wc + j * 16, h * 4);
-        #pragma unroll
-        for (int i = 0; i < kFm; i++)
+        for (int i = 0; i < kFm; i++) {
           #pragma unroll
-          for (int j = 0; j < kFn; j++) acc[i][j] = E::mfma(fq[j], fp[i], acc[i][j]);
+          for (int t = i * kReads / kFm; t < (i + 1) * kReads / kFm; t++)
+            read((h + 1) & 1, lds + (last ? then : use), last ? 0 : h + 1, t);
+          #pragma unroll
+          for (int j = 0; j < kFn; j++) acc[i][j] = E::mfma(fq[h & 1][j], fp[h & 1][i], acc[i][j]);
+          if (last) {
+            #pragma unroll
+            for (int t = i * kParts / kFm; t < (i + 1) * kParts / kFm; t++) part(t);
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        }
       }
-      if (!kDirect && s + 1 < stages) {
-        sp.store(lds + fill);
-        sq.store(lds + fill + OpP::kBytes);
-      }
-      use = use + OpP::kBytes + OpQ::kBytes == sizeof(lds) ? 0 : use + OpP::kBytes + OpQ::kBytes;
-      fill = fill + OpP::kBytes + OpQ::kBytes == sizeof(lds) ? 0 : fill + OpP::kBytes + OpQ::kBytes;
+      use = then;
     }
     if constexpr (kDirect) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no load into this LDS outlives the workgroup
   }
   // a lane holds row (lane & 15) and four consecutive columns of each 16 x 16 block
-  #pragma unroll
-  for (int i = 0; i < kFm; i++) {
-    const uint32_t row = row0 + wr + i * 16 + (lane & 15);
-    if (row >= row_end) continue;
+  const uint32_t row_first = row0 + wr + (lane & 15), col_first = col0 + wc + (lane >> 4) * 4;
+  float col_scale[kFn][4], bias[kFn][4];
+  if constexpr (E::kEs == 1) {
     #pragma unroll
-    for (int j = 0; j < kFn; j++) store_four<E, D>(a, out, row, col0 + wc + j * 16 + (lane >> 4) * 4, a.cols, acc[i][j]);
+    for (int j = 0; j < kFn; j++)
+      #pragma unroll
+      for (int c = 0; c < 4; c++) {
+        const uint32_t col = col_first + j * 16 + c < a.cols ? col_first + j * 16 + c : a.cols - 1;
+        col_scale[j][c] = a.col_scale[col];
+        bias[j][c] = a.bias ? a.bias[col] : 0.f;
+      }
   }
+  const auto store_tile = [&](auto whole) {
+    #pragma unroll
+    for (int i = 0; i < kFm; i++) {
+      const uint32_t row = row_first + i * 16;
+      if (!whole && row >= row_end) continue;
+      typename D::bits* to = out + (int64_t)row * a.out_stride + col_first;
+      float row_scale = 1.f;
+      if constexpr (E::kEs == 1) row_scale = a.row_scale[row];
+      #pragma unroll
+      for (int j = 0; j < kFn; j++) {
+        float v[4];
+        #pragma unroll
+        for (int c = 0; c < 4; c++) {
+          // the integer sum is exact; one product of scales, as the definition has it
+          if constexpr (E::kEs == 1) {
+            v[c] = (float)acc[i][j][c] * (row_scale * col_scale[j][c]);
+            if (a.bias) v[c] += bias[j][c];
+          } else {
+            v[c] = acc[i][j][c];
+          }
+        }
+        if (whole) store_f32<D, 4>(to + j * 16, v, 4);
+        else store_f32<D, 4>(to + j * 16, v, (int64_t)a.cols - (col_first + j * 16));
+      }
+    }
+  };
+  if (row0 + S::BM <= row_end && col0 + S::BN <= a.cols) store_tile(std::true_type{});
+  else store_tile(std::false_type{});
 }
 
 int launched(const char* name) {
