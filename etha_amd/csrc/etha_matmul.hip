@@ -316,12 +316,18 @@ __global__ __launch_bounds__(S::kThreads) void etha_matmul_kernel(const MatmulAr
   // Workgroups go to the 8 XCDs in turn: each XCD takes a run of the tiles, so that its L2 sees operands again.  In a run
   // the tiles go down bands of kBand row tiles.
   constexpr uint32_t kBand = 4;
-  uint32_t id = blockIdx.x;
+  // Groups of a sum over their rows cost as much as they have rows: there every XCD takes a run of every group's tiles.
+  const uint32_t runs = KIND == kGroupReduce ? a.n_groups : 1, n = gridDim.x / runs;
+  uint32_t id = blockIdx.x, first = 0;
+  if (KIND == kGroupReduce) {
+    first = id / n * n;
+    id -= first;
+  }
   {
-    const uint32_t n = gridDim.x, xcd = id & 7, each = n >> 3, more = n & 7;
+    const uint32_t xcd = id & 7, each = n >> 3, more = n & 7;
     id = xcd * each + (xcd < more ? xcd : more) + (id >> 3);
   }
-  const uint32_t row_tiles_all = gridDim.x / col_tiles, band = id / (kBand * col_tiles);
+  const uint32_t row_tiles_all = n / col_tiles, band = id / (kBand * col_tiles);
   const uint32_t in_band = row_tiles_all - band * kBand < kBand ? row_tiles_all - band * kBand : kBand;
   const uint32_t row_id = band * kBand + (id - band * kBand * col_tiles) % in_band;
   const uint32_t col0 = (id - band * kBand * col_tiles) / in_band * S::BN;
@@ -333,14 +339,14 @@ __global__ __launch_bounds__(S::kThreads) void etha_matmul_kernel(const MatmulAr
     row0 = row_id * S::BM;
     row_end = a.rows;
   } else if constexpr (KIND == kGroupReduce) {
-    const uint32_t row_tiles = (a.rows + S::BM - 1) / S::BM, group = row_id / row_tiles;
+    const uint32_t group = first / n;
     uint32_t lo, hi;
     group_bounds(a, group, &lo, &hi);
     red = hi - lo;
     p += (int64_t)lo * a.p_stride;
     q += (int64_t)lo * a.q_stride;
     out += (int64_t)group * a.out_group_stride;
-    row0 = row_id % row_tiles * S::BM;
+    row0 = row_id * S::BM;
     row_end = a.rows;
   } else {
     const GroupTile t = find_tile<S::BM>(a, row_id);
@@ -401,12 +407,15 @@ __global__ __launch_bounds__(S::kThreads) void etha_matmul_kernel(const MatmulAr
     #pragma unroll
     for (int t = 0; t < kReads; t++) read(0, lds, 0, t);
     uint32_t use = 0;
-    for (uint32_t s = 0; s < stages; s++) {
-      const uint32_t then = use + kStageBytes == sizeof(lds) ? 0 : use + kStageBytes;
-      static_assert(kHalves % 2 == 0, "an odd number of halves would change the sets' places every stage");
+    // Two halves an iteration, so that the sets of fragments keep their names; where that is two stages and their number is
+    // odd, the last half multiplies the zeros past the end of k.
+    constexpr int kStagesIter = kHalves == 1 ? 2 : 1;
+    for (uint32_t s = 0; s < stages; s += kStagesIter) {
+      static_assert(kHalves <= 2, "two halves an iteration");
       #pragma unroll
-      for (int h = 0; h < kHalves; h++) {
-        const bool last = h + 1 == kHalves;
+      for (int h = 0; h < 2; h++) {
+        const bool last = kHalves == 1 || h == 1;  // of its stage
+        const uint32_t then = use + kStageBytes == sizeof(lds) ? 0 : use + kStageBytes;
         if (last) {
           if constexpr (kDirect) {
             wait_stage<(kStages - 2) * kParts>();
@@ -424,7 +433,7 @@ __global__ __launch_bounds__(S::kThreads) void etha_matmul_kernel(const MatmulAr
         for (int i = 0; i < kFm; i++) {
           #pragma unroll
           for (int t = i * kReads / kFm; t < (i + 1) * kReads / kFm; t++)
-            read((h + 1) & 1, lds + (last ? then : use), last ? 0 : h + 1, t);
+            read((h + 1) & 1, lds + (last ? then : use), last ? 0 : 1, t);
           #pragma unroll
           for (int j = 0; j < kFn; j++) acc[i][j] = E::mfma(fq[h & 1][j], fp[h & 1][i], acc[i][j]);
           if (last) {
@@ -433,8 +442,8 @@ __global__ __launch_bounds__(S::kThreads) void etha_matmul_kernel(const MatmulAr
           }
           __builtin_amdgcn_sched_barrier(0);
         }
+        if (last) use = then;
       }
-      use = then;
     }
     if constexpr (kDirect) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no load into this LDS outlives the workgroup
   }
