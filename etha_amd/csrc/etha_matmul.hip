@@ -144,27 +144,27 @@ __device__ inline void group_bounds(const MatmulArgs& a, uint32_t group, uint32_
 }
 
 // ---- staging -------------------------------------------------------------------------------------------------------
-// A stage holds BKB bytes of k of both operands.  Where an operand lies k-contiguous in memory its LDS tile is ROWS rows of
-// BKB bytes, read 16 bytes of k a lane; where it lies transposed (16-bit elements) the tile is the memory's own [k][ROWS],
+// A stage holds kStageBytes of k of both operands.  Where an operand lies k-contiguous in memory its LDS tile is ROWS rows
+// of kStageBytes, read 16 bytes of k a lane; where it lies transposed (16-bit elements) the tile is the memory's own [k][ROWS],
 // read with the transposing LDS load, which hands each of 16 lanes four k of one column.  Either tile is a sequence of
 // 16-byte slots; which piece of memory a slot holds is permuted so that the lanes of one read touch all banks: by the row
 // where 16 rows are read at one k, in 32-byte column groups by (k & 3, k >> 3) where 8 rows of k are read at one column.
+constexpr int kStageBytes = 128;            // whole lines of memory: 64-byte pieces of rows were 10 % slower
 constexpr uint32_t kOutside = 0x80000000u;  // an offset that no operand's tile reaches: reads there give zeros
 
-template <typename E, bool TRANS_, int ROWS, int BKB, int THREADS_>
+template <typename E, bool TRANS_, int ROWS, int THREADS_>
 struct Operand {
   static constexpr bool kTrans = TRANS_;
   static constexpr int kEs = E::kEs, kThreads = THREADS_;
-  static constexpr int kStageK = BKB / kEs;
-  static constexpr int kBytes = ROWS * BKB, kSlots = kBytes / 16, kPer = kSlots / kThreads;
-  static constexpr int kPieces = kTrans ? ROWS / 8 : BKB / 16;  // slots of an LDS row
+  static constexpr int kStageK = kStageBytes / kEs;
+  static constexpr int kBytes = ROWS * kStageBytes, kSlots = kBytes / 16, kPer = kSlots / kThreads;
+  static constexpr int kPieces = kTrans ? ROWS / 8 : kStageBytes / 16;  // slots of an LDS row
   static_assert(kSlots % kThreads == 0 && kPer > 0, "every work-item stages the same number of slots");
 
   static __device__ uint32_t row_of(uint32_t slot) { return slot / kPieces; }
   static __device__ uint32_t swizzle(uint32_t row, uint32_t piece) {
     if constexpr (kTrans) return piece ^ ((((row & 3) | ((row >> 1) & 4)) << 1) & (kPieces - 1));
-    else if constexpr (kPieces == 8) return piece ^ (row & 7);
-    else return piece ^ ((row >> 2) & 3);
+    else return piece ^ (row & 7);
   }
   static __device__ uint32_t piece_of(uint32_t slot) { return swizzle(row_of(slot), slot % kPieces); }
 
@@ -173,7 +173,7 @@ struct Operand {
     const uint32_t lane = threadIdx.x & 63;
     if constexpr (!kTrans) {
       const uint32_t r = r0 + (lane & 15);
-      return *(const u32x4*)(lds + r * BKB + swizzle(r, kp0 + (lane >> 4)) * 16);
+      return *(const u32x4*)(lds + r * kStageBytes + swizzle(r, kp0 + (lane >> 4)) * 16);
     } else {
       typedef short s16x4 __attribute__((ext_vector_type(4)));
       typedef __attribute__((address_space(3))) s16x4* lds_ptr;
@@ -279,7 +279,9 @@ struct RegisterStage {
       const char* p = base + (int64_t)(row < n_rows ? row : n_rows - 1) * stride + (int64_t)k0 * OP::kEs + piece * 16;
       v[i] = k0 + OP::kStageK <= red ? load_raw<16>(p) : load_part<OP::kEs>(p, ((int64_t)red - k0) * OP::kEs - piece * 16);
     } else {  // memory row = k, a piece holds 8 tile rows
-      v[i] = load_part<OP::kEs>(base + (int64_t)(k0 + row) * stride + piece * 16, k0 + row < red ? ((int64_t)n_rows - piece * 8) * 2 : 0);
+      const char* p = base + (int64_t)(k0 + row) * stride + piece * 16;
+      v[i] = k0 + OP::kStageK <= red && n_rows * 2 == OP::kPieces * 16 ? load_raw<16>(p)
+                 : load_part<OP::kEs>(p, k0 + row < red ? ((int64_t)n_rows - piece * 8) * 2 : 0);
     }
   }
   __device__ void store(char* lds) const {
@@ -289,12 +291,12 @@ struct RegisterStage {
 };
 
 // ---- the tile kernel -----------------------------------------------------------------------------------------------
-// A tile of BM rows and BN columns, WM x WN waves, STAGES stages of BKB bytes of k in LDS.  The fragments of the next half
-// of a stage are read while the matrix units work on this one's.  One barrier a stage, in front of its last half: every
-// wave then has all it needs of the stage in registers, so that its LDS can take a stage further on.
-template <int BM_, int BN_, int WM_, int WN_, int BKB_, int STAGES_>
+// A tile of BM rows and BN columns, WM x WN waves, STAGES stages of kStageBytes of k in LDS.  The fragments of the next
+// half of a stage are read while the matrix units work on this one's.  One barrier a stage, in front of its second half:
+// every wave then has all it needs of the stage in registers, so that its LDS can take a stage further on.
+template <int BM_, int BN_, int WM_, int WN_, int STAGES_>
 struct Shape {
-  static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, BKB = BKB_, STAGES = STAGES_;
+  static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, STAGES = STAGES_;
   static constexpr int kThreads = WM * WN * 64;
 };
 
@@ -303,100 +305,113 @@ __device__ inline void wait_stage() {  // at most N loads into LDS outstanding; 
   asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" :: "n"(N) : "memory");
 }
 
-template <typename E, uint32_t KIND, typename D, typename S, template <typename> class STAGE>
-__global__ __launch_bounds__(S::kThreads) void etha_matmul_kernel(const MatmulArgs a) {
-  typedef Operand<E, KIND == kGroupReduce, S::BM, S::BKB, S::kThreads> OpP;
-  typedef Operand<E, KIND == kGroupReduce || KIND == kGroupRowsT, S::BN, S::BKB, S::kThreads> OpQ;
-  constexpr bool kDirect = STAGE<OpP>::kDirect;
-  constexpr int kStages = kDirect ? S::STAGES : 2, kFm = S::BM / S::WM / 16, kFn = S::BN / S::WN / 16;
-  constexpr uint32_t kStageK = OpP::kStageK;
-  __shared__ __align__(1024) char lds[kStages * (OpP::kBytes + OpQ::kBytes)];
-  const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+struct Tile {
+  const char *p, *q;
+  int64_t out;  // offset of its group's results, in elements
+  uint32_t row0, row_end, col0;
+  uint32_t red;  // 0 also for rows of no group: they become zeros
+  bool there;
+};
+
+// This workgroup's tile.
+template <typename E, uint32_t KIND, typename S>
+__device__ inline Tile locate(const MatmulArgs& a) {
+  constexpr bool kTransP = KIND == kGroupReduce, kTransQ = KIND == kGroupReduce || KIND == kGroupRowsT;
+  Tile t = {};
+  t.there = true;
+  uint32_t id = blockIdx.x;
   const uint32_t col_tiles = (a.cols + S::BN - 1) / S::BN;
   // Workgroups go to the 8 XCDs in turn: each XCD takes a run of the tiles, so that its L2 sees operands again.  In a run
-  // the tiles go down bands of kBand row tiles.
+  // the tiles go down bands of kBand row tiles.  Groups of a sum over their rows cost as much as they have rows: there every
+  // XCD takes a run of every group's tiles.
   constexpr uint32_t kBand = 4;
-  // Groups of a sum over their rows cost as much as they have rows: there every XCD takes a run of every group's tiles.
-  const uint32_t runs = KIND == kGroupReduce ? a.n_groups : 1, n = gridDim.x / runs;
-  uint32_t id = blockIdx.x, first = 0;
-  if (KIND == kGroupReduce) {
-    first = id / n * n;
-    id -= first;
-  }
-  {
-    const uint32_t xcd = id & 7, each = n >> 3, more = n & 7;
-    id = xcd * each + (xcd < more ? xcd : more) + (id >> 3);
-  }
-  const uint32_t row_tiles_all = n / col_tiles, band = id / (kBand * col_tiles);
-  const uint32_t in_band = row_tiles_all - band * kBand < kBand ? row_tiles_all - band * kBand : kBand;
-  const uint32_t row_id = band * kBand + (id - band * kBand * col_tiles) % in_band;
-  const uint32_t col0 = (id - band * kBand * col_tiles) / in_band * S::BN;
-  uint32_t row0, row_end, red = a.red;
-  const char *p = a.p, *q = a.q;
-  typename D::bits* out = (typename D::bits*)a.out;
-  bool zero = false;
-  if constexpr (KIND == kPlain) {
-    row0 = row_id * S::BM;
-    row_end = a.rows;
-  } else if constexpr (KIND == kGroupReduce) {
-    const uint32_t group = first / n;
+  const uint32_t n = KIND == kGroupReduce ? gridDim.x / a.n_groups : gridDim.x;
+  const uint32_t group = KIND == kGroupReduce ? id / n : 0;
+  id -= group * n;
+  const uint32_t xcd = id & 7, each = n >> 3, more = n & 7;
+  id = xcd * each + (xcd < more ? xcd : more) + (id >> 3);
+  const uint32_t row_tiles = n / col_tiles, band = id / (kBand * col_tiles);
+  const uint32_t in_band = row_tiles - band * kBand < kBand ? row_tiles - band * kBand : kBand;
+  id -= band * kBand * col_tiles;
+  const uint32_t row_id = band * kBand + id % in_band;
+  t.col0 = id / in_band * S::BN;
+  t.p = a.p;
+  t.q = a.q;
+  t.red = a.red;
+  t.row0 = row_id * S::BM;
+  t.row_end = a.rows;
+  if constexpr (KIND == kGroupReduce) {
     uint32_t lo, hi;
     group_bounds(a, group, &lo, &hi);
-    red = hi - lo;
-    p += (int64_t)lo * a.p_stride;
-    q += (int64_t)lo * a.q_stride;
-    out += (int64_t)group * a.out_group_stride;
-    row0 = row_id * S::BM;
-    row_end = a.rows;
-  } else {
-    const GroupTile t = find_tile<S::BM>(a, row_id);
-    if (!t.found) return;
-    row0 = t.lo + t.tile * S::BM;
-    row_end = t.hi;
-    zero = t.group == a.n_groups;
-    if (!zero) q += (int64_t)t.group * a.q_group_stride;
+    t.red = hi - lo;
+    t.p += (int64_t)lo * a.p_stride;
+    t.q += (int64_t)lo * a.q_stride;
+    t.out = (int64_t)group * a.out_group_stride;
+  } else if constexpr (KIND != kPlain) {
+    const GroupTile g = find_tile<S::BM>(a, row_id);
+    t.there = g.found;
+    t.row0 = g.lo + g.tile * S::BM;
+    t.row_end = g.hi;
+    if (g.group == a.n_groups) t.red = 0;
+    else t.q += (int64_t)g.group * a.q_group_stride;
   }
-  const uint32_t n_rows = row_end - row0 < S::BM ? row_end - row0 : S::BM;
-  const uint32_t n_cols = a.cols - col0 < S::BN ? a.cols - col0 : S::BN;
-  p += OpP::kTrans ? (int64_t)row0 * E::kEs : (int64_t)row0 * a.p_stride;
-  q += OpQ::kTrans ? (int64_t)col0 * E::kEs : (int64_t)col0 * a.q_stride;
+  t.p += kTransP ? (int64_t)t.row0 * E::kEs : (int64_t)t.row0 * a.p_stride;
+  t.q += kTransQ ? (int64_t)t.col0 * E::kEs : (int64_t)t.col0 * a.q_stride;
+  return t;
+}
 
-  typename E::acc acc[kFm][kFn] = {};
+template <typename E, uint32_t KIND, typename D, typename S, template <typename> class STAGE>
+__global__ __launch_bounds__(S::kThreads) void etha_matmul_kernel(const MatmulArgs a) {
+  typedef Operand<E, KIND == kGroupReduce, S::BM, S::kThreads> OpP;
+  typedef Operand<E, KIND == kGroupReduce || KIND == kGroupRowsT, S::BN, S::kThreads> OpQ;
+  constexpr bool kDirect = STAGE<OpP>::kDirect;
+  constexpr int kStages = kDirect ? S::STAGES : 2, kFm = S::BM / S::WM / 16, kFn = S::BN / S::WN / 16;
+  constexpr uint32_t kStageK = OpP::kStageK, kBytes = OpP::kBytes + OpQ::kBytes;
+  __shared__ __align__(1024) char lds[kStages * kBytes];
+  const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const uint32_t wr = wave / S::WN * (S::BM / S::WM), wc = wave % S::WN * (S::BN / S::WN);
-  const uint32_t stages = zero ? 0 : (red + kStageK - 1) / kStageK;
-  if (stages) {
-    STAGE<OpP> sp;
-    STAGE<OpQ> sq;
-    sp.init(p, a.p_stride, n_rows, red);
-    sq.init(q, a.q_stride, n_cols, red);
-    constexpr uint32_t kStageBytes = OpP::kBytes + OpQ::kBytes;
-    constexpr int kHalves = S::BKB / 64;
-    uint32_t next = 0;  // the first stage that is not on its way yet
-    const auto begin = [&](char* to) {
-      sp.begin(to, next * kStageK, red);
-      sq.begin(to + OpP::kBytes, next * kStageK, red);
-      next++;
-    };
-    constexpr int kParts = OpP::kPer + OpQ::kPer;
-    const auto part = [&](int t) {
-      if (t < OpP::kPer) sp.part(t);
-      else sq.part(t - OpP::kPer);
-    };
-    const auto load = [&](char* to) {
-      begin(to);
-      #pragma unroll
-      for (int t = 0; t < kParts; t++) part(t);
-    };
-    u32x4 fp[2][kFm], fq[2][kFn];
-    constexpr int kReads = kFm + kFn;
-    const auto read = [&](int set, const char* from, int half, int t) {
-      if (t < kFn) fq[set][t] = OpQ::fragment(from + OpP::kBytes, wc + t * 16, half * 4);
-      else fp[set][t - kFn] = OpP::fragment(from, wr + (t - kFn) * 16, half * 4);
-    };
+
+  const Tile tile = locate<E, KIND, S>(a);
+  if (!tile.there) return;
+  STAGE<OpP> sp;
+  STAGE<OpQ> sq;
+  {
+    const uint32_t n_rows = tile.row_end - tile.row0, n_cols = a.cols - tile.col0;
+    sp.init(tile.p, a.p_stride, n_rows < S::BM ? n_rows : S::BM, tile.red);
+    sq.init(tile.q, a.q_stride, n_cols < S::BN ? n_cols : S::BN, tile.red);
+  }
+  uint32_t next = 0;  // k of the first stage that is not on its way yet
+  const auto begin = [&](char* to) {
+    sp.begin(to, next, tile.red);
+    sq.begin(to + OpP::kBytes, next, tile.red);
+    next += kStageK;
+  };
+  constexpr int kParts = OpP::kPer + OpQ::kPer;
+  const auto part = [&](int t) {
+    if (t < OpP::kPer) sp.part(t);
+    else sq.part(t - OpP::kPer);
+  };
+  const auto load = [&](char* to) {
+    begin(to);
+    #pragma unroll
+    for (int t = 0; t < kParts; t++) part(t);
+  };
+  u32x4 fp[2][kFm], fq[2][kFn];
+  // fragments to read in a row of matrix instructions: done well before the barrier waits for them
+#ifndef READ_ROWS
+#define READ_ROWS 3 / 4
+#endif
+  constexpr int kReads = kFm + kFn, kReadRows = kFm * READ_ROWS > 0 ? kFm * READ_ROWS : 1, kReadsRow = (kReads + kReadRows - 1) / kReadRows;
+  const auto read = [&](int set, const char* from, int half, int t) {
+    if (t < kFn) fq[set][t] = OpQ::fragment(from + OpP::kBytes, wc + t * 16, half * 4);
+    else fp[set][t - kFn] = OpP::fragment(from, wr + (t - kFn) * 16, half * 4);
+  };
+  typename E::acc acc[kFm][kFn] = {};
+  if (tile.red) {
     load(lds);
     if constexpr (kDirect) {
       #pragma unroll
-      for (int s = 1; s < kStages; s++) load(lds + s * kStageBytes);
+      for (int s = 1; s < kStages; s++) load(lds + s * kBytes);
       wait_stage<(kStages - 1) * kParts>();
     } else {
       sp.store(lds);
@@ -407,19 +422,14 @@ __global__ __launch_bounds__(S::kThreads) void etha_matmul_kernel(const MatmulAr
     #pragma unroll
     for (int t = 0; t < kReads; t++) read(0, lds, 0, t);
     uint32_t use = 0;
-    // Two halves an iteration, so that the sets of fragments keep their names; where that is two stages and their number is
-    // odd, the last half multiplies the zeros past the end of k.
-    constexpr int kStagesIter = kHalves == 1 ? 2 : 1;
-    for (uint32_t s = 0; s < stages; s += kStagesIter) {
-      static_assert(kHalves <= 2, "two halves an iteration");
+    for (uint32_t k = 0; k < tile.red; k += kStageK) {
+      const uint32_t then = use + kBytes == sizeof(lds) ? 0 : use + kBytes;
       #pragma unroll
       for (int h = 0; h < 2; h++) {
-        const bool last = kHalves == 1 || h == 1;  // of its stage
-        const uint32_t then = use + kStageBytes == sizeof(lds) ? 0 : use + kStageBytes;
-        if (last) {
+        if (h == 1) {
           if constexpr (kDirect) {
             wait_stage<(kStages - 2) * kParts>();
-            begin(lds + use);  // past the end of k it brings zeros: the count of loads stays the same
+            begin(lds + use);
           } else {
             sp.store(lds + then);
             sq.store(lds + then + OpP::kBytes);
@@ -432,23 +442,23 @@ __global__ __launch_bounds__(S::kThreads) void etha_matmul_kernel(const MatmulAr
         #pragma unroll
         for (int i = 0; i < kFm; i++) {
           #pragma unroll
-          for (int t = i * kReads / kFm; t < (i + 1) * kReads / kFm; t++)
-            read((h + 1) & 1, lds + (last ? then : use), last ? 0 : 1, t);
+          for (int t = i * kReadsRow; t < (i + 1) * kReadsRow && t < kReads; t++) read(h ^ 1, lds + (h ? then : use), h ^ 1, t);
           #pragma unroll
-          for (int j = 0; j < kFn; j++) acc[i][j] = E::mfma(fq[h & 1][j], fp[h & 1][i], acc[i][j]);
-          if (last) {
+          for (int j = 0; j < kFn; j++) acc[i][j] = E::mfma(fq[h][j], fp[h][i], acc[i][j]);
+          if (h == 1) {
             #pragma unroll
             for (int t = i * kParts / kFm; t < (i + 1) * kParts / kFm; t++) part(t);
           }
           __builtin_amdgcn_sched_barrier(0);
         }
-        if (last) use = then;
       }
+      use = then;
     }
     if constexpr (kDirect) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no load into this LDS outlives the workgroup
   }
   // a lane holds row (lane & 15) and four consecutive columns of each 16 x 16 block
-  const uint32_t row_first = row0 + wr + (lane & 15), col_first = col0 + wc + (lane >> 4) * 4;
+  const uint32_t row_first = tile.row0 + wr + (lane & 15), col_first = tile.col0 + wc + (lane >> 4) * 4;
+  typename D::bits* out = (typename D::bits*)a.out + tile.out;
   float col_scale[kFn][4], bias[kFn][4];
   if constexpr (E::kEs == 1) {
     #pragma unroll
@@ -460,33 +470,63 @@ __global__ __launch_bounds__(S::kThreads) void etha_matmul_kernel(const MatmulAr
         bias[j][c] = a.bias ? a.bias[col] : 0.f;
       }
   }
+  // 16-bit results of two neighbouring blocks change places between the lanes, so that a lane stores 16 bytes and four of
+  // them 64 bytes of a row, instead of 8 and 32
+  constexpr bool kPairs = sizeof(typename D::bits) == 2 && kFn % 2 == 0;
   const auto store_tile = [&](auto whole) {
     #pragma unroll
     for (int i = 0; i < kFm; i++) {
       const uint32_t row = row_first + i * 16;
-      if (!whole && row >= row_end) continue;
-      typename D::bits* to = out + (int64_t)row * a.out_stride + col_first;
       float row_scale = 1.f;
-      if constexpr (E::kEs == 1) row_scale = a.row_scale[row];
+      if constexpr (E::kEs == 1) row_scale = a.row_scale[whole || row < tile.row_end ? row : tile.row_end - 1];
+      typename D::bits* to = out + (int64_t)row * a.out_stride;
+      float v[kFn][4];
       #pragma unroll
-      for (int j = 0; j < kFn; j++) {
-        float v[4];
+      for (int j = 0; j < kFn; j++)
         #pragma unroll
         for (int c = 0; c < 4; c++) {
           // the integer sum is exact; one product of scales, as the definition has it
           if constexpr (E::kEs == 1) {
-            v[c] = (float)acc[i][j][c] * (row_scale * col_scale[j][c]);
-            if (a.bias) v[c] += bias[j][c];
+            v[j][c] = (float)acc[i][j][c] * (row_scale * col_scale[j][c]);
+            if (a.bias) v[j][c] += bias[j][c];
           } else {
-            v[c] = acc[i][j][c];
+            v[j][c] = acc[i][j][c];
           }
         }
-        if (whole) store_f32<D, 4>(to + j * 16, v, 4);
-        else store_f32<D, 4>(to + j * 16, v, (int64_t)a.cols - (col_first + j * 16));
+      if constexpr (kPairs) {
+        #pragma unroll
+        for (int j = 0; j < kFn; j += 2) {
+          u32x4 w;
+          #pragma unroll
+          for (int c = 0; c < 2; c++) {
+            const uint32_t x = (uint32_t)D::from_f32(v[j][2 * c]) | (uint32_t)D::from_f32(v[j][2 * c + 1]) << 16;
+            const uint32_t y = (uint32_t)D::from_f32(v[j + 1][2 * c]) | (uint32_t)D::from_f32(v[j + 1][2 * c + 1]) << 16;
+            const u32x2 r = __builtin_amdgcn_permlane16_swap(x, y, false, false);
+            w[c] = r.x;
+            w[2 + c] = r.y;
+          }
+          // groups of 16 lanes: columns 0..7 of block j, of block j + 1, then 8..15 of either
+          const uint32_t col = tile.col0 + wc + j * 16 + (lane >> 4 & 1) * 16 + (lane >> 5) * 8;
+          if (whole) {
+            store_raw<16>(to + col, w);
+          } else if (row < tile.row_end) {
+            if (col + 8 <= a.cols) {
+              store_raw<16>(to + col, w);
+            } else {
+              #pragma unroll
+              for (int e = 0; e < 8; e++)
+                if (col + e < a.cols) to[col + e] = (typename D::bits)(w[e >> 1] >> (16 * (e & 1)));
+            }
+          }
+        }
+      } else if (whole || row < tile.row_end) {
+        #pragma unroll
+        for (int j = 0; j < kFn; j++)
+          store_f32<D, 4>(to + col_first + j * 16, v[j], whole ? 4 : (int64_t)a.cols - (col_first + j * 16));
       }
     }
   };
-  if (row0 + S::BM <= row_end && col0 + S::BN <= a.cols) store_tile(std::true_type{});
+  if (tile.row0 + S::BM <= tile.row_end && tile.col0 + S::BN <= a.cols) store_tile(std::true_type{});
   else store_tile(std::false_type{});
 }
 
@@ -505,35 +545,12 @@ int check_sizes(const char* what, uint64_t rows, uint64_t cols, uint64_t red, ui
   return ETHA_OK;
 }
 
-// Whether an operand's tiles can be brought straight into LDS, see DirectStage.
-bool is_direct(const void* base, int64_t stride, int64_t group_stride, uint64_t k_bytes, bool trans) {
-  return !(((uintptr_t)base | (uint64_t)stride | (uint64_t)group_stride) & 15) && (trans || !(k_bytes & 15)) && stride >= 0 &&
-         stride < 1 << 22;
+// Whether an operand's tiles can be brought straight into LDS, see DirectStage.  `across`: elements of a row of memory
+// where it lies transposed; rows that overlap (a broadcast gradient) would leave what is past the end of k within the tile.
+bool is_direct(const void* base, int64_t stride, int64_t group_stride, uint64_t k_bytes, bool trans, uint64_t across) {
+  return !(((uintptr_t)base | (uint64_t)stride | (uint64_t)group_stride) & 15) && stride >= 0 && stride < 1 << 22 &&
+         (trans ? (uint64_t)stride >= across * 2 : !(k_bytes & 15));
 }
-
-template <typename E, uint32_t KIND, typename D, typename S>
-int launch_matmul(const char* what, const MatmulArgs& a, uint64_t row_tiles, bool direct, void* stream) {
-  const uint64_t col_tiles = ((uint64_t)a.cols + S::BN - 1) / S::BN, blocks = row_tiles * col_tiles;
-  if (blocks >= 1ull << 22) return fail(ETHA_ERR_UNSUPPORTED, "%s: the product is too large for one call", what);
-  if (!blocks) return ETHA_OK;
-  const dim3 grid((uint32_t)blocks), block(S::kThreads);
-  if (direct) hipLaunchKernelGGL((etha_matmul_kernel<E, KIND, D, S, DirectStage>), grid, block, 0, (hipStream_t)stream, a);
-  else hipLaunchKernelGGL((etha_matmul_kernel<E, KIND, D, S, RegisterStage>), grid, block, 0, (hipStream_t)stream, a);
-  return launched("etha_matmul_kernel");
-}
-
-#ifndef SHAPE_L
-#define SHAPE_L 256, 256, 2, 4, 128, 2
-#endif
-#ifndef SHAPE_M
-#define SHAPE_M 128, 128, 2, 2, 128, 3
-#endif
-#ifndef SHAPE_S
-#define SHAPE_S 32, 64, 1, 4, 128, 6
-#endif
-typedef Shape<SHAPE_L> ShapeL;
-typedef Shape<SHAPE_M> ShapeM;
-typedef Shape<SHAPE_S> ShapeS;
 
 // No group wastes more than one row tile, and a group with rows has at least one.
 uint64_t row_tiles_of(const MatmulArgs& a, uint32_t kind, int bm) {
@@ -543,23 +560,51 @@ uint64_t row_tiles_of(const MatmulArgs& a, uint32_t kind, int bm) {
   return (a.rows - groups) / bm + groups;
 }
 
+template <typename E, uint32_t KIND, typename D, typename S, template <typename> class STAGE>
+int launch_matmul(const char* what, const MatmulArgs& a, void* stream) {
+  const uint64_t row_tiles = row_tiles_of(a, KIND, S::BM);
+  const uint64_t col_tiles = ((uint64_t)a.cols + S::BN - 1) / S::BN, blocks = row_tiles * col_tiles;
+  if (blocks >= 1ull << 22) return fail(ETHA_ERR_UNSUPPORTED, "%s: the product is too large for one call", what);
+  if (!blocks) return ETHA_OK;
+  hipLaunchKernelGGL((etha_matmul_kernel<E, KIND, D, S, STAGE>), dim3((uint32_t)blocks), dim3(S::kThreads), 0, (hipStream_t)stream, a);
+  return launched("etha_matmul_kernel");
+}
+
+#ifndef SHAPE_L
+#define SHAPE_L 256, 256, 2, 4, 2
+#endif
+#ifndef SHAPE_M
+#define SHAPE_M 128, 128, 2, 4, 2
+#endif
+#ifndef SHAPE_S
+#define SHAPE_S 32, 64, 1, 4, 6
+#endif
+#ifndef SHAPE_R
+#define SHAPE_R 128, 128, 2, 4, 2
+#endif
+typedef Shape<SHAPE_R> ShapeR;
+typedef Shape<SHAPE_L> ShapeL;
+typedef Shape<SHAPE_M> ShapeM;
+typedef Shape<SHAPE_S> ShapeS;
+
 template <typename E, uint32_t KIND, typename D>
 int shaped_matmul(const char* what, const MatmulArgs& a, bool direct, void* stream) {
   // rows a group has on average: the height of the tiles that it fills
   const uint64_t rows = KIND == kGroupRows || KIND == kGroupRowsT ? a.rows / (a.n_groups ? a.n_groups : 1) : a.rows;
   const auto tiles = [&](int bm, int bn) { return row_tiles_of(a, KIND, bm) * (((uint64_t)a.cols + bn - 1) / bn); };
   if (rows <= 32 && KIND != kGroupReduce)
-    return launch_matmul<E, KIND, D, ShapeS>(what, a, row_tiles_of(a, KIND, ShapeS::BM), direct, stream);
-  if (rows > 128 && tiles(ShapeL::BM, ShapeL::BN) >= 192)
-    return launch_matmul<E, KIND, D, ShapeL>(what, a, row_tiles_of(a, KIND, ShapeL::BM), direct, stream);
-  return launch_matmul<E, KIND, D, ShapeM>(what, a, row_tiles_of(a, KIND, ShapeM::BM), direct, stream);
+    return direct ? launch_matmul<E, KIND, D, ShapeS, DirectStage>(what, a, stream) : launch_matmul<E, KIND, D, ShapeS, RegisterStage>(what, a, stream);
+  if (!direct) return launch_matmul<E, KIND, D, ShapeR, RegisterStage>(what, a, stream);
+  if (rows > 128 && tiles(ShapeL::BM, ShapeL::BN) >= 192) return launch_matmul<E, KIND, D, ShapeL, DirectStage>(what, a, stream);
+  return launch_matmul<E, KIND, D, ShapeM, DirectStage>(what, a, stream);
 }
 
 template <typename E, uint32_t KIND>
 int run_matmul(const char* what, const MatmulArgs& a, uint32_t out_dtype, void* stream) {
   constexpr bool kTransP = KIND == kGroupReduce, kTransQ = KIND == kGroupReduce || KIND == kGroupRowsT;
   const uint64_t k_bytes = (uint64_t)a.red * E::kEs;
-  const bool direct = is_direct(a.p, a.p_stride, 0, k_bytes, kTransP) && is_direct(a.q, a.q_stride, a.q_group_stride, k_bytes, kTransQ);
+  const bool direct = is_direct(a.p, a.p_stride, 0, k_bytes, kTransP, a.rows) &&
+                      is_direct(a.q, a.q_stride, a.q_group_stride, k_bytes, kTransQ, a.cols);
   if (out_dtype == ETHA_F32) return shaped_matmul<E, KIND, F32>(what, a, direct, stream);
   if (out_dtype == ETHA_BF16) return shaped_matmul<E, KIND, BF16>(what, a, direct, stream);
   return shaped_matmul<E, KIND, F16>(what, a, direct, stream);

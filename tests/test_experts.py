@@ -200,6 +200,15 @@ def test_views(gpu_device):
         check_weight(matrices, gs, xs, offsets[1:5])
         one = grad[:1, :1].expand(x.shape[0], 95)  # a broadcast gradient
         check_rows(grouped_linear_grad_rows(one, ws, offsets[1:5]), one, ws, offsets[1:5], transposed=True)
+    for rows in (5, 70, 300):  # one row for all: its stride is zero
+        x, weight, offsets, grad = case(gen, [rows, 3], 128, 256, torch.bfloat16, gpu_device)
+        one, many = grad[:1].expand(rows + 3, 128), x[:1].expand(rows + 3, 256)
+        check_weight(grouped_linear_grad_weight(one, x, offsets), one, x, offsets)
+        check_weight(grouped_linear_grad_weight(grad, many, offsets), grad, many, offsets)
+        check_rows(grouped_linear_grad_rows(one, weight, offsets), one, weight, offsets, transposed=True)
+        check_rows(grouped_linear(many, weight, offsets), many, weight, offsets)
+        same = weight[:1].expand(2, 128, 256)  # one matrix for all experts
+        check_rows(grouped_linear(x, same, offsets), x, same, offsets)
 
 
 @pytest.mark.gpu
