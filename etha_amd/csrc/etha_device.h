@@ -6,6 +6,8 @@
 
 #include <cstdint>
 
+#include "etha_reshard.h"
+
 namespace etha_device {
 
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
@@ -96,6 +98,75 @@ __device__ inline void store_f32(typename T::bits* p, const float (&v)[N], int64
   }
 }
 
+// ---- rows to 8 bits ----------------------------------------------------------------------------------------------
+// the largest magnitude so far by its bits: infinity is above all numbers, NaN above infinity
+__device__ inline uint32_t largest_bits(const float (&v)[8], uint32_t top) {
+  #pragma unroll
+  for (int i = 0; i < 8; i++) {
+    const uint32_t m = __builtin_bit_cast(uint32_t, v[i]) & 0x7fffffffu;
+    top = m > top ? m : top;
+  }
+  return top;
+}
+__device__ inline uint32_t wave_max(uint32_t v) {
+  #pragma unroll
+  for (int d = 32; d; d >>= 1) {
+    const uint32_t o = __shfl_xor(v, d);
+    v = o > v ? o : v;
+  }
+  return v;
+}
+
+// scale = max|x| * (1 / 127) in fp32; q = x / scale rounded half to even - of the exact quotient: with q0 next to it,
+// r = x - q0 * scale is a multiple of ulp(scale) / 2 below scale and so an fp32 number, which the fused multiply-add
+// gives exactly; comparing |r| with scale / 2 then settles the rounding.
+struct RowScale {
+  float scale, inverse;
+  bool none, tiny;
+  __device__ explicit RowScale(uint32_t top) {
+    scale = __builtin_bit_cast(float, top) * (1.f / 127.f);
+    none = !(scale > 0.f) || top >= 0x7f800000u;  // a row of zeros, or one that holds an infinity or NaN
+    // a scale below the smallest normal number may have no finite inverse: the quotient is formed by division there
+    tiny = scale < 1.2e-38f;
+    inverse = 1.f / scale;
+  }
+  // near: x / scale, give or take a few roundings
+  __device__ uint32_t value(float x, float near) const {
+    float q = __builtin_rintf(near);
+    const float r = __builtin_fmaf(-q, scale, x);
+    const float twice = 2.f * __builtin_fabsf(r);
+    // off by one, or a tie that went to the odd side
+    if (twice > scale || (twice == scale && ((int)q & 1))) q += (r > 0.f) ? 1.f : -1.f;
+    return (uint32_t)(int)__builtin_fmaxf(-127.f, __builtin_fminf(127.f, q)) & 255u;
+  }
+  __device__ u32x2 pack(const float (&v)[8]) const {
+    u32x2 w = {0, 0};
+    if (none) return w;
+    float near[8];
+    if (tiny) {
+      #pragma unroll
+      for (int i = 0; i < 8; i++) near[i] = v[i] / scale;
+    } else {
+      #pragma unroll
+      for (int i = 0; i < 8; i++) near[i] = v[i] * inverse;
+    }
+    #pragma unroll
+    for (int i = 0; i < 8; i++) w[i >> 2] |= value(v[i], near[i]) << (8 * (i & 3));
+    return w;
+  }
+};
+
 }  // namespace etha_device
+
+// ---- host ----
+// Calls f with the tag of the element type (checked before).
+template <typename F>
+inline void with_type(uint32_t dtype, F&& f) {
+  if (dtype == ETHA_F32) f(etha_device::F32{});
+  else if (dtype == ETHA_BF16) f(etha_device::BF16{});
+  else f(etha_device::F16{});
+}
+
+
 
 #endif  // ETHA_DEVICE_H

@@ -530,6 +530,158 @@ __global__ __launch_bounds__(S::kThreads) void etha_matmul_kernel(const MatmulAr
   else store_tile(std::false_type{});
 }
 
+// ---- few rows --------------------------------------------------------------------------------------------------------
+// Up to 16 rows against a matrix: what counts is that the matrix streams.  A workgroup of 8 waves takes 32 columns and
+// each wave every eighth 128-byte line of k, straight from memory into the registers that the matrix instructions read (a
+// lane takes 32 bytes of a line; both operands are read in that order, so the order of k does not matter), no LDS and no
+// barrier on the way; the eight partial sums are added up in LDS in the waves' order.
+// With SX the rows come as floating-point numbers and are converted to 8 bits in the workgroup, into LDS, while the first
+// lines of the matrix are on their way: one launch instead of two.
+constexpr int kFewRows = 16, kFewCols = 32, kFewWaves = 8, kFewThreads = kFewWaves * 64, kFewAhead = 4;
+constexpr uint32_t kFewLds = 32768;  // bytes of converted rows at most
+
+struct FewArgs {
+  MatmulArgs m;
+  const void* x;     // SX: rows to be converted
+  int64_t x_stride;  // elements
+};
+
+template <typename E, uint32_t KIND, typename D, typename SX>
+__global__ __launch_bounds__(kFewThreads) void etha_few_rows_kernel(const FewArgs few) {
+  constexpr bool kConvert = !std::is_void_v<SX>;
+  const MatmulArgs& a = few.m;
+  __shared__ typename std::conditional<E::kEs == 1, int, float>::type s_sum[kFewWaves][kFewRows * kFewCols];
+  __shared__ __align__(16) char s_x[kConvert ? kFewLds + kFewRows * 160 : 16];
+  __shared__ uint32_t s_top[kConvert ? kFewRows : 1][kFewWaves];
+  const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t col_tiles = (a.cols + kFewCols - 1) / kFewCols;
+  const uint32_t col0 = blockIdx.x % col_tiles * kFewCols, row_id = blockIdx.x / col_tiles;
+  uint32_t row0 = row_id * kFewRows, row_end = a.rows, red = a.red;
+  const char *p = a.p, *q = a.q;
+  if constexpr (KIND != kPlain) {
+    const GroupTile g = find_tile<kFewRows>(a, row_id);
+    if (!g.found) return;
+    row0 = g.lo + g.tile * kFewRows;
+    row_end = g.hi;
+    if (g.group == a.n_groups) red = 0;
+    else q += (int64_t)g.group * a.q_group_stride;
+  }
+  const uint32_t n_rows = row_end - row0 < kFewRows ? row_end - row0 : kFewRows;
+  const int64_t bytes = (int64_t)red * E::kEs;
+  const uint32_t whole = (uint32_t)(bytes / 128);
+  const uint32_t at = (lane >> 4) * 32, r = lane & 15;
+  const uint32_t xr = r < n_rows ? r : n_rows - 1;  // rows past the last repeat it; their results are dropped
+  const char* xp = p + (int64_t)(row0 + xr) * a.p_stride + at;
+  const char* wp[2];
+  #pragma unroll
+  for (int j = 0; j < 2; j++) {
+    const uint32_t c = col0 + j * 16 + r;
+    wp[j] = q + (int64_t)(c < a.cols ? c : a.cols - 1) * a.q_stride + at;
+  }
+  const uint32_t pitch = (uint32_t)(bytes + 127) / 128 * 128 + 32;  // of converted rows
+  typename E::acc acc[2] = {};
+  u32x4 w[kFewAhead][2][2], x[kFewAhead][2];
+  const auto load_w = [&](uint32_t line) {
+    #pragma unroll
+    for (int u = 0; u < kFewAhead; u++)
+      #pragma unroll
+      for (int j = 0; j < 2; j++)
+        #pragma unroll
+        for (int h = 0; h < 2; h++) w[u][j][h] = load_raw<16, true>(wp[j] + (int64_t)(line + u * kFewWaves) * 128 + h * 16);
+  };
+  const auto load_x = [&](int u, uint32_t line) {
+    #pragma unroll
+    for (int h = 0; h < 2; h++) {
+      if constexpr (kConvert) x[u][h] = *(const u32x4*)(s_x + xr * pitch + line * 128 + at + h * 16);
+      else x[u][h] = load_raw<16>(xp + (int64_t)line * 128 + h * 16);
+    }
+  };
+  const auto multiply = [&](int u) {
+    #pragma unroll
+    for (int h = 0; h < 2; h++)
+      #pragma unroll
+      for (int j = 0; j < 2; j++) acc[j] = E::mfma(w[u][j][h], x[u][h], acc[j]);
+  };
+  // lines wave, wave + 8, ...: batches of kFewAhead of them, then one by one
+  uint32_t line = wave;
+  const auto batch = [&]() { return line + (kFewAhead - 1) * kFewWaves < whole; };
+  const bool early = batch();
+  if (early) load_w(line);
+  if constexpr (kConvert) {
+    const typename SX::bits* rows = (const typename SX::bits*)few.x;
+    for (uint32_t m = 0; m < n_rows; m++) {
+      uint32_t top = 0;
+      for (uint32_t k = threadIdx.x * 8; k < red; k += kFewThreads * 8) {
+        float v[8];
+        load_f32<SX, 8>(v, rows + (int64_t)(row0 + m) * few.x_stride + k, (int64_t)red - k);
+        top = largest_bits(v, top);
+      }
+      top = wave_max(top);
+      if (lane == 0) s_top[m][wave] = top;
+    }
+    __syncthreads();
+    for (uint32_t m = 0; m < n_rows; m++) {
+      uint32_t top = 0;
+      #pragma unroll
+      for (int i = 0; i < kFewWaves; i++) top = s_top[m][i] > top ? s_top[m][i] : top;
+      const RowScale scale(top);
+      for (uint32_t k = threadIdx.x * 8; k < pitch - 32; k += kFewThreads * 8) {
+        float v[8];
+        load_f32<SX, 8>(v, rows + (int64_t)(row0 + m) * few.x_stride + k, (int64_t)red - k);
+        *(u32x2*)(s_x + m * pitch + k) = scale.pack(v);  // past the end of k: zeros
+      }
+    }
+    __syncthreads();
+  }
+  if (early) {
+    for (;;) {
+      #pragma unroll
+      for (int u = 0; u < kFewAhead; u++) load_x(u, line + u * kFewWaves);
+      #pragma unroll
+      for (int u = 0; u < kFewAhead; u++) multiply(u);
+      line += kFewAhead * kFewWaves;
+      if (!batch()) break;
+      load_w(line);
+    }
+  }
+  for (; line * 128 < bytes; line += kFewWaves) {
+    #pragma unroll
+    for (int h = 0; h < 2; h++) {
+      const int64_t left = bytes - (int64_t)line * 128 - at - h * 16;
+      #pragma unroll
+      for (int j = 0; j < 2; j++) w[0][j][h] = load_part<E::kEs>(wp[j] + (int64_t)line * 128 + h * 16, left);
+      if constexpr (!kConvert) x[0][h] = load_part<E::kEs>(xp + (int64_t)line * 128 + h * 16, left);
+    }
+    if constexpr (kConvert) load_x(0, line);
+    multiply(0);
+  }
+  #pragma unroll
+  for (int j = 0; j < 2; j++)
+    #pragma unroll
+    for (int c = 0; c < 4; c++) s_sum[wave][j * 256 + lane * 4 + c] = acc[j][c];
+  __syncthreads();
+  const uint32_t t = threadIdx.x, row = row0 + (t >> 2 & 15), col = col0 + (t >> 8) * 16 + (t >> 6 & 3) * 4 + (t & 3);
+  if (row >= row_end || col >= a.cols) return;
+  auto sum = s_sum[0][t];
+  #pragma unroll
+  for (int i = 1; i < kFewWaves; i++) sum += s_sum[i][t];
+  float v = (float)sum;
+  if constexpr (E::kEs == 1) {
+    float row_scale;
+    if constexpr (kConvert) {
+      uint32_t top = 0;
+      #pragma unroll
+      for (int i = 0; i < kFewWaves; i++) top = s_top[row - row0][i] > top ? s_top[row - row0][i] : top;
+      row_scale = RowScale(top).scale;
+    } else {
+      row_scale = a.row_scale[row];
+    }
+    v *= row_scale * a.col_scale[col];
+    if (a.bias) v += a.bias[col];
+  }
+  ((typename D::bits*)a.out)[(int64_t)row * a.out_stride + col] = D::from_f32(v);
+}
+
 int launched(const char* name) {
   g_kernel_launches.fetch_add(1, std::memory_order_relaxed);
   const hipError_t e = hipGetLastError();
@@ -587,11 +739,26 @@ typedef Shape<SHAPE_L> ShapeL;
 typedef Shape<SHAPE_M> ShapeM;
 typedef Shape<SHAPE_S> ShapeS;
 
+template <typename E, uint32_t KIND, typename D, typename SX>
+int launch_few(const char* what, const FewArgs& few, void* stream) {
+  const uint64_t blocks = row_tiles_of(few.m, KIND, kFewRows) * (((uint64_t)few.m.cols + kFewCols - 1) / kFewCols);
+  if (blocks >= 1ull << 22) return fail(ETHA_ERR_UNSUPPORTED, "%s: the product is too large for one call", what);
+  hipLaunchKernelGGL((etha_few_rows_kernel<E, KIND, D, SX>), dim3((uint32_t)blocks), dim3(kFewThreads), 0, (hipStream_t)stream, few);
+  return launched("etha_few_rows_kernel");
+}
+
 template <typename E, uint32_t KIND, typename D>
 int shaped_matmul(const char* what, const MatmulArgs& a, bool direct, void* stream) {
   // rows a group has on average: the height of the tiles that it fills
   const uint64_t rows = KIND == kGroupRows || KIND == kGroupRowsT ? a.rows / (a.n_groups ? a.n_groups : 1) : a.rows;
   const auto tiles = [&](int bm, int bn) { return row_tiles_of(a, KIND, bm) * (((uint64_t)a.cols + bn - 1) / bn); };
+  if constexpr (KIND == kPlain || KIND == kGroupRows) {
+    if (rows <= kFewRows) {
+      FewArgs few = {};
+      few.m = a;
+      return launch_few<E, KIND, D, void>(what, few, stream);
+    }
+  }
   if (rows <= 32 && KIND != kGroupReduce)
     return direct ? launch_matmul<E, KIND, D, ShapeS, DirectStage>(what, a, stream) : launch_matmul<E, KIND, D, ShapeS, RegisterStage>(what, a, stream);
   if (!direct) return launch_matmul<E, KIND, D, ShapeR, RegisterStage>(what, a, stream);
@@ -611,6 +778,10 @@ int run_matmul(const char* what, const MatmulArgs& a, uint32_t out_dtype, void* 
 }
 
 bool is_out(uint32_t dtype) { return dtype == ETHA_F32 || dtype == ETHA_BF16 || dtype == ETHA_F16; }
+
+// Rows that the few-rows kernel converts itself: it reads them once for every 32 columns, so there must not be many of them.
+bool is_few(uint64_t rows, uint64_t width) { return rows <= 4 && rows * ((width + 127) / 128 * 128) <= kFewLds; }
+uint64_t padded_width(uint64_t width) { return (width + 15) / 16 * 16; }
 
 template <uint32_t KIND>
 int run_grouped(const char* what, const MatmulArgs& a, uint32_t dtype, uint32_t out_dtype, void* stream) {
@@ -651,6 +822,53 @@ int etha_int8_matmul(const int8_t* x, const float* x_scale, uint64_t rows, int64
   a.col_scale = w_scale;
   a.bias = bias;
   return run_matmul<ElemI8, kPlain>("etha_int8_matmul", a, out_dtype, stream);
+}
+
+int etha_int8_linear_workspace(uint64_t rows, uint64_t width, uint64_t* bytes) {
+  if (!bytes) return fail(ETHA_ERR_INVALID, "etha_int8_linear_workspace: null result");
+  const int rc = check_sizes("etha_int8_linear_workspace", rows, 0, width, ETHA_INT8_MAX_WIDTH);
+  if (rc != ETHA_OK) return rc;
+  *bytes = is_few(rows, width) ? 0 : rows * padded_width(width) + rows * 4;
+  return ETHA_OK;
+}
+
+int etha_int8_linear(const void* x, uint32_t dtype, uint64_t rows, int64_t x_stride, const int8_t* w, const float* w_scale,
+                     uint64_t cols, int64_t w_stride, uint64_t width, const float* bias, void* out, uint32_t out_dtype,
+                     int64_t out_stride, void* workspace, uint64_t workspace_bytes, void* stream) {
+  int rc = check_sizes("etha_int8_linear", rows, cols, width, ETHA_INT8_MAX_WIDTH);
+  if (rc != ETHA_OK) return rc;
+  if (!is_out(dtype) || !is_out(out_dtype)) return fail(ETHA_ERR_UNSUPPORTED, "etha_int8_linear: element types are f32, bf16 and f16");
+  if (!rows || !cols) return ETHA_OK;
+  if ((width && (!x || !w)) || !w_scale || !out) return fail(ETHA_ERR_INVALID, "etha_int8_linear: null tensor");
+  if (is_few(rows, width)) {
+    FewArgs few = {};
+    few.x = x;
+    few.x_stride = x_stride;
+    few.m.q = (const char*)w;
+    few.m.out = out;
+    few.m.q_stride = w_stride;
+    few.m.out_stride = out_stride;
+    few.m.rows = (uint32_t)rows;
+    few.m.cols = (uint32_t)cols;
+    few.m.red = (uint32_t)width;
+    few.m.col_scale = w_scale;
+    few.m.bias = bias;
+    with_type(dtype, [&](auto s) {
+      with_type(out_dtype, [&](auto d) {
+        rc = launch_few<ElemI8, kPlain, decltype(d), decltype(s)>("etha_int8_linear", few, stream);
+      });
+    });
+    return rc;
+  }
+  const uint64_t pitch = padded_width(width);
+  if (!workspace || workspace_bytes < rows * pitch + rows * 4 || ((uintptr_t)workspace & 15))
+    return fail(ETHA_ERR_INVALID, "etha_int8_linear: the workspace has to hold %llu bytes at a 16-byte address",
+                (unsigned long long)(rows * pitch + rows * 4));
+  int8_t* values = (int8_t*)workspace;
+  float* scales = (float*)((char*)workspace + rows * pitch);
+  rc = etha_quantize_rows(x, dtype, rows, width, x_stride, values, (int64_t)pitch, scales, stream);
+  if (rc != ETHA_OK) return rc;
+  return etha_int8_matmul(values, scales, rows, (int64_t)pitch, w, w_scale, cols, w_stride, width, bias, out, out_dtype, out_stride, stream);
 }
 
 int etha_grouped_matmul(const void* x, uint32_t dtype, uint64_t rows, int64_t x_stride, const void* w, uint64_t n_groups,

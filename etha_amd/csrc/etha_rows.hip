@@ -412,10 +412,7 @@ __global__ __launch_bounds__(kGradWaves* kWave) void etha_embedding_join_kernel(
 }
 
 // ---- rows to 8 bits --------------------------------------------------------------------------------------------
-// scale = max|x| * (1 / 127) in fp32, q = x / scale rounded half to even - of the exact quotient:
-// with q0 next to it, r = x - q0 * scale is a multiple of ulp(scale) / 2 below 2 * scale and so an fp32 number, which
-// the fused multiply-add gives exactly; comparing |r| with scale / 2 then settles the rounding.  The row stays in
-// registers between its maximum and its conversion, so it is read once.
+// The row stays in registers between its maximum and its conversion (RowScale), so it is read once.
 struct QuantArgs {
   const void* x;
   int8_t* values;
@@ -423,15 +420,6 @@ struct QuantArgs {
   uint64_t rows, width;
   int64_t x_stride, values_stride;
 };
-
-__device__ inline int to_8_bits(float x, float scale, float near) {
-  float q = __builtin_rintf(near);  // near: x / scale, give or take a few roundings
-  const float r = __builtin_fmaf(-q, scale, x);
-  const float twice = 2.f * __builtin_fabsf(r);
-  // off by one, or a tie that went to the odd side
-  if (twice > scale || (twice == scale && ((int)q & 1))) q += (r > 0.f) ? 1.f : -1.f;
-  return (int)__builtin_fmaxf(-127.f, __builtin_fminf(127.f, q));
-}
 
 template <typename S, int THREADS, int CHUNKS>
 __global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS) void etha_quantize_rows_kernel(const QuantArgs a) {
@@ -450,18 +438,10 @@ __global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS) void etha_quantize_r
     for (int c = 0; c < CHUNKS; c++) {
       const int64_t at = base + ((int64_t)c * THREADS + tid) * 8;
       load_f32<S, 8>(v[c], x + at, width - at);
-      #pragma unroll
-      for (int i = 0; i < 8; i++) {
-        const uint32_t m = __builtin_bit_cast(uint32_t, v[c][i]) & 0x7fffffffu;
-        top = m > top ? m : top;
-      }
+      top = largest_bits(v[c], top);
     }
   }
-  #pragma unroll
-  for (int d = 32; d; d >>= 1) {
-    const uint32_t o = __shfl_xor(top, d);
-    top = o > top ? o : top;
-  }
+  top = wave_max(top);
   if (kWaves > 1) {
     if ((threadIdx.x & 63) == 0) s_max[threadIdx.x >> 6] = top;
     __syncthreads();
@@ -469,11 +449,7 @@ __global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS) void etha_quantize_r
     for (int w = 0; w < kWaves; w++) top = s_max[w] > top ? s_max[w] : top;
   }
   if (!there) return;
-  const float scale = __builtin_bit_cast(float, top) * (1.f / 127.f);
-  const bool none = !(scale > 0.f) || top >= 0x7f800000u;  // a row of zeros, or one that holds an infinity or NaN
-  // a scale below the smallest normal number may have no finite inverse: the quotient is formed by division there
-  const bool tiny = scale < 1.2e-38f;
-  const float inverse = tiny ? 0.f : 1.f / scale;
+  const RowScale scale(top);
   const bool again = width > (int64_t)THREADS * CHUNKS * 8;
   for (int64_t base = 0; base < width; base += THREADS * CHUNKS * 8) {
     #pragma unroll
@@ -481,35 +457,20 @@ __global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS) void etha_quantize_r
       const int64_t at = base + ((int64_t)c * THREADS + tid) * 8;
       if (at >= width) continue;
       if (again) load_f32<S, 8>(v[c], x + at, width - at);
-      int q[8];
-      #pragma unroll
-      for (int i = 0; i < 8; i++) q[i] = none ? 0 : to_8_bits(v[c][i], scale, tiny ? v[c][i] / scale : v[c][i] * inverse);
-      uint32_t w[2];
-      #pragma unroll
-      for (int i = 0; i < 2; i++)
-        w[i] = (q[4 * i] & 255) | (q[4 * i + 1] & 255) << 8 | (q[4 * i + 2] & 255) << 16 | (uint32_t)(q[4 * i + 3] & 255) << 24;
+      const u32x2 packed = scale.pack(v[c]);
       if (width - at >= 8) {
-        u32x2 packed = {w[0], w[1]};
         store_raw<8>(out + at, packed);
       } else {
         for (int i = 0; i < 8; i++)
-          if (i < width - at) out[at + i] = (int8_t)q[i];
+          if (i < width - at) out[at + i] = (int8_t)(packed[i >> 2] >> (8 * (i & 3)));
       }
     }
   }
-  if (tid == 0) a.scales[row] = scale;
+  if (tid == 0) a.scales[row] = scale.scale;
 }
 
 // ---- host side ---------------------------------------------------------------------------------------------------
 int es_of(uint32_t dtype) { return dtype == ETHA_F32 ? 4 : dtype == ETHA_BF16 || dtype == ETHA_F16 ? 2 : 0; }
-
-// Calls f with the tag of the element type (checked before by es_of).
-template <typename F>
-void with_type(uint32_t dtype, F&& f) {
-  if (dtype == ETHA_F32) f(F32{});
-  else if (dtype == ETHA_BF16) f(BF16{});
-  else f(F16{});
-}
 
 int log2_up(uint64_t x) {
   int l = 0;

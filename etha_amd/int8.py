@@ -52,6 +52,22 @@ def _check_scales(what: str, name: str, scales: torch.Tensor, shape) -> torch.Te
     return scales if scales.is_contiguous() else scales.contiguous()
 
 
+def _weight_operands(what, x, weight, weight_scales, bias):
+    if weight.dtype != torch.int8:
+        raise ValueError(f"{what}: the weight is {weight.dtype}, not int8")
+    if weight.dim() != 2 or x.dim() == 0 or x.shape[-1] != weight.shape[1]:
+        raise ValueError(f"{what}: {tuple(x.shape)} times {tuple(weight.shape)} (channels, width)")
+    channels, width = weight.shape
+    if width > INT8_MAX_WIDTH:
+        raise ValueError(f"{what}: width {width}; a sum over more than {INT8_MAX_WIDTH} products may leave 32 bits")
+    weight_scales = _check_scales(what, "weight_scales", weight_scales, (channels,))
+    if bias is not None:
+        bias = _check_scales(what, "bias", bias, (channels,))
+    weight, stride = readable_rows(weight)
+    rows = x.numel() // width if width else x.shape[:-1].numel()
+    return weight, stride, weight_scales, bias, channels, width, rows
+
+
 def int8_matmul(x: torch.Tensor, x_scales: torch.Tensor, weight: torch.Tensor, weight_scales: torch.Tensor, *,
                 bias: torch.Tensor | None = None, dtype: torch.dtype = torch.bfloat16, out: torch.Tensor | None = None) -> torch.Tensor:
     """``(x * x_scales[..., None]) @ (weight * weight_scales[:, None]).T + bias`` of 8-bit operands, in ``dtype``.
@@ -59,40 +75,47 @@ def int8_matmul(x: torch.Tensor, x_scales: torch.Tensor, weight: torch.Tensor, w
     ``x``: int8 ``[..., width]``; ``weight``: int8 ``[channels, width]``; scales and ``bias`` fp32.  The sum over the integers
     is exact (``width`` up to 131071); scales and bias are applied in fp32 and rounded once.
     """
-    if x.dtype != torch.int8 or weight.dtype != torch.int8:
-        raise ValueError(f"int8_matmul: operands are {x.dtype} and {weight.dtype}, not int8")
-    if weight.dim() != 2 or x.dim() == 0 or x.shape[-1] != weight.shape[1]:
-        raise ValueError(f"int8_matmul: {tuple(x.shape)} times {tuple(weight.shape)} (channels, width)")
-    refuse_grad("int8_matmul", x_scales, weight_scales, bias)
-    channels, width = weight.shape
-    rows = x.numel() // width if width else x.shape[:-1].numel()
-    x_scales = _check_scales("int8_matmul", "x_scales", x_scales, x.shape[:-1])
-    weight_scales = _check_scales("int8_matmul", "weight_scales", weight_scales, (channels,))
-    if bias is not None:
-        bias = _check_scales("int8_matmul", "bias", bias, (channels,))
-    if width > INT8_MAX_WIDTH:
-        raise ValueError(f"int8_matmul: width {width}; a sum over more than {INT8_MAX_WIDTH} products may leave 32 bits")
+    what = "int8_matmul"
+    if x.dtype != torch.int8:
+        raise ValueError(f"{what}: x is {x.dtype}, not int8")
+    refuse_grad(what, x_scales, weight_scales, bias)
+    weight, w_stride, weight_scales, bias, channels, width, rows = _weight_operands(what, x, weight, weight_scales, bias)
+    x_scales = _check_scales(what, "x_scales", x_scales, x.shape[:-1])
     source, stride = readable_rows(x)
-    weight, weight_stride = readable_rows(weight)
-    device = check_device("int8_matmul", x, x_scales, weight, weight_scales, bias, out)
+    if out is not None:
+        out_stride = check_out(what, out, (*x.shape[:-1], channels), DTYPE_CODES, x, x_scales, weight, weight_scales, bias)
+    device = check_device(what, x, x_scales, weight, weight_scales, bias, out)
     if out is None:
-        out_code = code_of("int8_matmul", dtype)
+        code_of(what, dtype)
         out, out_stride = torch.empty((*x.shape[:-1], channels), dtype=dtype, device=device), channels
-    else:
-        out_stride = check_out("int8_matmul", out, (*x.shape[:-1], channels), DTYPE_CODES, x, x_scales, weight, weight_scales, bias)
-        out_code = DTYPE_CODES[out.dtype]
     call(device, _native.lib().etha_int8_matmul, "etha_int8_matmul", source.data_ptr(), x_scales.data_ptr(), rows, stride,
-         weight.data_ptr(), weight_scales.data_ptr(), channels, weight_stride, width, None if bias is None else bias.data_ptr(),
-         out.data_ptr(), out_code, out_stride)
+         weight.data_ptr(), weight_scales.data_ptr(), channels, w_stride, width, None if bias is None else bias.data_ptr(),
+         out.data_ptr(), DTYPE_CODES[out.dtype], out_stride)
     return out
 
 
 def int8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scales: torch.Tensor, *, bias: torch.Tensor | None = None,
                 dtype: torch.dtype | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
-    """A linear layer over an 8-bit weight: ``x`` (fp32, bf16 or fp16) is converted with a scale for each token
-    (:func:`quantize_rows`) and multiplied (:func:`int8_matmul`); the result is in ``dtype`` (default: that of ``x``)."""
-    refuse_grad("int8_linear", x)
-    if out is None and dtype is None:
-        dtype = x.dtype
-    values, scales = quantize_rows(x)
-    return int8_matmul(values, scales, weight, weight_scales, bias=bias, dtype=dtype, out=out)
+    """A linear layer over an 8-bit weight: ``x`` (fp32, bf16 or fp16) is converted with a scale for each token, as
+    :func:`quantize_rows` does it, and multiplied, as :func:`int8_matmul` does it, with the same bits; the result is in
+    ``dtype`` (default: that of ``x``)."""
+    what = "int8_linear"
+    refuse_grad(what, x, weight_scales, bias)
+    x_code = code_of(what, x.dtype)
+    weight, w_stride, weight_scales, bias, channels, width, rows = _weight_operands(what, x, weight, weight_scales, bias)
+    source, stride = readable_rows(x)
+    if out is not None:
+        out_stride = check_out(what, out, (*x.shape[:-1], channels), DTYPE_CODES, x, weight, weight_scales, bias)
+        if dtype is not None and dtype != out.dtype:
+            raise ValueError(f"{what}: dtype {dtype} and an out of {out.dtype}")
+    device = check_device(what, x, weight, weight_scales, bias, out)
+    if out is None:
+        dtype = dtype or x.dtype
+        code_of(what, dtype)
+        out, out_stride = torch.empty((*x.shape[:-1], channels), dtype=dtype, device=device), channels
+    nbytes = _native.int8_linear_workspace(rows, width)
+    workspace = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+    call(device, _native.lib().etha_int8_linear, "etha_int8_linear", source.data_ptr(), x_code, rows, stride, weight.data_ptr(),
+         weight_scales.data_ptr(), channels, w_stride, width, None if bias is None else bias.data_ptr(), out.data_ptr(),
+         DTYPE_CODES[out.dtype], out_stride, workspace.data_ptr() if nbytes else None, nbytes)
+    return out

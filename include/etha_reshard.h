@@ -370,6 +370,16 @@ int etha_int8_matmul(const int8_t* x, const float* x_scale, uint64_t rows, int64
                      int64_t out_stride, void* stream);
 
 /*
+ * A linear layer over 8-bit weights: the rows of x go to 8 bits as etha_quantize_rows does it and through the product as
+ * etha_int8_matmul does it, with the same bits.  The workspace (16-byte aligned, at least the bytes that
+ * etha_int8_linear_workspace names, which may be none) may be used again once the launches have finished.
+ */
+int etha_int8_linear_workspace(uint64_t rows, uint64_t width, uint64_t* bytes);
+int etha_int8_linear(const void* x, uint32_t dtype, uint64_t rows, int64_t x_stride, const int8_t* w, const float* w_scale,
+                     uint64_t cols, int64_t w_stride, uint64_t width, const float* bias, void* out, uint32_t out_dtype,
+                     int64_t out_stride, void* workspace, uint64_t workspace_bytes, void* stream);
+
+/*
  * Products grouped by expert.  Rows [offsets[e], offsets[e+1]) of x belong to expert e (offsets: n_groups + 1 entries on
  * the device; an entry outside [0, rows] or below an earlier one is taken as the nearest that is not).
  * etha_grouped_matmul: out[t,:] = x[t,:] * w[e]^T with w[e] a [cols, red] matrix, or x[t,:] * w[e] with w[e] a [red, cols]

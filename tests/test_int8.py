@@ -95,6 +95,15 @@ def test_entry_points_refuse_what_they_cannot_take():
     assert mul(m=1 << 31) == nat.ERR_UNSUPPORTED
     assert mul(x=None) == nat.ERR_INVALID and mul(ws=None) == nat.ERR_INVALID and mul(o=None) == nat.ERR_INVALID
     assert mul(m=0) == 0 and mul(n=0) == 0
+    lin = lambda **k: lib.etha_int8_linear(*{**dict(x=0x1000, d=nat.BF16, m=40, xp=16, w=0x1000, ws=0x1000, n=4, wp=16, k=16, b=None, o=0x1000,
+                                                    od=nat.BF16, op=4, wk=0x1000, wb=1 << 20, st=None), **k}.values())
+    assert lin(k=131072) == nat.ERR_UNSUPPORTED and lin(d=nat.I8) == nat.ERR_UNSUPPORTED and lin(od=nat.F64) == nat.ERR_UNSUPPORTED
+    assert lin(x=None) == nat.ERR_INVALID and lin(ws=None) == nat.ERR_INVALID and lin(o=None) == nat.ERR_INVALID
+    assert lin(wk=None) == nat.ERR_INVALID and lin(wb=16) == nat.ERR_INVALID and lin(wk=0x1008) == nat.ERR_INVALID
+    assert lin(m=0) == 0 and lin(n=0) == 0
+    assert nat.int8_linear_workspace(0, 100) == 0 and nat.int8_linear_workspace(40, 100) == 40 * 112 + 160
+    with pytest.raises(nat.EthaNativeError):
+        nat.int8_linear_workspace(1, 131072)
 
 
 # ---- rows -------------------------------------------------------------------------------------------------------------
