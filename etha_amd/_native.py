@@ -153,7 +153,7 @@ _SIGNATURES = {
     "etha_quantize_rows": (c_int, [c_void_p, c_uint32, c_uint64, c_uint64, c_int64, c_void_p, c_int64, c_void_p, c_void_p]),
     "etha_int8_matmul": (c_int, [c_void_p, c_void_p, c_uint64, c_int64, c_void_p, c_void_p, c_uint64, c_int64, c_uint64, c_void_p,
                                  c_void_p, c_uint32, c_int64, c_void_p]),
-    "etha_int8_linear_workspace": (c_int, [c_uint64, c_uint64, POINTER(c_uint64)]),
+    "etha_int8_linear_workspace": (c_int, [c_uint64, c_uint64, c_uint64, POINTER(c_uint64)]),
     "etha_int8_linear": (c_int, [c_void_p, c_uint32, c_uint64, c_int64, c_void_p, c_void_p, c_uint64, c_int64, c_uint64, c_void_p,
                                  c_void_p, c_uint32, c_int64, c_void_p, c_uint64, c_void_p]),
     "etha_grouped_matmul": (c_int, [c_void_p, c_uint32, c_uint64, c_int64, c_void_p, c_uint64, c_uint64, c_uint64, c_int64, c_int64,
@@ -432,10 +432,10 @@ def embedding_grad_workspace(n_tokens: int, n_rows: int, width: int, grad_dtype:
     return out.value
 
 
-def int8_linear_workspace(rows: int, width: int) -> int:
+def int8_linear_workspace(rows: int, cols: int, width: int) -> int:
     """Bytes of workspace that ``etha_int8_linear`` needs for these sizes."""
     out = c_uint64()
-    _check("etha_int8_linear_workspace", lib().etha_int8_linear_workspace(rows, width, byref(out)))
+    _check("etha_int8_linear_workspace", lib().etha_int8_linear_workspace(rows, cols, width, byref(out)))
     return out.value
 
 

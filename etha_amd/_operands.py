@@ -92,8 +92,9 @@ def check_out(what: str, out: torch.Tensor, shape, dtypes, *inputs: torch.Tensor
 
 def refuse_grad(what: str, *inputs: torch.Tensor | None) -> None:
     """For operators without a gradient: a silent cut of the graph would train on nothing."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in inputs):
-        raise RuntimeError(f"{what} has no gradient: call it under torch.no_grad() or detach its inputs")
+    for t in inputs:
+        if t is not None and t.requires_grad and torch.is_grad_enabled():
+            raise RuntimeError(f"{what} has no gradient: call it under torch.no_grad() or detach its inputs")
 
 
 def refuse_captured_backward(what: str) -> None:
@@ -103,12 +104,21 @@ def refuse_captured_backward(what: str) -> None:
         raise RuntimeError(f"the backward pass of {what} cannot be captured into a graph: capture a call of its gradient function")
 
 
-def call(device: torch.device, func, name: str, *args) -> None:
-    """``func(*args, stream)`` on the current stream of ``device``, which becomes the current device for the call."""
-    if device.index != torch.cuda.current_device():
+_current_device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else None
+_current_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else None
+
+
+def call(device: torch.device, name: str, *args) -> None:
+    """Entry point ``name`` with ``args`` and the current stream of ``device``, which is the current device for the call.
+
+    Where a kernel takes a few microseconds the host is what a call costs: stream and device are asked for without the
+    objects that ``torch.cuda`` wraps them in.
+    """
+    index = device.index
+    if index != _current_device():
         with torch.cuda.device(device):
-            rc = func(*args, torch.cuda.current_stream(device).cuda_stream)
+            rc = getattr(_native.lib(), name)(*args, _current_stream(index))
     else:
-        rc = func(*args, torch.cuda.current_stream(device).cuda_stream)
+        rc = getattr(_native.lib(), name)(*args, _current_stream(index))
     if rc != 0:
         _native._check(name, rc)

@@ -398,10 +398,7 @@ __global__ __launch_bounds__(S::kThreads) void etha_matmul_kernel(const MatmulAr
   };
   u32x4 fp[2][kFm], fq[2][kFn];
   // fragments to read in a row of matrix instructions: done well before the barrier waits for them
-#ifndef READ_ROWS
-#define READ_ROWS 3 / 4
-#endif
-  constexpr int kReads = kFm + kFn, kReadRows = kFm * READ_ROWS > 0 ? kFm * READ_ROWS : 1, kReadsRow = (kReads + kReadRows - 1) / kReadRows;
+  constexpr int kReads = kFm + kFn, kReadRows = kFm * 3 / 4 > 0 ? kFm * 3 / 4 : 1, kReadsRow = (kReads + kReadRows - 1) / kReadRows;
   const auto read = [&](int set, const char* from, int half, int t) {
     if (t < kFn) fq[set][t] = OpQ::fragment(from + OpP::kBytes, wc + t * 16, half * 4);
     else fp[set][t - kFn] = OpP::fragment(from, wr + (t - kFn) * 16, half * 4);
@@ -531,13 +528,16 @@ __global__ __launch_bounds__(S::kThreads) void etha_matmul_kernel(const MatmulAr
 }
 
 // ---- few rows --------------------------------------------------------------------------------------------------------
-// Up to 16 rows against a matrix: what counts is that the matrix streams.  A workgroup of 8 waves takes 32 columns and
-// each wave every eighth 128-byte line of k, straight from memory into the registers that the matrix instructions read (a
-// lane takes 32 bytes of a line; both operands are read in that order, so the order of k does not matter), no LDS and no
-// barrier on the way; the eight partial sums are added up in LDS in the waves' order.
+// A few rows against a matrix: what counts is that the matrix streams.  A workgroup of 8 waves takes 16 columns and
+// each wave every eighth 128-byte line of k.  A load brings 8 rows of one line, whole lines and not kept in the caches:
+// read by itself a 235 MB matrix comes in at 6.1 TB/s that way, at 4.1 to 5.3 TB/s where an instruction reads 64 bytes of
+// each of 16 rows as the matrix instructions want them.  A corner of LDS that is the wave's own turns one layout into the
+// other, without a barrier.  The eight partial sums are added up in LDS in the waves' order.
 // With SX the rows come as floating-point numbers and are converted to 8 bits in the workgroup, into LDS, while the first
 // lines of the matrix are on their way: one launch instead of two.
-constexpr int kFewRows = 16, kFewCols = 32, kFewWaves = 8, kFewThreads = kFewWaves * 64, kFewAhead = 4;
+// MT blocks of 16 rows share what is read of the matrix.
+constexpr int kFewCols = 16, kFewWaves = 8, kFewThreads = kFewWaves * 64;
+constexpr int kFewConverted = 4;     // rows that are converted here: every 16 columns read them again
 constexpr uint32_t kFewLds = 32768;  // bytes of converted rows at most
 
 struct FewArgs {
@@ -546,140 +546,178 @@ struct FewArgs {
   int64_t x_stride;  // elements
 };
 
-template <typename E, uint32_t KIND, typename D, typename SX>
+template <typename E, uint32_t KIND, typename D, typename SX, int MT>
 __global__ __launch_bounds__(kFewThreads) void etha_few_rows_kernel(const FewArgs few) {
   constexpr bool kConvert = !std::is_void_v<SX>;
+  constexpr int kRows = MT * 16, kAhead = MT == 1 ? 4 : 2;
+  typedef typename std::conditional<E::kEs == 1, int, float>::type sum_t;
   const MatmulArgs& a = few.m;
-  __shared__ typename std::conditional<E::kEs == 1, int, float>::type s_sum[kFewWaves][kFewRows * kFewCols];
-  __shared__ __align__(16) char s_x[kConvert ? kFewLds + kFewRows * 160 : 16];
-  __shared__ uint32_t s_top[kConvert ? kFewRows : 1][kFewWaves];
+  // a line of 16 columns and of the rows, later the sums; all of it the wave's own until the last barrier
+  __shared__ __align__(1024) char s_turn[kFewWaves][2048 + (kConvert ? 0 : MT * 2048)];
+  __shared__ __align__(16) char s_x[kConvert ? kFewLds + kFewConverted * 32 : 16];
+  __shared__ uint32_t s_top[kConvert ? kFewConverted : 1][kFewWaves];
   const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const uint32_t col_tiles = (a.cols + kFewCols - 1) / kFewCols;
   const uint32_t col0 = blockIdx.x % col_tiles * kFewCols, row_id = blockIdx.x / col_tiles;
-  uint32_t row0 = row_id * kFewRows, row_end = a.rows, red = a.red;
+  uint32_t row0 = row_id * kRows, row_end = a.rows, red = a.red;
   const char *p = a.p, *q = a.q;
   if constexpr (KIND != kPlain) {
-    const GroupTile g = find_tile<kFewRows>(a, row_id);
+    const GroupTile g = find_tile<kRows>(a, row_id);
     if (!g.found) return;
-    row0 = g.lo + g.tile * kFewRows;
+    row0 = g.lo + g.tile * kRows;
     row_end = g.hi;
     if (g.group == a.n_groups) red = 0;
     else q += (int64_t)g.group * a.q_group_stride;
   }
-  const uint32_t n_rows = row_end - row0 < kFewRows ? row_end - row0 : kFewRows;
+  const uint32_t n_rows = row_end - row0 < kRows ? row_end - row0 : kRows;
   const int64_t bytes = (int64_t)red * E::kEs;
   const uint32_t whole = (uint32_t)(bytes / 128);
-  const uint32_t at = (lane >> 4) * 32, r = lane & 15;
-  const uint32_t xr = r < n_rows ? r : n_rows - 1;  // rows past the last repeat it; their results are dropped
-  const char* xp = p + (int64_t)(row0 + xr) * a.p_stride + at;
-  const char* wp[2];
+  // a load: row lane >> 3 of 8, piece lane & 7 of its line; columns past the last repeat it, rows past the last are not read
+  const uint32_t lrow = lane >> 3, at = (lane & 7) * 16;
+  const char *wp[2], *xp[2 * MT];
   #pragma unroll
   for (int j = 0; j < 2; j++) {
-    const uint32_t c = col0 + j * 16 + r;
+    const uint32_t c = col0 + j * 8 + lrow;
     wp[j] = q + (int64_t)(c < a.cols ? c : a.cols - 1) * a.q_stride + at;
   }
-  const uint32_t pitch = (uint32_t)(bytes + 127) / 128 * 128 + 32;  // of converted rows
-  typename E::acc acc[2] = {};
-  u32x4 w[kFewAhead][2][2], x[kFewAhead][2];
-  const auto load_w = [&](uint32_t line) {
+  #pragma unroll
+  for (int j = 0; j < 2 * MT; j++) xp[j] = p + (int64_t)(row0 + j * 8 + lrow) * a.p_stride + at;
+  char* turn = s_turn[wave];
+  const uint32_t put = lrow * 128 + (((lane & 7) ^ lrow) << 4);
+  const uint32_t r = lane & 15, pitch = (uint32_t)(bytes + 127) / 128 * 128 + 32;  // of converted rows
+  typename E::acc acc[MT] = {};
+  u32x4 w[kAhead][2], x[kAhead][2 * MT] = {};
+  const auto load = [&](uint32_t line) {
     #pragma unroll
-    for (int u = 0; u < kFewAhead; u++)
+    for (int u = 0; u < kAhead; u++) {
+      const int64_t k = (int64_t)(line + u * kFewWaves) * 128;
       #pragma unroll
-      for (int j = 0; j < 2; j++)
+      for (int j = 0; j < 2; j++) w[u][j] = load_raw<16, true>(wp[j] + k);
+      if constexpr (!kConvert) {
         #pragma unroll
-        for (int h = 0; h < 2; h++) w[u][j][h] = load_raw<16, true>(wp[j] + (int64_t)(line + u * kFewWaves) * 128 + h * 16);
+        for (int j = 0; j < 2 * MT; j++)
+          if (j * 8 + lrow < n_rows) x[u][j] = load_raw<16>(xp[j] + k);
+      }
+    }
   };
-  const auto load_x = [&](int u, uint32_t line) {
+  const auto multiply = [&](int u, uint32_t line) {
+    #pragma unroll
+    for (int j = 0; j < 2; j++) *(u32x4*)(turn + j * 1024 + put) = w[u][j];
+    if constexpr (!kConvert) {
+      #pragma unroll
+      for (int j = 0; j < 2 * MT; j++)
+        if (j * 8 < n_rows) *(u32x4*)(turn + 2048 + j * 1024 + put) = x[u][j];
+    }
     #pragma unroll
     for (int h = 0; h < 2; h++) {
-      if constexpr (kConvert) x[u][h] = *(const u32x4*)(s_x + xr * pitch + line * 128 + at + h * 16);
-      else x[u][h] = load_raw<16>(xp + (int64_t)line * 128 + h * 16);
+      const uint32_t piece = h * 4 + (lane >> 4), get = r * 128 + ((piece ^ (r & 7)) << 4);
+      const u32x4 fw = *(const u32x4*)(turn + get);
+      #pragma unroll
+      for (int m = 0; m < MT; m++) {
+        if (m * 16 >= n_rows) break;
+        const uint32_t xr = m * 16 + r < n_rows ? m * 16 + r : n_rows - 1;  // rows past the last repeat it, and are dropped
+        u32x4 fx;
+        if constexpr (kConvert) fx = *(const u32x4*)(s_x + xr * pitch + line * 128 + piece * 16);
+        else fx = *(const u32x4*)(turn + 2048 + xr * 128 + ((piece ^ (xr & 7)) << 4));
+        acc[m] = E::mfma(fw, fx, acc[m]);
+      }
     }
   };
-  const auto multiply = [&](int u) {
-    #pragma unroll
-    for (int h = 0; h < 2; h++)
-      #pragma unroll
-      for (int j = 0; j < 2; j++) acc[j] = E::mfma(w[u][j][h], x[u][h], acc[j]);
-  };
-  // lines wave, wave + 8, ...: batches of kFewAhead of them, then one by one
+  // lines wave, wave + 8, ...: batches of kAhead of them, then one by one
   uint32_t line = wave;
-  const auto batch = [&]() { return line + (kFewAhead - 1) * kFewWaves < whole; };
+  const auto batch = [&]() { return line + (kAhead - 1) * kFewWaves < whole; };
   const bool early = batch();
-  if (early) load_w(line);
+  if (early) load(line);
   if constexpr (kConvert) {
     const typename SX::bits* rows = (const typename SX::bits*)few.x;
-    for (uint32_t m = 0; m < n_rows; m++) {
-      uint32_t top = 0;
-      for (uint32_t k = threadIdx.x * 8; k < red; k += kFewThreads * 8) {
-        float v[8];
-        load_f32<SX, 8>(v, rows + (int64_t)(row0 + m) * few.x_stride + k, (int64_t)red - k);
-        top = largest_bits(v, top);
+    const uint32_t k0 = threadIdx.x * 8;
+    float kept[kFewConverted][8];  // the first 4096 of a row stay in registers, all rows' loads are on their way at once
+    #pragma unroll
+    for (uint32_t m = 0; m < kFewConverted; m++)
+      if (m < n_rows) load_f32<SX, 8>(kept[m], rows + (int64_t)(row0 + m) * few.x_stride + k0, (int64_t)red - k0);
+    #pragma unroll
+    for (uint32_t m = 0; m < kFewConverted; m++)
+      if (m < n_rows) {
+        uint32_t top = largest_bits(kept[m], 0);
+        for (uint32_t k = k0 + kFewThreads * 8; k < red; k += kFewThreads * 8) {
+          float v[8];
+          load_f32<SX, 8>(v, rows + (int64_t)(row0 + m) * few.x_stride + k, (int64_t)red - k);
+          top = largest_bits(v, top);
+        }
+        top = wave_max(top);
+        if (lane == 0) s_top[m][wave] = top;
       }
-      top = wave_max(top);
-      if (lane == 0) s_top[m][wave] = top;
-    }
     __syncthreads();
-    for (uint32_t m = 0; m < n_rows; m++) {
-      uint32_t top = 0;
-      #pragma unroll
-      for (int i = 0; i < kFewWaves; i++) top = s_top[m][i] > top ? s_top[m][i] : top;
-      const RowScale scale(top);
-      for (uint32_t k = threadIdx.x * 8; k < pitch - 32; k += kFewThreads * 8) {
-        float v[8];
-        load_f32<SX, 8>(v, rows + (int64_t)(row0 + m) * few.x_stride + k, (int64_t)red - k);
-        *(u32x2*)(s_x + m * pitch + k) = scale.pack(v);  // past the end of k: zeros
+    #pragma unroll
+    for (uint32_t m = 0; m < kFewConverted; m++)
+      if (m < n_rows) {
+        uint32_t top = 0;
+        #pragma unroll
+        for (int i = 0; i < kFewWaves; i++) top = s_top[m][i] > top ? s_top[m][i] : top;
+        const RowScale scale(top);
+        if (k0 < pitch - 32) *(u32x2*)(s_x + m * pitch + k0) = scale.pack(kept[m]);  // past the end of k: zeros
+        for (uint32_t k = k0 + kFewThreads * 8; k < pitch - 32; k += kFewThreads * 8) {
+          float v[8];
+          load_f32<SX, 8>(v, rows + (int64_t)(row0 + m) * few.x_stride + k, (int64_t)red - k);
+          *(u32x2*)(s_x + m * pitch + k) = scale.pack(v);
+        }
       }
-    }
     __syncthreads();
   }
   if (early) {
     for (;;) {
       #pragma unroll
-      for (int u = 0; u < kFewAhead; u++) load_x(u, line + u * kFewWaves);
-      #pragma unroll
-      for (int u = 0; u < kFewAhead; u++) multiply(u);
-      line += kFewAhead * kFewWaves;
+      for (int u = 0; u < kAhead; u++) multiply(u, line + u * kFewWaves);
+      line += kAhead * kFewWaves;
       if (!batch()) break;
-      load_w(line);
+      load(line);
     }
   }
   for (; line * 128 < bytes; line += kFewWaves) {
     #pragma unroll
-    for (int h = 0; h < 2; h++) {
-      const int64_t left = bytes - (int64_t)line * 128 - at - h * 16;
-      #pragma unroll
-      for (int j = 0; j < 2; j++) w[0][j][h] = load_part<E::kEs>(wp[j] + (int64_t)line * 128 + h * 16, left);
-      if constexpr (!kConvert) x[0][h] = load_part<E::kEs>(xp + (int64_t)line * 128 + h * 16, left);
+    for (int j = 0; j < 2; j++) {
+      const int64_t k = (int64_t)line * 128, left = bytes - k - at;
+      w[0][j] = load_part<E::kEs>(wp[j] + k, left);
     }
-    if constexpr (kConvert) load_x(0, line);
-    multiply(0);
+    if constexpr (!kConvert) {
+      #pragma unroll
+      for (int j = 0; j < 2 * MT; j++) {
+        const int64_t k = (int64_t)line * 128, left = bytes - k - at;
+        if (j * 8 + lrow < n_rows) x[0][j] = load_part<E::kEs>(xp[j] + k, left);
+      }
+    }
+    multiply(0, line);
   }
+  sum_t* sums = (sum_t*)turn;
   #pragma unroll
-  for (int j = 0; j < 2; j++)
+  for (int m = 0; m < MT; m++)
     #pragma unroll
-    for (int c = 0; c < 4; c++) s_sum[wave][j * 256 + lane * 4 + c] = acc[j][c];
+    for (int c = 0; c < 4; c++) sums[m * 256 + lane * 4 + c] = acc[m][c];
   __syncthreads();
-  const uint32_t t = threadIdx.x, row = row0 + (t >> 2 & 15), col = col0 + (t >> 8) * 16 + (t >> 6 & 3) * 4 + (t & 3);
-  if (row >= row_end || col >= a.cols) return;
-  auto sum = s_sum[0][t];
   #pragma unroll
-  for (int i = 1; i < kFewWaves; i++) sum += s_sum[i][t];
-  float v = (float)sum;
-  if constexpr (E::kEs == 1) {
-    float row_scale;
-    if constexpr (kConvert) {
-      uint32_t top = 0;
-      #pragma unroll
-      for (int i = 0; i < kFewWaves; i++) top = s_top[row - row0][i] > top ? s_top[row - row0][i] : top;
-      row_scale = RowScale(top).scale;
-    } else {
-      row_scale = a.row_scale[row];
+  for (int e = 0; e < (MT + 1) / 2; e++) {
+    const uint32_t t = threadIdx.x + e * kFewThreads;
+    const uint32_t row = row0 + (t >> 8) * 16 + (t >> 2 & 15), col = col0 + (t >> 6 & 3) * 4 + (t & 3);
+    if (t >= kRows * kFewCols || row >= row_end || col >= a.cols) continue;
+    sum_t sum = ((const sum_t*)s_turn[0])[t];
+    #pragma unroll
+    for (int i = 1; i < kFewWaves; i++) sum += ((const sum_t*)s_turn[i])[t];
+    float v = (float)sum;
+    if constexpr (E::kEs == 1) {
+      float row_scale;
+      if constexpr (kConvert) {
+        uint32_t top = 0;
+        #pragma unroll
+        for (int i = 0; i < kFewWaves; i++) top = s_top[row - row0][i] > top ? s_top[row - row0][i] : top;
+        row_scale = RowScale(top).scale;
+      } else {
+        row_scale = a.row_scale[row];
+      }
+      v *= row_scale * a.col_scale[col];
+      if (a.bias) v += a.bias[col];
     }
-    v *= row_scale * a.col_scale[col];
-    if (a.bias) v += a.bias[col];
+    ((typename D::bits*)a.out)[(int64_t)row * a.out_stride + col] = D::from_f32(v);
   }
-  ((typename D::bits*)a.out)[(int64_t)row * a.out_stride + col] = D::from_f32(v);
 }
 
 int launched(const char* name) {
@@ -704,6 +742,12 @@ bool is_direct(const void* base, int64_t stride, int64_t group_stride, uint64_t 
          (trans ? (uint64_t)stride >= across * 2 : !(k_bytes & 15));
 }
 
+// Tile shapes.  Measured on grouped bf16 products, 8 x [3584, 4096]: 256 x 256 with 8 waves 433 us at 16384 rows (4 waves
+// 600 us, stages of 64 bytes of k 465 us), 128 x 128 with 8 waves 59 us at 1024 rows (4 waves 87 us), 32 x 64 52 us at 256.
+typedef Shape<256, 256, 2, 4, 2> ShapeL;
+typedef Shape<128, 128, 2, 4, 2> ShapeM;  // also for operands that go through registers
+typedef Shape<32, 64, 1, 4, 6> ShapeS;
+
 // No group wastes more than one row tile, and a group with rows has at least one.
 uint64_t row_tiles_of(const MatmulArgs& a, uint32_t kind, int bm) {
   if (kind == kPlain) return ((uint64_t)a.rows + bm - 1) / bm;
@@ -722,48 +766,65 @@ int launch_matmul(const char* what, const MatmulArgs& a, void* stream) {
   return launched("etha_matmul_kernel");
 }
 
-#ifndef SHAPE_L
-#define SHAPE_L 256, 256, 2, 4, 2
-#endif
-#ifndef SHAPE_M
-#define SHAPE_M 128, 128, 2, 4, 2
-#endif
-#ifndef SHAPE_S
-#define SHAPE_S 32, 64, 1, 4, 6
-#endif
-#ifndef SHAPE_R
-#define SHAPE_R 128, 128, 2, 4, 2
-#endif
-typedef Shape<SHAPE_R> ShapeR;
-typedef Shape<SHAPE_L> ShapeL;
-typedef Shape<SHAPE_M> ShapeM;
-typedef Shape<SHAPE_S> ShapeS;
 
-template <typename E, uint32_t KIND, typename D, typename SX>
+template <typename E, uint32_t KIND, typename D, typename SX, int MT>
 int launch_few(const char* what, const FewArgs& few, void* stream) {
-  const uint64_t blocks = row_tiles_of(few.m, KIND, kFewRows) * (((uint64_t)few.m.cols + kFewCols - 1) / kFewCols);
+  const uint64_t blocks = row_tiles_of(few.m, KIND, MT * 16) * (((uint64_t)few.m.cols + kFewCols - 1) / kFewCols);
   if (blocks >= 1ull << 22) return fail(ETHA_ERR_UNSUPPORTED, "%s: the product is too large for one call", what);
-  hipLaunchKernelGGL((etha_few_rows_kernel<E, KIND, D, SX>), dim3((uint32_t)blocks), dim3(kFewThreads), 0, (hipStream_t)stream, few);
+  hipLaunchKernelGGL((etha_few_rows_kernel<E, KIND, D, SX, MT>), dim3((uint32_t)blocks), dim3(kFewThreads), 0, (hipStream_t)stream, few);
   return launched("etha_few_rows_kernel");
+}
+
+// What a choice of tiles costs, in microseconds, by what bounded the shapes where they were measured: a workgroup takes in
+// its operands at about 45 GB/s, all of them together at about 11 TB/s, and the matrices come from memory at `gbs`.  A rule
+// on sizes alone; the rows of a group are taken as even, half a tile a group as lost.
+double tile_cost(const MatmulArgs& a, uint32_t kind, int es, int bm, int bn, int resident, double gbs) {
+  const double k_bytes = (double)a.red * es;
+  const double groups = kind == kPlain ? 1 : a.n_groups < a.rows ? (a.n_groups ? a.n_groups : 1) : a.rows;
+  const double high = a.rows / groups < bm ? a.rows / groups : bm;  // rows of a tile that there are
+  double row_tiles = kind == kPlain ? (double)((a.rows + bm - 1) / bm) : a.rows / (double)bm + groups / 2;
+  if (row_tiles < groups) row_tiles = groups;
+  const double tiles = row_tiles * ((a.cols + bn - 1) / bn), bytes = (high + bn) * k_bytes;
+  const double rounds = (double)(uint64_t)((tiles + resident - 1) / resident);
+  double us = rounds * bytes / 45e3;
+  if (tiles * bytes / 11e6 > us) us = tiles * bytes / 11e6;
+  if (groups * a.cols * k_bytes / gbs / 1e3 > us) us = groups * a.cols * k_bytes / gbs / 1e3;
+  return us;
 }
 
 template <typename E, uint32_t KIND, typename D>
 int shaped_matmul(const char* what, const MatmulArgs& a, bool direct, void* stream) {
-  // rows a group has on average: the height of the tiles that it fills
-  const uint64_t rows = KIND == kGroupRows || KIND == kGroupRowsT ? a.rows / (a.n_groups ? a.n_groups : 1) : a.rows;
-  const auto tiles = [&](int bm, int bn) { return row_tiles_of(a, KIND, bm) * (((uint64_t)a.cols + bn - 1) / bn); };
-  if constexpr (KIND == kPlain || KIND == kGroupRows) {
-    if (rows <= kFewRows) {
-      FewArgs few = {};
-      few.m = a;
-      return launch_few<E, KIND, D, void>(what, few, stream);
+  if constexpr (KIND == kGroupReduce) {
+    // the tall reduction pays for the large tile from about a stage or two of rows on, if there are tiles for every CU
+    const uint64_t tiles = row_tiles_of(a, KIND, ShapeL::BM) * (((uint64_t)a.cols + ShapeL::BN - 1) / ShapeL::BN);
+    if (!direct) return launch_matmul<E, KIND, D, ShapeM, RegisterStage>(what, a, stream);
+    if (tiles >= 192 && a.red / a.n_groups >= 96) return launch_matmul<E, KIND, D, ShapeL, DirectStage>(what, a, stream);
+    return launch_matmul<E, KIND, D, ShapeM, DirectStage>(what, a, stream);
+  } else {
+    double cost[6];
+    const double none = 1e30;
+    const bool few = KIND != kGroupRowsT;
+    cost[0] = few ? tile_cost(a, KIND, E::kEs, 16, kFewCols, 512, 6000) : none;
+    cost[1] = few ? tile_cost(a, KIND, E::kEs, 32, kFewCols, 512, 6000) : none;
+    cost[2] = few ? tile_cost(a, KIND, E::kEs, 64, kFewCols, 256, 6000) : none;
+    cost[3] = tile_cost(a, KIND, E::kEs, ShapeS::BM, ShapeS::BN, 512, 4600);
+    cost[4] = tile_cost(a, KIND, E::kEs, ShapeM::BM, ShapeM::BN, 512, 5200);
+    cost[5] = direct ? tile_cost(a, KIND, E::kEs, ShapeL::BM, ShapeL::BN, 256, 4600) : none;
+    int best = 0;
+    for (int i = 1; i < 6; i++)
+      if (cost[i] < cost[best]) best = i;
+    if constexpr (few) {
+      FewArgs args = {};
+      args.m = a;
+      if (best == 0) return launch_few<E, KIND, D, void, 1>(what, args, stream);
+      if (best == 1) return launch_few<E, KIND, D, void, 2>(what, args, stream);
+      if (best == 2) return launch_few<E, KIND, D, void, 4>(what, args, stream);
     }
-  }
-  if (rows <= 32 && KIND != kGroupReduce)
+    if (best == 5) return launch_matmul<E, KIND, D, ShapeL, DirectStage>(what, a, stream);
+    if (best == 4)
+      return direct ? launch_matmul<E, KIND, D, ShapeM, DirectStage>(what, a, stream) : launch_matmul<E, KIND, D, ShapeM, RegisterStage>(what, a, stream);
     return direct ? launch_matmul<E, KIND, D, ShapeS, DirectStage>(what, a, stream) : launch_matmul<E, KIND, D, ShapeS, RegisterStage>(what, a, stream);
-  if (!direct) return launch_matmul<E, KIND, D, ShapeR, RegisterStage>(what, a, stream);
-  if (rows > 128 && tiles(ShapeL::BM, ShapeL::BN) >= 192) return launch_matmul<E, KIND, D, ShapeL, DirectStage>(what, a, stream);
-  return launch_matmul<E, KIND, D, ShapeM, DirectStage>(what, a, stream);
+  }
 }
 
 template <typename E, uint32_t KIND>
@@ -779,8 +840,13 @@ int run_matmul(const char* what, const MatmulArgs& a, uint32_t out_dtype, void* 
 
 bool is_out(uint32_t dtype) { return dtype == ETHA_F32 || dtype == ETHA_BF16 || dtype == ETHA_F16; }
 
-// Rows that the few-rows kernel converts itself: it reads them once for every 32 columns, so there must not be many of them.
-bool is_few(uint64_t rows, uint64_t width) { return rows <= 4 && rows * ((width + 127) / 128 * 128) <= kFewLds; }
+// Rows that the few-rows kernel converts itself.  Every 16 columns convert them again while their part of the matrix
+// arrives: one row costs less than a launch (14336 x 4096: 14.2 us, 16.5 us with a launch of its own), further rows do where
+// the workgroups are all resident and a row fits the registers (1024 x 4096: 9.5 us for 4 rows, 13 us; 14336 x 4096: 24 us).
+bool is_few(uint64_t rows, uint64_t cols, uint64_t width) {
+  const uint64_t padded = (width + 127) / 128 * 128;
+  return padded <= kFewLds && (rows == 1 || (rows <= kFewConverted && cols <= 8192 && padded <= kFewThreads * 8));
+}
 uint64_t padded_width(uint64_t width) { return (width + 15) / 16 * 16; }
 
 template <uint32_t KIND>
@@ -824,11 +890,11 @@ int etha_int8_matmul(const int8_t* x, const float* x_scale, uint64_t rows, int64
   return run_matmul<ElemI8, kPlain>("etha_int8_matmul", a, out_dtype, stream);
 }
 
-int etha_int8_linear_workspace(uint64_t rows, uint64_t width, uint64_t* bytes) {
+int etha_int8_linear_workspace(uint64_t rows, uint64_t cols, uint64_t width, uint64_t* bytes) {
   if (!bytes) return fail(ETHA_ERR_INVALID, "etha_int8_linear_workspace: null result");
-  const int rc = check_sizes("etha_int8_linear_workspace", rows, 0, width, ETHA_INT8_MAX_WIDTH);
+  const int rc = check_sizes("etha_int8_linear_workspace", rows, cols, width, ETHA_INT8_MAX_WIDTH);
   if (rc != ETHA_OK) return rc;
-  *bytes = is_few(rows, width) ? 0 : rows * padded_width(width) + rows * 4;
+  *bytes = is_few(rows, cols, width) ? 0 : rows * padded_width(width) + rows * 4;
   return ETHA_OK;
 }
 
@@ -840,7 +906,7 @@ int etha_int8_linear(const void* x, uint32_t dtype, uint64_t rows, int64_t x_str
   if (!is_out(dtype) || !is_out(out_dtype)) return fail(ETHA_ERR_UNSUPPORTED, "etha_int8_linear: element types are f32, bf16 and f16");
   if (!rows || !cols) return ETHA_OK;
   if ((width && (!x || !w)) || !w_scale || !out) return fail(ETHA_ERR_INVALID, "etha_int8_linear: null tensor");
-  if (is_few(rows, width)) {
+  if (is_few(rows, cols, width)) {
     FewArgs few = {};
     few.x = x;
     few.x_stride = x_stride;
@@ -855,7 +921,7 @@ int etha_int8_linear(const void* x, uint32_t dtype, uint64_t rows, int64_t x_str
     few.m.bias = bias;
     with_type(dtype, [&](auto s) {
       with_type(out_dtype, [&](auto d) {
-        rc = launch_few<ElemI8, kPlain, decltype(d), decltype(s)>("etha_int8_linear", few, stream);
+        rc = launch_few<ElemI8, kPlain, decltype(d), decltype(s), 1>("etha_int8_linear", few, stream);
       });
     });
     return rc;

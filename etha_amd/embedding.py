@@ -43,7 +43,7 @@ def _lookup(tokens, weight, scale, first_row, dtype, out):
         out_stride = check_out("embedding", out, (*tokens.shape, width), DTYPE_CODES, tokens, weight)
         out_code = DTYPE_CODES[out.dtype]
         device = check_device("embedding", weight, tokens, out)
-    call(device, _native.lib().etha_embedding, "etha_embedding", source.data_ptr(), token_code, tokens.numel(), weight.data_ptr(),
+    call(device, "etha_embedding", source.data_ptr(), token_code, tokens.numel(), weight.data_ptr(),
          weight_code, rows, width, stride, first_row, scale, out.data_ptr(), out_code, out_stride)
     return out
 
@@ -110,7 +110,7 @@ def embedding_grad(grad: torch.Tensor, tokens: torch.Tensor, n_rows: int, *, sca
         device = check_device("embedding_grad", grad, tokens, out)
     nbytes = _native.embedding_grad_workspace(n_tokens, n_rows, width, grad_code)
     workspace = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
-    call(device, _native.lib().etha_embedding_grad, "etha_embedding_grad", grad.data_ptr(), grad_code, grad_stride, source.data_ptr(),
+    call(device, "etha_embedding_grad", grad.data_ptr(), grad_code, grad_stride, source.data_ptr(),
          token_code, n_tokens, n_rows, width, first_row, scale, out.data_ptr(), out_code, out_stride, int(accumulate),
          workspace.data_ptr() if nbytes else None, nbytes)
     return out

@@ -54,7 +54,7 @@ def _product(what, x, weight, offsets, transposed, out):
     device = check_device(what, x, weight, offsets, out)
     if fresh:
         out, out_stride = torch.empty((rows, cols), dtype=x.dtype, device=device), cols
-    call(device, _native.lib().etha_grouped_matmul, "etha_grouped_matmul", source.data_ptr(), _OPERANDS[x.dtype], rows, stride,
+    call(device, "etha_grouped_matmul", source.data_ptr(), _OPERANDS[x.dtype], rows, stride,
          weight.data_ptr(), experts, cols, red, w_stride, w_group, int(transposed), offsets.data_ptr(), out.data_ptr(),
          DTYPE_CODES[out.dtype], out_stride, int(fresh))
     return out
@@ -119,7 +119,7 @@ def grouped_linear_grad_weight(grad: torch.Tensor, x: torch.Tensor, offsets: tor
     device = check_device(what, x, grad, offsets, out)
     if out is None:
         out = torch.empty((experts, n, k), dtype=dtype, device=device)
-    call(device, _native.lib().etha_grouped_matmul_reduce, "etha_grouped_matmul_reduce", g.data_ptr(), r.data_ptr(), _OPERANDS[x.dtype],
+    call(device, "etha_grouped_matmul_reduce", g.data_ptr(), r.data_ptr(), _OPERANDS[x.dtype],
          x.shape[0], g_stride, r_stride, experts, n, k, offsets.data_ptr(), out.data_ptr(), DTYPE_CODES[out.dtype], out.stride(1),
          out.stride(0))
     return out

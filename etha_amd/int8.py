@@ -41,7 +41,7 @@ def quantize_rows(x: torch.Tensor, *, values: torch.Tensor | None = None,
         values, values_stride = torch.empty(x.shape, dtype=torch.int8, device=device), width
     if scales is None:
         scales = torch.empty(x.shape[:-1], dtype=torch.float32, device=device)
-    call(device, _native.lib().etha_quantize_rows, "etha_quantize_rows", source.data_ptr(), code, rows, width, stride,
+    call(device, "etha_quantize_rows", source.data_ptr(), code, rows, width, stride,
          values.data_ptr(), values_stride, scales.data_ptr())
     return values, scales
 
@@ -88,7 +88,7 @@ def int8_matmul(x: torch.Tensor, x_scales: torch.Tensor, weight: torch.Tensor, w
     if out is None:
         code_of(what, dtype)
         out, out_stride = torch.empty((*x.shape[:-1], channels), dtype=dtype, device=device), channels
-    call(device, _native.lib().etha_int8_matmul, "etha_int8_matmul", source.data_ptr(), x_scales.data_ptr(), rows, stride,
+    call(device, "etha_int8_matmul", source.data_ptr(), x_scales.data_ptr(), rows, stride,
          weight.data_ptr(), weight_scales.data_ptr(), channels, w_stride, width, None if bias is None else bias.data_ptr(),
          out.data_ptr(), DTYPE_CODES[out.dtype], out_stride)
     return out
@@ -113,9 +113,9 @@ def int8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scales: torch.Tens
         dtype = dtype or x.dtype
         code_of(what, dtype)
         out, out_stride = torch.empty((*x.shape[:-1], channels), dtype=dtype, device=device), channels
-    nbytes = _native.int8_linear_workspace(rows, width)
+    nbytes = _native.int8_linear_workspace(rows, channels, width)
     workspace = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
-    call(device, _native.lib().etha_int8_linear, "etha_int8_linear", source.data_ptr(), x_code, rows, stride, weight.data_ptr(),
+    call(device, "etha_int8_linear", source.data_ptr(), x_code, rows, stride, weight.data_ptr(),
          weight_scales.data_ptr(), channels, w_stride, width, None if bias is None else bias.data_ptr(), out.data_ptr(),
          DTYPE_CODES[out.dtype], out_stride, workspace.data_ptr() if nbytes else None, nbytes)
     return out

@@ -374,7 +374,7 @@ int etha_int8_matmul(const int8_t* x, const float* x_scale, uint64_t rows, int64
  * etha_int8_matmul does it, with the same bits.  The workspace (16-byte aligned, at least the bytes that
  * etha_int8_linear_workspace names, which may be none) may be used again once the launches have finished.
  */
-int etha_int8_linear_workspace(uint64_t rows, uint64_t width, uint64_t* bytes);
+int etha_int8_linear_workspace(uint64_t rows, uint64_t cols, uint64_t width, uint64_t* bytes);
 int etha_int8_linear(const void* x, uint32_t dtype, uint64_t rows, int64_t x_stride, const int8_t* w, const float* w_scale,
                      uint64_t cols, int64_t w_stride, uint64_t width, const float* bias, void* out, uint32_t out_dtype,
                      int64_t out_stride, void* workspace, uint64_t workspace_bytes, void* stream);

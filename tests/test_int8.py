@@ -101,9 +101,9 @@ def test_entry_points_refuse_what_they_cannot_take():
     assert lin(x=None) == nat.ERR_INVALID and lin(ws=None) == nat.ERR_INVALID and lin(o=None) == nat.ERR_INVALID
     assert lin(wk=None) == nat.ERR_INVALID and lin(wb=16) == nat.ERR_INVALID and lin(wk=0x1008) == nat.ERR_INVALID
     assert lin(m=0) == 0 and lin(n=0) == 0
-    assert nat.int8_linear_workspace(0, 100) == 0 and nat.int8_linear_workspace(40, 100) == 40 * 112 + 160
+    assert nat.int8_linear_workspace(0, 8, 100) == 0 and nat.int8_linear_workspace(40, 8, 100) == 40 * 112 + 160
     with pytest.raises(nat.EthaNativeError):
-        nat.int8_linear_workspace(1, 131072)
+        nat.int8_linear_workspace(1, 8, 131072)
 
 
 # ---- rows -------------------------------------------------------------------------------------------------------------
@@ -219,7 +219,7 @@ def test_product_of_views(gpu_device):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", DTYPES, ids=str)
-@pytest.mark.parametrize("m,n,k", [(1, 515, 4096), (1, 64, 77), (3, 1000, 1001), (8, 512, 2048), (40, 200, 512), (300, 400, 640)])
+@pytest.mark.parametrize("m,n,k", [(1, 515, 4096), (1, 64, 77), (1, 40, 33001), (2, 300, 4100), (4, 9000, 256), (3, 1000, 1001), (8, 512, 2048), (40, 200, 512), (300, 400, 640)])
 def test_linear(gpu_device, m, n, k, dtype):
     gen = torch.Generator(device=gpu_device).manual_seed(m * n + k)
     _, _, w, ws = operands(gen, 1, n, k, gpu_device)
