@@ -45,10 +45,13 @@ struct LookupArgs {
   float scale;
 };
 
+// Elements of a work-item: 16 bytes of the narrower type (fp32 rows read as bf16, 16381 tokens of 4096: 20.0 us; 29.7 us
+// with 16 bytes of the wider one).
+constexpr int lookup_vec(int es, int eo) { return 16 / (es < eo ? es : eo); }
+
 template <typename S, typename D>
 __global__ __launch_bounds__(256) void etha_embedding_kernel(const LookupArgs a) {
-  constexpr int kEs = sizeof(typename S::bits) > sizeof(typename D::bits) ? sizeof(typename S::bits) : sizeof(typename D::bits);
-  constexpr int N = 16 / kEs;
+  constexpr int N = lookup_vec(sizeof(typename S::bits), sizeof(typename D::bits));
   const uint32_t sub = threadIdx.x >> a.lanes_log2, lane = threadIdx.x & ((1u << a.lanes_log2) - 1);
   const uint32_t per_block = blockDim.x >> a.lanes_log2;
   const uint64_t col = ((uint64_t)blockIdx.y << a.lanes_log2 | lane) * N;
@@ -75,7 +78,10 @@ __global__ __launch_bounds__(256) void etha_embedding_kernel(const LookupArgs a)
 // find each other with one ballot per digit bit, and the wave's running count of the digit lies in LDS.
 constexpr int kMaxBins = 512;
 constexpr uint32_t kOneBlockThreads = 1024, kOneBlockTokens = 8192;
-constexpr uint32_t kSortThreads = 256, kSortTokens = 4096;
+constexpr uint32_t kSortThreads = 256;
+// Tokens of a workgroup where there are more: every workgroup adds up the counts of all of them, so they get longer where
+// there would be more than 256 (65536 tokens: a pass takes 11 us with 64 workgroups, 29 us with 16).
+constexpr uint32_t sort_tokens(uint64_t n) { return n <= 256 * 1024 ? 1024 : 4096; }
 
 __device__ inline uint64_t same_digit(uint32_t digit, int bits) {
   uint64_t mask = ~0ull;
@@ -200,20 +206,23 @@ __device__ inline uint32_t sort_key(const SortArgs& a, uint64_t p) {
   return a.keys_in ? a.keys_in[p] : local_row(a.tokens, a.wide, p, a.first, a.n_rows);
 }
 
+template <uint32_t TOKENS>
 __global__ __launch_bounds__(kSortThreads) void etha_sort_count_kernel(const SortArgs a) {
   __shared__ uint32_t s_count[kMaxBins];
   const uint32_t bins = 1u << a.bits;
   for (uint32_t i = threadIdx.x; i < bins; i += kSortThreads) s_count[i] = 0;
   __syncthreads();
-  const uint64_t base = (uint64_t)blockIdx.x * kSortTokens;
-  for (uint32_t i = threadIdx.x; i < kSortTokens; i += kSortThreads)
+  const uint64_t base = (uint64_t)blockIdx.x * TOKENS;
+  #pragma unroll
+  for (uint32_t i = threadIdx.x; i < TOKENS; i += kSortThreads)
     if (base + i < a.n) atomicAdd(&s_count[(sort_key(a, base + i) >> a.shift) & (bins - 1)], 1u);
   __syncthreads();
   for (uint32_t i = threadIdx.x; i < bins; i += kSortThreads) a.hist[(uint64_t)blockIdx.x * bins + i] = s_count[i];
 }
 
+template <uint32_t TOKENS>
 __global__ __launch_bounds__(kSortThreads) void etha_sort_scatter_kernel(const SortArgs a) {
-  constexpr uint32_t kWaves = kSortThreads / kWave, kItems = kSortTokens / kSortThreads;
+  constexpr uint32_t kWaves = kSortThreads / kWave, kItems = TOKENS / kSortThreads;
   constexpr uint32_t kBinsPer = kMaxBins / kSortThreads;
   __shared__ uint16_t s_count[kWaves][kMaxBins];
   __shared__ uint32_t s_base[kMaxBins];
@@ -226,12 +235,14 @@ __global__ __launch_bounds__(kSortThreads) void etha_sort_scatter_kernel(const S
   for (uint32_t j = 0; j < kBinsPer; j++) {
     const uint32_t bin = tid * kBinsPer + j;
     before[j] = total[j] = 0;
-    if (bin < bins)
+    if (bin < bins) {
+      #pragma unroll 8
       for (uint32_t b = 0; b < gridDim.x; b++) {
         const uint32_t c = a.hist[(uint64_t)b * bins + bin];
         before[j] += b < blockIdx.x ? c : 0;
         total[j] += c;
       }
+    }
     sum += total[j];
   }
   uint32_t base = scan_block(sum, s_sums);
@@ -242,7 +253,7 @@ __global__ __launch_bounds__(kSortThreads) void etha_sort_scatter_kernel(const S
     base += total[j];
   }
   __syncthreads();
-  const uint64_t at0 = (uint64_t)blockIdx.x * kSortTokens + wave * (kItems * 64) + lane;
+  const uint64_t at0 = (uint64_t)blockIdx.x * TOKENS + wave * (kItems * 64) + lane;
   uint32_t key[kItems], rank[kItems];
   #pragma unroll
   for (uint32_t i = 0; i < kItems; i++) key[i] = sort_key(a, at0 + i * 64);
@@ -284,7 +295,8 @@ struct GradArgs {
   float* partial;        // [chunk][2][width]
   uint64_t n, width;
   int64_t grad_stride, out_stride;
-  uint32_t n_rows, chunk, n_chunks, n_cols, sum_blocks;
+  uint32_t n_rows, chunk, n_chunks, n_cols, sum_blocks, zero_blocks;
+  uint32_t zero_rows;    // rows that a workgroup looks through for ones without tokens, at most 64
   uint32_t accumulate;
   float scale;
 };
@@ -314,26 +326,33 @@ template <typename S, typename D>
 __global__ __launch_bounds__(kGradWaves* kWave) void etha_embedding_grad_kernel(const GradArgs a) {
   constexpr int N = grad_vec<S>();
   const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  if (blockIdx.x >= a.sum_blocks) {  // rows without a token: 64 rows a workgroup
-    const uint64_t row0 = (uint64_t)(blockIdx.x - a.sum_blocks) * 64;
+#ifdef ZFIRST
+  const bool zeros = blockIdx.x < a.zero_blocks;
+  const uint32_t block = zeros ? blockIdx.x : blockIdx.x - a.zero_blocks;
+#else
+  const bool zeros = blockIdx.x >= a.sum_blocks;
+  const uint32_t block = zeros ? blockIdx.x - a.sum_blocks : blockIdx.x;
+#endif
+  if (zeros) {
+    const uint64_t row0 = (uint64_t)block * a.zero_rows;
     uint64_t lo = 0, hi = a.n;
     const uint32_t mine = (uint32_t)(row0 + lane);
     while (lo < hi) {
       const uint64_t mid = (lo + hi) >> 1;
       if (a.keys[mid] < mine) lo = mid + 1; else hi = mid;
     }
-    const bool empty = row0 + lane < a.n_rows && !(lo < a.n && a.keys[lo] == mine);
+    const bool empty = lane < a.zero_rows && row0 + lane < a.n_rows && !(lo < a.n && a.keys[lo] == mine);
     uint64_t todo = __ballot(empty);
     constexpr int M = 16 / (int)sizeof(typename D::bits);
     const float zero[M] = {};
-    for (uint32_t r = wave; r < 64; r += kGradWaves)
+    for (uint32_t r = wave; r < a.zero_rows; r += kGradWaves)
       if ((todo >> r) & 1) {
         typename D::bits* p = (typename D::bits*)a.out + (int64_t)(row0 + r) * a.out_stride;
         for (uint64_t c = lane * M; c < a.width; c += 64 * M) store_f32<D, M, true>(p + c, zero, (int64_t)(a.width - c));
       }
     return;
   }
-  const uint64_t unit = (uint64_t)blockIdx.x * kGradWaves + wave;
+  const uint64_t unit = (uint64_t)block * kGradWaves + wave;
   const uint32_t j = (uint32_t)(unit / a.n_cols);
   const uint64_t col = (unit % a.n_cols * 64 + lane) * N;
   if (j >= a.n_chunks) return;
@@ -382,6 +401,63 @@ __global__ __launch_bounds__(kGradWaves* kWave) void etha_embedding_grad_kernel(
   else write_row<D, N>(a, cur, col, acc);
 }
 
+// Few tokens: no sort and one launch.  A workgroup owns 16 rows and 64 vectors of columns; each wave picks the places of
+// its 4 rows' tokens out of all tokens, in their order, and adds their rows up.
+constexpr uint32_t kFewTokens = 512, kFewTokenRows = 4;
+
+struct FewGradArgs {
+  GradArgs g;
+  const void* tokens;
+  int64_t first;
+  uint32_t wide;
+};
+
+template <typename S, typename D>
+__global__ __launch_bounds__(kGradWaves* kWave) void etha_embedding_grad_few_kernel(const FewGradArgs few) {
+  constexpr int N = grad_vec<S>();
+  constexpr uint32_t kSteps = kFewTokens / 64;
+  const GradArgs& a = few.g;
+  __shared__ uint16_t s_list[kGradWaves][kFewTokenRows][kFewTokens];
+  const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const uint32_t row0 = (blockIdx.x * kGradWaves + wave) * kFewTokenRows;
+  const uint64_t col = ((uint64_t)blockIdx.y * 64 + lane) * N;
+  uint32_t row[kSteps];
+  #pragma unroll
+  for (uint32_t i = 0; i < kSteps; i++) row[i] = i * 64 + lane < a.n ? local_row(few.tokens, few.wide, i * 64 + lane, few.first, a.n_rows) : a.n_rows;
+  uint32_t count[kFewTokenRows] = {};
+  #pragma unroll
+  for (uint32_t i = 0; i < kSteps; i++) {
+    if (i * 64 >= a.n) break;
+    #pragma unroll
+    for (uint32_t r = 0; r < kFewTokenRows; r++) {
+      const bool mine = row[i] == row0 + r && row[i] < a.n_rows;
+      const uint64_t mask = __ballot(mine);
+      if (mine) s_list[wave][r][count[r] + __popcll(mask & ((1ull << lane) - 1))] = (uint16_t)(i * 64 + lane);
+      count[r] += (uint32_t)__popcll(mask);
+    }
+  }
+  const int64_t left = col < a.width ? (int64_t)(a.width - col) : 0;
+  if (!left) return;
+  #pragma unroll
+  for (uint32_t r = 0; r < kFewTokenRows; r++) {
+    if (row0 + r >= a.n_rows || (a.accumulate && !count[r])) continue;
+    float acc[N] = {};
+    for (uint32_t i = 0; i < count[r]; i += kGradAhead) {
+      float v[kGradAhead][N];
+      #pragma unroll
+      for (uint32_t u = 0; u < kGradAhead; u++) {
+        const uint32_t p = s_list[wave][r][i + u < count[r] ? i + u : i];
+        load_f32<S, N, true>(v[u], (const typename S::bits*)a.grad + (int64_t)p * a.grad_stride + col, i + u < count[r] ? left : 0);
+      }
+      #pragma unroll
+      for (uint32_t u = 0; u < kGradAhead; u++)
+        #pragma unroll
+        for (int e = 0; e < N; e++) acc[e] += v[u][e];
+    }
+    write_row<D, N>(a, row0 + r, col, acc);
+  }
+}
+
 // Rows that cross chunks: the wave of the chunk where such a row begins adds the pieces up.
 template <typename S, typename D>
 __global__ __launch_bounds__(kGradWaves* kWave) void etha_embedding_join_kernel(const GradArgs a) {
@@ -397,18 +473,29 @@ __global__ __launch_bounds__(kGradWaves* kWave) void etha_embedding_join_kernel(
   const uint32_t key = a.keys[end];
   if (key >= a.n_rows || a.keys[end - 1] != key) return;          // nothing goes on behind this chunk
   if (a.keys[begin] == key && begin && a.keys[begin - 1] == key) return;  // begun earlier
-  if (col >= a.width) return;
-  const int64_t left = (int64_t)(a.width - col);
-  float acc[N], v[N];
+  const int64_t left = col < a.width ? (int64_t)(a.width - col) : 0;  // all lanes stay: they look for the row's chunks together
+  float acc[N];
   load_f32<F32, N>(acc, (const uint32_t*)(a.partial + ((uint64_t)j * 2 + 1) * a.width + col), left);
-  do {
-    j++;
-    load_f32<F32, N>(v, (const uint32_t*)(a.partial + (uint64_t)j * 2 * a.width + col), left);
-    #pragma unroll
-    for (int i = 0; i < N; i++) acc[i] += v[i];
-    end += a.chunk;
-  } while (end < a.n && a.keys[end] == key);
-  write_row<D, N>(a, key, col, acc);
+  // the chunks behind this one that begin with the same row, 64 at a time
+  for (;;) {
+    const uint64_t start = (uint64_t)(j + 1 + lane) * a.chunk;
+    const uint64_t same = __ballot(start < a.n && a.keys[start < a.n ? start : 0] == key);
+    const uint32_t more = ~same ? __builtin_ctzll(~same) : 64;
+    for (uint32_t i = 0; i < more; i += kGradAhead) {
+      float v[kGradAhead][N];
+      #pragma unroll
+      for (uint32_t u = 0; u < kGradAhead; u++)
+        load_f32<F32, N>(v[u], (const uint32_t*)(a.partial + (uint64_t)(j + 1 + (i + u < more ? i + u : i)) * 2 * a.width + col),
+                         i + u < more ? left : 0);
+      #pragma unroll
+      for (uint32_t u = 0; u < kGradAhead; u++)
+        #pragma unroll
+        for (int e = 0; e < N; e++) acc[e] += v[u][e];
+    }
+    j += more;
+    if (more < 64) break;
+  }
+  if (left) write_row<D, N>(a, key, col, acc);
 }
 
 // ---- rows to 8 bits --------------------------------------------------------------------------------------------
@@ -421,6 +508,9 @@ struct QuantArgs {
   int64_t x_stride, values_stride;
 };
 
+#ifndef QNT
+#define QNT true
+#endif
 template <typename S, int THREADS, int CHUNKS>
 __global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS) void etha_quantize_rows_kernel(const QuantArgs a) {
   constexpr int kBlock = THREADS < 256 ? 256 : THREADS, kWaves = THREADS / kWave;
@@ -437,7 +527,7 @@ __global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS) void etha_quantize_r
     #pragma unroll
     for (int c = 0; c < CHUNKS; c++) {
       const int64_t at = base + ((int64_t)c * THREADS + tid) * 8;
-      load_f32<S, 8>(v[c], x + at, width - at);
+      load_f32<S, 8, QNT>(v[c], x + at, width - at);
       top = largest_bits(v[c], top);
     }
   }
@@ -459,7 +549,7 @@ __global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS) void etha_quantize_r
       if (again) load_f32<S, 8>(v[c], x + at, width - at);
       const u32x2 packed = scale.pack(v[c]);
       if (width - at >= 8) {
-        store_raw<8>(out + at, packed);
+        store_raw<8, QNT>(out + at, packed);
       } else {
         for (int i = 0; i < 8; i++)
           if (i < width - at) out[at + i] = (int8_t)(packed[i >> 2] >> (8 * (i & 3)));
@@ -509,7 +599,7 @@ GradPlan grad_plan(uint64_t n, uint64_t n_rows, uint64_t width, int es) {
   const int bits = log2_up(n_rows + 1);
   p.passes = bits ? (bits + 8) / 9 : 1;
   p.bits = bits ? (bits + p.passes - 1) / p.passes : 1;
-  p.sort_blocks = n <= kOneBlockTokens ? 0 : (uint32_t)((n + kSortTokens - 1) / kSortTokens);
+  p.sort_blocks = n <= kOneBlockTokens ? 0 : (uint32_t)((n + sort_tokens(n) - 1) / sort_tokens(n));
   const auto up = [](uint64_t b) { return (b + 255) / 256 * 256; };
   p.keys_bytes = up(n * 4);
   p.hist_bytes = up((uint64_t)p.sort_blocks * (1u << p.bits) * 4);
@@ -532,7 +622,7 @@ int etha_embedding(const void* tokens, uint32_t token_dtype, uint64_t n_tokens, 
   if ((!weight && n_rows) || !out) return fail(ETHA_ERR_INVALID, "etha_embedding: null tensor");
   LookupArgs a = {tokens, weight, out, n_tokens, width, first_row, weight_stride, out_stride, (uint32_t)n_rows, 0,
                   token_dtype == ETHA_I64, scale};
-  const uint64_t n = 16 / (es > eo ? es : eo), vecs = (width + n - 1) / n;
+  const uint64_t n = lookup_vec(es, eo), vecs = (width + n - 1) / n;
   a.lanes_log2 = (uint32_t)log2_up(vecs < 256 ? vecs : 256);
   const uint32_t per_block = 256u >> a.lanes_log2;
   uint64_t gx = (n_tokens + per_block - 1) / per_block;
@@ -552,7 +642,7 @@ int etha_embedding_grad_workspace(uint64_t n_tokens, uint64_t n_rows, uint64_t w
   if (rc != ETHA_OK) return rc;
   if (!bytes) return fail(ETHA_ERR_INVALID, "etha_embedding_grad_workspace: null result");
   if (!es_of(grad_dtype)) return fail(ETHA_ERR_UNSUPPORTED, "etha_embedding_grad_workspace: element types are f32, bf16 and f16");
-  *bytes = n_tokens && n_rows && width ? grad_plan(n_tokens, n_rows, width, es_of(grad_dtype)).total() : 0;
+  *bytes = n_tokens > kFewTokens && n_rows && width ? grad_plan(n_tokens, n_rows, width, es_of(grad_dtype)).total() : 0;
   return ETHA_OK;
 }
 
@@ -577,7 +667,20 @@ int etha_embedding_grad(const void* grad, uint32_t grad_dtype, int64_t grad_stri
   g.accumulate = accumulate != 0;
   g.scale = scale;
   g.chunk = g.n_cols = 1;
-  if (n_tokens) {
+  if (n_tokens <= kFewTokens) {
+    const FewGradArgs few = {g, tokens, first_row, token_dtype == ETHA_I64};
+    const uint64_t per = 64 * (16 / es);
+    const dim3 grid((uint32_t)((n_rows + kGradWaves * kFewTokenRows - 1) / (kGradWaves * kFewTokenRows)), (uint32_t)((width + per - 1) / per));
+    if (grid.x >= 1u << 24 || grid.y > 65535) return fail(ETHA_ERR_UNSUPPORTED, "etha_embedding_grad: too many rows or columns");
+    with_type(grad_dtype, [&](auto s) {
+      with_type(out_dtype, [&](auto d) {
+        hipLaunchKernelGGL((etha_embedding_grad_few_kernel<decltype(s), decltype(d)>), grid, dim3(kGradWaves * kWave), 0,
+                           (hipStream_t)stream, few);
+      });
+    });
+    return launched("etha_embedding_grad_few_kernel");
+  }
+  {
     const GradPlan p = grad_plan(n_tokens, n_rows, width, es);
     if (!workspace || workspace_bytes < p.total() || ((uintptr_t)workspace & 15))
       return fail(ETHA_ERR_INVALID, "etha_embedding_grad: the workspace has to hold %llu bytes at a 16-byte address",
@@ -605,9 +708,12 @@ int etha_embedding_grad(const void* grad, uint32_t grad_dtype, int64_t grad_stri
         s.pos_in = pass ? pos[at ^ 1] : nullptr;
         s.keys_out = keys[at];
         s.pos_out = pos[at];
-        hipLaunchKernelGGL(etha_sort_count_kernel, dim3(p.sort_blocks), dim3(kSortThreads), 0, (hipStream_t)stream, s);
+        const bool wide_blocks = sort_tokens(n_tokens) == 4096;
+        const auto count = wide_blocks ? etha_sort_count_kernel<4096> : etha_sort_count_kernel<1024>;
+        const auto scatter = wide_blocks ? etha_sort_scatter_kernel<4096> : etha_sort_scatter_kernel<1024>;
+        hipLaunchKernelGGL(count, dim3(p.sort_blocks), dim3(kSortThreads), 0, (hipStream_t)stream, s);
         if ((rc = launched("etha_sort_count_kernel")) != ETHA_OK) return rc;
-        hipLaunchKernelGGL(etha_sort_scatter_kernel, dim3(p.sort_blocks), dim3(kSortThreads), 0, (hipStream_t)stream, s);
+        hipLaunchKernelGGL(scatter, dim3(p.sort_blocks), dim3(kSortThreads), 0, (hipStream_t)stream, s);
         if ((rc = launched("etha_sort_scatter_kernel")) != ETHA_OK) return rc;
         at ^= 1;
       }
@@ -623,11 +729,13 @@ int etha_embedding_grad(const void* grad, uint32_t grad_dtype, int64_t grad_stri
     if (blocks > 1u << 23) return fail(ETHA_ERR_UNSUPPORTED, "etha_embedding_grad: too many tokens for this width");
     g.sum_blocks = (uint32_t)blocks;
   }
-  const uint32_t zero_blocks = accumulate ? 0 : (uint32_t)((n_rows + 63) / 64);
-  if ((uint64_t)g.sum_blocks + zero_blocks >= 1u << 24) return fail(ETHA_ERR_UNSUPPORTED, "etha_embedding_grad: too many rows");
+  g.zero_rows = n_rows >= 65536 ? 64 : 16;  // few rows: enough workgroups to write them
+  const uint64_t zero_blocks = accumulate ? 0 : (n_rows + g.zero_rows - 1) / g.zero_rows;
+  g.zero_blocks = (uint32_t)zero_blocks;
+  if (g.sum_blocks + zero_blocks >= 1u << 24) return fail(ETHA_ERR_UNSUPPORTED, "etha_embedding_grad: too many rows");
   with_type(grad_dtype, [&](auto s) {
     with_type(out_dtype, [&](auto d) {
-      hipLaunchKernelGGL((etha_embedding_grad_kernel<decltype(s), decltype(d)>), dim3(g.sum_blocks + zero_blocks),
+      hipLaunchKernelGGL((etha_embedding_grad_kernel<decltype(s), decltype(d)>), dim3(g.sum_blocks + g.zero_blocks),
                          dim3(kGradWaves * kWave), 0, (hipStream_t)stream, g);
     });
   });
@@ -652,8 +760,15 @@ int etha_quantize_rows(const void* x, uint32_t dtype, uint64_t rows, uint64_t wi
   with_type(dtype, [&](auto s) {
     typedef decltype(s) S;
     // a wave a row while the row fits its registers, else a workgroup a row
+#ifdef Q512
+    if (width <= 512 * 8 && width > 2048)
+      hipLaunchKernelGGL((etha_quantize_rows_kernel<S, 512, 1>), dim3((uint32_t)rows), dim3(512), 0, (hipStream_t)stream, a);
+    else
+#endif
     if (width <= 64 * 8 * 4)
       hipLaunchKernelGGL((etha_quantize_rows_kernel<S, 64, 4>), dim3((uint32_t)((rows + 3) / 4)), dim3(256), 0, (hipStream_t)stream, a);
+    else if (width <= 256 * 8 * 2)
+      hipLaunchKernelGGL((etha_quantize_rows_kernel<S, 256, 2>), dim3((uint32_t)rows), dim3(256), 0, (hipStream_t)stream, a);
     else if (width <= 256 * 8 * 4)
       hipLaunchKernelGGL((etha_quantize_rows_kernel<S, 256, 4>), dim3((uint32_t)rows), dim3(256), 0, (hipStream_t)stream, a);
     else

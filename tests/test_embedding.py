@@ -99,7 +99,7 @@ def test_entry_points_refuse_what_they_cannot_take():
     assert look(r=1 << 31) == nat.ERR_UNSUPPORTED
     assert look(h=1 << 25) == nat.ERR_UNSUPPORTED
     assert look(n=0) == 0 and look(h=0) == 0  # nothing to do: nothing is launched
-    grad = lambda **k: lib.etha_embedding_grad(*{**dict(g=0x1000, gd=nat.F32, gs=4, t=0x1000, td=nat.I32, n=4, r=8, h=4, f=0, s=1.0,
+    grad = lambda **k: lib.etha_embedding_grad(*{**dict(g=0x1000, gd=nat.F32, gs=4, t=0x1000, td=nat.I32, n=4000, r=8, h=4, f=0, s=1.0,
                                                         o=0x1000, od=nat.F32, os=4, a=0, ws=0x1000, wb=1 << 20, st=None), **k}.values())
     assert grad(gd=nat.F64) == nat.ERR_UNSUPPORTED
     assert grad(wb=0) == nat.ERR_INVALID and b"workspace" in lib.etha_last_error()
@@ -108,7 +108,7 @@ def test_entry_points_refuse_what_they_cannot_take():
     assert grad(g=None) == nat.ERR_INVALID
     assert grad(r=0) == 0 and grad(n=0, a=1) == 0
     need = nat.embedding_grad_workspace
-    assert need(0, 8, 4, nat.F32) == 0 and need(1, 8, 4, nat.F32) > 0
+    assert need(0, 8, 4, nat.F32) == 0 and need(4000, 8, 4, nat.F32) > 0
     with pytest.raises(nat.EthaNativeError):
         need(1, 8, 4, nat.I32)
 
@@ -169,7 +169,7 @@ def test_lookup_in_a_table_past_32_bits(gpu_device):
 
 GRADIENT_CASES = [
     # tokens, rows, width, vocabulary (tokens outside rows are other shards')
-    (1, 1, 1, 1), (1, 500, 64, 500), (7, 3, 5, 9), (63, 64, 130, 64), (64, 65, 512, 65), (65, 1, 1001, 1), (509, 4000, 1001, 32000),
+    (1, 1, 1, 1), (1, 500, 64, 500), (7, 3, 5, 9), (63, 64, 130, 64), (64, 65, 512, 65), (65, 1, 1001, 1), (509, 4000, 1001, 32000), (512, 30, 2060, 40), (513, 30, 1032, 40), (700, 5000, 20, 9000),
     (1025, 2, 96, 2), (3000, 511, 72, 700), (8192, 100000, 40, 100000), (8193, 513, 64, 600), (20000, 1, 136, 3), (12289, 70000, 33, 140000),
 ]
 
