@@ -213,7 +213,6 @@ __global__ __launch_bounds__(kSortThreads) void etha_sort_count_kernel(const Sor
   for (uint32_t i = threadIdx.x; i < bins; i += kSortThreads) s_count[i] = 0;
   __syncthreads();
   const uint64_t base = (uint64_t)blockIdx.x * TOKENS;
-  #pragma unroll
   for (uint32_t i = threadIdx.x; i < TOKENS; i += kSortThreads)
     if (base + i < a.n) atomicAdd(&s_count[(sort_key(a, base + i) >> a.shift) & (bins - 1)], 1u);
   __syncthreads();
@@ -295,8 +294,7 @@ struct GradArgs {
   float* partial;        // [chunk][2][width]
   uint64_t n, width;
   int64_t grad_stride, out_stride;
-  uint32_t n_rows, chunk, n_chunks, n_cols, sum_blocks, zero_blocks;
-  uint32_t zero_rows;    // rows that a workgroup looks through for ones without tokens, at most 64
+  uint32_t n_rows, chunk, n_chunks, n_cols, sum_blocks;
   uint32_t accumulate;
   float scale;
 };
@@ -318,6 +316,9 @@ __device__ inline void write_row(const GradArgs& a, uint32_t row, uint64_t col, 
 }
 
 constexpr int kGradWaves = 4, kGradAhead = 8;
+// Rows that a workgroup looks through for ones without tokens: one a wave, so that they are written in address order by
+// workgroups that live as shortly as a copy's (128256 x 4096 in bf16: 327 us with 4 rows, 357 us with 64).
+constexpr uint32_t kZeroRows = 4;
 
 template <typename S>
 constexpr int grad_vec() { return 16 / (int)sizeof(typename S::bits); }
@@ -326,33 +327,26 @@ template <typename S, typename D>
 __global__ __launch_bounds__(kGradWaves* kWave) void etha_embedding_grad_kernel(const GradArgs a) {
   constexpr int N = grad_vec<S>();
   const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#ifdef ZFIRST
-  const bool zeros = blockIdx.x < a.zero_blocks;
-  const uint32_t block = zeros ? blockIdx.x : blockIdx.x - a.zero_blocks;
-#else
-  const bool zeros = blockIdx.x >= a.sum_blocks;
-  const uint32_t block = zeros ? blockIdx.x - a.sum_blocks : blockIdx.x;
-#endif
-  if (zeros) {
-    const uint64_t row0 = (uint64_t)block * a.zero_rows;
+  if (blockIdx.x >= a.sum_blocks) {  // rows without a token
+    const uint64_t row0 = (uint64_t)(blockIdx.x - a.sum_blocks) * kZeroRows;
     uint64_t lo = 0, hi = a.n;
     const uint32_t mine = (uint32_t)(row0 + lane);
     while (lo < hi) {
       const uint64_t mid = (lo + hi) >> 1;
       if (a.keys[mid] < mine) lo = mid + 1; else hi = mid;
     }
-    const bool empty = lane < a.zero_rows && row0 + lane < a.n_rows && !(lo < a.n && a.keys[lo] == mine);
+    const bool empty = lane < kZeroRows && row0 + lane < a.n_rows && !(lo < a.n && a.keys[lo] == mine);
     uint64_t todo = __ballot(empty);
     constexpr int M = 16 / (int)sizeof(typename D::bits);
     const float zero[M] = {};
-    for (uint32_t r = wave; r < a.zero_rows; r += kGradWaves)
+    for (uint32_t r = wave; r < kZeroRows; r += kGradWaves)
       if ((todo >> r) & 1) {
         typename D::bits* p = (typename D::bits*)a.out + (int64_t)(row0 + r) * a.out_stride;
         for (uint64_t c = lane * M; c < a.width; c += 64 * M) store_f32<D, M, true>(p + c, zero, (int64_t)(a.width - c));
       }
     return;
   }
-  const uint64_t unit = (uint64_t)block * kGradWaves + wave;
+  const uint64_t unit = (uint64_t)blockIdx.x * kGradWaves + wave;
   const uint32_t j = (uint32_t)(unit / a.n_cols);
   const uint64_t col = (unit % a.n_cols * 64 + lane) * N;
   if (j >= a.n_chunks) return;
@@ -508,9 +502,6 @@ struct QuantArgs {
   int64_t x_stride, values_stride;
 };
 
-#ifndef QNT
-#define QNT true
-#endif
 template <typename S, int THREADS, int CHUNKS>
 __global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS) void etha_quantize_rows_kernel(const QuantArgs a) {
   constexpr int kBlock = THREADS < 256 ? 256 : THREADS, kWaves = THREADS / kWave;
@@ -527,7 +518,7 @@ __global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS) void etha_quantize_r
     #pragma unroll
     for (int c = 0; c < CHUNKS; c++) {
       const int64_t at = base + ((int64_t)c * THREADS + tid) * 8;
-      load_f32<S, 8, QNT>(v[c], x + at, width - at);
+      load_f32<S, 8, true>(v[c], x + at, width - at);
       top = largest_bits(v[c], top);
     }
   }
@@ -549,7 +540,7 @@ __global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS) void etha_quantize_r
       if (again) load_f32<S, 8>(v[c], x + at, width - at);
       const u32x2 packed = scale.pack(v[c]);
       if (width - at >= 8) {
-        store_raw<8, QNT>(out + at, packed);
+        store_raw<8, true>(out + at, packed);
       } else {
         for (int i = 0; i < 8; i++)
           if (i < width - at) out[at + i] = (int8_t)(packed[i >> 2] >> (8 * (i & 3)));
@@ -589,11 +580,11 @@ GradPlan grad_plan(uint64_t n, uint64_t n_rows, uint64_t width, int es) {
   GradPlan p = {};
   const uint64_t per = 64 * (16 / es);
   p.n_cols = (uint32_t)((width + per - 1) / per);
-  // chunks of 64 places, shorter while there would be fewer waves than the chip holds a few of per SIMD, longer
-  // where the pieces of rows that cross chunks would need more than 2048 places in the workspace
-  uint64_t chunk = 64;
+  // chunks of 128 places, shorter while there would be fewer waves than the chip holds a few of per SIMD, longer where the
+  // pieces of rows that cross chunks would need more than 2048 places in the workspace
+  uint64_t chunk = 128;
   while (chunk > 8 && (n + chunk - 1) / chunk * p.n_cols < 4096) chunk >>= 1;
-  while ((n + chunk - 1) / chunk > 2048 && chunk >= 64) chunk += 64;
+  if ((n + chunk - 1) / chunk > 2048 && chunk == 128) chunk = ((n + 2047) / 2048 + 127) / 128 * 128;
   p.chunk = (uint32_t)chunk;
   p.n_chunks = (uint32_t)((n + chunk - 1) / chunk);
   const int bits = log2_up(n_rows + 1);
@@ -729,13 +720,11 @@ int etha_embedding_grad(const void* grad, uint32_t grad_dtype, int64_t grad_stri
     if (blocks > 1u << 23) return fail(ETHA_ERR_UNSUPPORTED, "etha_embedding_grad: too many tokens for this width");
     g.sum_blocks = (uint32_t)blocks;
   }
-  g.zero_rows = n_rows >= 65536 ? 64 : 16;  // few rows: enough workgroups to write them
-  const uint64_t zero_blocks = accumulate ? 0 : (n_rows + g.zero_rows - 1) / g.zero_rows;
-  g.zero_blocks = (uint32_t)zero_blocks;
+  const uint64_t zero_blocks = accumulate ? 0 : (n_rows + kZeroRows - 1) / kZeroRows;
   if (g.sum_blocks + zero_blocks >= 1u << 24) return fail(ETHA_ERR_UNSUPPORTED, "etha_embedding_grad: too many rows");
   with_type(grad_dtype, [&](auto s) {
     with_type(out_dtype, [&](auto d) {
-      hipLaunchKernelGGL((etha_embedding_grad_kernel<decltype(s), decltype(d)>), dim3(g.sum_blocks + g.zero_blocks),
+      hipLaunchKernelGGL((etha_embedding_grad_kernel<decltype(s), decltype(d)>), dim3((uint32_t)(g.sum_blocks + zero_blocks)),
                          dim3(kGradWaves * kWave), 0, (hipStream_t)stream, g);
     });
   });
@@ -759,12 +748,8 @@ int etha_quantize_rows(const void* x, uint32_t dtype, uint64_t rows, uint64_t wi
   const QuantArgs a = {x, values, scales, rows, width, x_stride, values_stride};
   with_type(dtype, [&](auto s) {
     typedef decltype(s) S;
-    // a wave a row while the row fits its registers, else a workgroup a row
-#ifdef Q512
-    if (width <= 512 * 8 && width > 2048)
-      hipLaunchKernelGGL((etha_quantize_rows_kernel<S, 512, 1>), dim3((uint32_t)rows), dim3(512), 0, (hipStream_t)stream, a);
-    else
-#endif
+    // a wave a row while the row fits its registers, else a workgroup a row, with no more registers than the row needs
+    // (64128 rows of 4096 in fp32: 222 us with room for 4096, 236 us with room for 8192)
     if (width <= 64 * 8 * 4)
       hipLaunchKernelGGL((etha_quantize_rows_kernel<S, 64, 4>), dim3((uint32_t)((rows + 3) / 4)), dim3(256), 0, (hipStream_t)stream, a);
     else if (width <= 256 * 8 * 2)
