@@ -2,7 +2,8 @@
 
 An inference job that holds its projections in 8 bits turns every weight shard that a redistribute delivers into integers
 with one scale for each output channel (:func:`quantize_rows`), and multiplies tokens, converted the same way with one scale
-for each token, with them (:func:`int8_linear`).
+for each token, with them (:func:`int8_linear`).  :class:`Int8Weight` is such a weight as the target of a transfer:
+``ReshardJob`` (``TensorSpec.target_int8``) and ``TensorBusClient.register_tensors`` convert it when its values have arrived.
 """
 
 from __future__ import annotations
@@ -119,3 +120,28 @@ def int8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scales: torch.Tens
          weight_scales.data_ptr(), channels, w_stride, width, None if bias is None else bias.data_ptr(), out.data_ptr(),
          DTYPE_CODES[out.dtype], out_stride, workspace.data_ptr() if nbytes else None, nbytes)
     return out
+
+
+class Int8Weight:
+    """A weight in 8 bits that a transfer fills: the transfer writes ``landing`` (``[..., channels, width]`` in fp32, bf16 or
+    fp16), :meth:`refresh` converts it into ``values`` (int8) and ``scales`` (fp32, one for each channel), which keep their
+    addresses, so that captured graphs read the new weights."""
+
+    def __init__(self, landing: torch.Tensor):
+        if landing.dim() < 2:
+            raise ValueError(f"Int8Weight: a weight of {landing.dim()} dims has no channels")
+        code_of("Int8Weight", landing.dtype)
+        self.landing = landing
+        self.values = torch.zeros(landing.shape, dtype=torch.int8, device=landing.device)
+        self.scales = torch.zeros(landing.shape[:-1], dtype=torch.float32, device=landing.device)
+
+    def refresh(self) -> "Int8Weight":
+        """Convert what lies in ``landing``, on the current stream."""
+        with torch.no_grad():
+            quantize_rows(self.landing, values=self.values, scales=self.scales)
+        return self
+
+    def linear(self, x: torch.Tensor, *, bias: torch.Tensor | None = None, dtype: torch.dtype | None = None,
+               out: torch.Tensor | None = None) -> torch.Tensor:
+        """:func:`int8_linear` over this weight (two dims)."""
+        return int8_linear(x, self.values, self.scales, bias=bias, dtype=dtype, out=out)

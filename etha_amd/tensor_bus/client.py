@@ -20,6 +20,7 @@ from typing import Literal
 
 import torch
 
+from ..int8 import Int8Weight
 from .command_queue import BusyError, CommandQueue, Completion
 from .commands import CleanupBatch, InitPair, QueryStatus, RegisterTensors, Transfer
 from .ipc_tensor import export_tensor, release_local
@@ -32,10 +33,11 @@ HEARTBEAT_MAX_AGE = 5.0  # seconds (client.py:374)
 class BatchHandler:
     """Handle of one registered batch (``client.py:30-107``)."""
 
-    def __init__(self, client: "TensorBusClient", batch_id: str, pair_names: list[str]):
+    def __init__(self, client: "TensorBusClient", batch_id: str, pair_names: list[str], int8_weights: tuple = ()):
         self._client_ref = weakref.ref(client)
         self.batch_id = batch_id
         self.pair_names = pair_names
+        self.int8_weights = int8_weights
         self._closed = False
 
     @property
@@ -46,9 +48,22 @@ class BatchHandler:
         return client
 
     def transfer(self, transfer_type: Literal["send", "recv"], blocking: bool = False, timeout: float = 30.0) -> Completion:
+        """As the client's ``transfer``.  A blocking ``recv`` also converts the batch's 8-bit weights (on the current
+        stream); after one that does not block call :meth:`refresh_int8` once it has completed."""
         msg = Transfer(batch_id=self.batch_id, transfer_type=transfer_type)
-        return self.client._execute_command_with_semaphore(
+        done = self.client._execute_command_with_semaphore(
             msg, "transfer", context_id=f"batch_{self.batch_id}_{transfer_type}", blocking=blocking, timeout=timeout)
+        if blocking and transfer_type == "recv":
+            self.refresh_int8()
+        return done
+
+    def refresh_int8(self) -> None:
+        """Convert the batch's 8-bit weights from what the last transfer brought (no counterpart in the reference); waits
+        for it, because the agent's stream, which the next transfer is written on, does not."""
+        for weight in self.int8_weights:
+            weight.refresh()
+        for device in {weight.landing.device for weight in self.int8_weights}:
+            torch.cuda.current_stream(device).synchronize()
 
     def query_transfer_signal(self, blocking: bool = True, timeout: float = 30.0) -> bool:
         return self.client.query_transfer_signal(self.batch_id, blocking=blocking, timeout=timeout)
@@ -165,11 +180,17 @@ class TensorBusClient:
         state = self._read_state() or {}
         return bool(state.get("batches", {}).get(batch_id, {}).get("transfer_signal", False))
 
-    def register_tensors(self, batch_id: str, tensors: list[tuple[torch.Tensor, str]], bucket_size: int | None = None,
+    def register_tensors(self, batch_id: str, tensors: list[tuple[torch.Tensor | Int8Weight, str]], bucket_size: int | None = None,
                          timeout: float = 30.0) -> BatchHandler:
-        """Register tensors across pairs; always blocks until every rank of the batch has registered."""
+        """Register tensors across pairs; always blocks until every rank of the batch has registered.
+
+        A receiving rank may register an :class:`~etha_amd.int8.Int8Weight`: its ``landing`` is the tensor that is filled,
+        and the handler converts it behind each transfer.
+        """
         if not tensors:
             raise ValueError("tensors list cannot be empty")
+        int8_weights = tuple(t for t, _ in tensors if isinstance(t, Int8Weight))
+        tensors = [(t.landing if isinstance(t, Int8Weight) else t, pair_name) for t, pair_name in tensors]
         for t, _ in tensors:
             if t.device.type == "cuda":
                 torch.cuda.current_stream(t.device).synchronize()  # the agent works on its own stream
@@ -184,7 +205,7 @@ class TensorBusClient:
             for _, p in payloads:
                 release_local(p)
         unique_pair_names = list(dict.fromkeys(pair_name for _, pair_name in tensors))
-        return BatchHandler(client=self, batch_id=batch_id, pair_names=unique_pair_names)
+        return BatchHandler(client=self, batch_id=batch_id, pair_names=unique_pair_names, int8_weights=int8_weights)
 
     def close(self):
         self.command_queue.close()

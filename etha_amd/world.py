@@ -17,6 +17,7 @@ import torch
 from torch.distributed.tensor.placement_types import Partial, Replicate
 
 from .comm import LoopbackWire, PartialGroup, bucket_comm, chunk_to_bucket_ops, get_m2m_map, m2m_to_chunks
+from .int8 import Int8Weight
 from .layout import local_shape, local_shard, mesh_coord
 
 
@@ -40,6 +41,10 @@ class TensorSpec:
     # non-contiguous parents are legal, tests/test_communication_replicate_shard.py:99-113)
     source_layout: str = "contiguous"
     target_layout: str = "contiguous"
+    # the inference side holds this weight in 8 bits with a scale for each output channel (etha_amd.int8): the transfer
+    # writes the target shard as ever, and the shard is converted behind it.  A shard has its own scales: those of a
+    # channel that is cut (Shard of the last dim) cover the shard's part of it.
+    target_int8: bool = False
 
 
 def transfer_dtype_rule(source: torch.dtype, target: torch.dtype) -> torch.dtype:
@@ -133,6 +138,7 @@ class ReshardJob:
     max_in_flight: int = 2
     source_locals: list[dict[int, torch.Tensor]] = field(default_factory=list, init=False)
     target_locals: list[dict[int, torch.Tensor]] = field(default_factory=list, init=False)
+    target_int8: list[dict[int, Int8Weight]] = field(default_factory=list, init=False)  # of the specs that ask for it
     globals_: list[torch.Tensor | None] = field(default_factory=list, init=False)
     send_buckets: dict[int, list] = field(default_factory=dict, init=False)
     recv_buckets: dict[int, list] = field(default_factory=dict, init=False)
@@ -193,6 +199,7 @@ class ReshardJob:
                     tgt_local[r] = self._rehome("target", tgt_local[r])
             self.source_locals.append(src_local)
             self.target_locals.append(tgt_local)
+            self.target_int8.append({r: Int8Weight(t) for r, t in tgt_local.items()} if spec.target_int8 else {})
             self.globals_.append(glob if self.keep_globals else None)
             # ---- plan, rank by rank
             key = (str(spec.source_mesh), spec.source_placements, str(spec.target_mesh), spec.target_placements)
@@ -249,7 +256,7 @@ class ReshardJob:
     def run(self, merge_launches: bool = False, synchronize: bool = True, fanout: int = 1) -> None:
         """One transfer: every source rank calls ``bucket_comm`` on its send list, then every target rank on its
         receive list.  With a ring pool the senders fill their slots and wait on the wire; the receivers' calls
-        then move both sides along until every bucket has been unpacked."""
+        then move both sides along until every bucket has been unpacked.  Targets in 8 bits are converted behind it."""
         if self.wire.pool_mode == "ring":  # this process plays every rank: queue all pipelines, step them together
             self.run_send(merge_launches, fanout, drive=False)
             self.run_recv(merge_launches, fanout, drive=False)
@@ -259,6 +266,9 @@ class ReshardJob:
             self.run_recv(merge_launches, fanout)
         if not self.wire.idle():
             raise RuntimeError(f"transfer did not complete; still waiting for a peer: {self.wire.pending()}")
+        for weights in self.target_int8:
+            for weight in weights.values():
+                weight.refresh()
         if synchronize and self.device.type == "cuda":
             torch.cuda.current_stream(self.device).synchronize()
 
