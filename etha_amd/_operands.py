@@ -11,15 +11,15 @@ DTYPE_CODES = {torch.float32: _native.F32, torch.bfloat16: _native.BF16, torch.f
 TOKEN_CODES = {torch.int32: _native.I32, torch.int64: _native.I64}
 
 
-def check_device(what: str, first: torch.Tensor, *others: torch.Tensor | None) -> torch.device:
-    """The one GPU that all operands live on."""
-    device = first.device
-    if device.type != "cuda":
-        raise RuntimeError(f"{what}: tensors live on {device}; this operator only runs on a GPU (there is no CPU path)")
+def check_device(what: str, first: torch.Tensor, *others: torch.Tensor | None) -> int:
+    """Index of the one GPU that all operands live on."""
+    index = first.get_device()
+    if index < 0:
+        raise RuntimeError(f"{what}: tensors live on {first.device}; this operator only runs on a GPU (there is no CPU path)")
     for t in others:
-        if t is not None and t.device != device:
-            raise ValueError(f"{what}: operands live on {device} and {t.device}")
-    return device
+        if t is not None and t.get_device() != index:
+            raise ValueError(f"{what}: operands live on {first.device} and {t.device}")
+    return index
 
 
 def code_of(what: str, dtype: torch.dtype) -> int:
@@ -49,10 +49,14 @@ def row_stride(t: torch.Tensor) -> int | None:
     return t.shape[-1] if stride is None else stride
 
 
-def readable_rows(t: torch.Tensor) -> tuple[torch.Tensor, int]:
-    """``t`` or, where its rows do not lie at one distance, a contiguous copy; and that distance."""
+MOST_STRIDE = 1 << 23  # bytes between the rows of a product's operand
+
+
+def readable_rows(t: torch.Tensor, most: int | None = None) -> tuple[torch.Tensor, int]:
+    """``t`` or, where its rows do not lie at one distance (of at most ``most`` bytes), a contiguous copy; and that
+    distance in elements."""
     stride = row_stride(t)
-    if stride is None:
+    if stride is None or (most is not None and stride * t.element_size() > most):
         t = t.contiguous()
         stride = row_stride(t)
     return t, stride
@@ -104,21 +108,24 @@ def refuse_captured_backward(what: str) -> None:
         raise RuntimeError(f"the backward pass of {what} cannot be captured into a graph: capture a call of its gradient function")
 
 
-_current_device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else None
-_current_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else None
+_current_device = getattr(torch._C, "_cuda_getDevice", None)
+_current_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+_entry_points: dict = {}
 
 
-def call(device: torch.device, name: str, *args) -> None:
-    """Entry point ``name`` with ``args`` and the current stream of ``device``, which is the current device for the call.
+def call(index: int, name: str, *args) -> None:
+    """Entry point ``name`` with ``args`` and the current stream of GPU ``index``, which is the current device for the call.
 
     Where a kernel takes a few microseconds the host is what a call costs: stream and device are asked for without the
     objects that ``torch.cuda`` wraps them in.
     """
-    index = device.index
-    if index != _current_device():
-        with torch.cuda.device(device):
-            rc = getattr(_native.lib(), name)(*args, _current_stream(index))
+    func = _entry_points.get(name)
+    if func is None:
+        func = _entry_points[name] = getattr(_native.lib(), name)
+    if index == _current_device():
+        rc = func(*args, _current_stream(index))
     else:
-        rc = getattr(_native.lib(), name)(*args, _current_stream(index))
+        with torch.cuda.device(index):
+            rc = func(*args, _current_stream(index))
     if rc != 0:
         _native._check(name, rc)

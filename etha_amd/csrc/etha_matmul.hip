@@ -160,6 +160,7 @@ struct Operand {
   static constexpr int kBytes = ROWS * kStageBytes, kSlots = kBytes / 16, kPer = kSlots / kThreads;
   static constexpr int kPieces = kTrans ? ROWS / 8 : kStageBytes / 16;  // slots of an LDS row
   static_assert(kSlots % kThreads == 0 && kPer > 0, "every work-item stages the same number of slots");
+  static_assert(kPer == 1 || kThreads / kPieces % 16 == 0, "all slots of a work-item hold the same piece of their rows");
 
   static __device__ uint32_t row_of(uint32_t slot) { return slot / kPieces; }
   static __device__ uint32_t swizzle(uint32_t row, uint32_t piece) {
@@ -233,7 +234,6 @@ struct DirectStage {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
                  :: "s"(to + i * OP::kThreads * 16), "v"(at[i] | outside), "s"(rsrc) : "memory");
   }
-  __device__ void store(char*) const {}
 };
 
 // 16 bytes at p of which `left` exist; the others read as zero
@@ -254,37 +254,71 @@ __device__ inline u32x4 load_part(const char* p, int64_t left) {
   return v;
 }
 
-// Through registers: any start, any distance, any length of k.  The next stage's loads are in flight during a stage.
+// n bytes (0 to 16) dropped at the low end, zeros in at the high end
+__device__ inline u32x4 shift_bytes(u32x4 v, uint32_t n) {
+  uint64_t lo = (uint64_t)v.y << 32 | v.x, hi = (uint64_t)v.w << 32 | v.z;
+  if (n >= 8) {
+    lo = n >= 16 ? 0 : hi >> ((n - 8) * 8);
+    hi = 0;
+  } else if (n) {
+    lo = lo >> (n * 8) | hi << (64 - n * 8);
+    hi >>= n * 8;
+  }
+  return u32x4{(uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32)};
+}
+
+// Through registers: any start, any distance, any length of rows from 16 bytes on.  The next stage's loads are in flight
+// during a stage, so there are no branches about them: a piece that reaches over its row's end is loaded from 16 bytes
+// before that end, and shifted into place when it is stored to LDS.
 template <typename OP>
 struct RegisterStage {
   static constexpr bool kDirect = false;
   u32x4 v[OP::kPer];
   const char* base;
-  int64_t stride;
-  uint32_t n_rows;
+  uint32_t stride, n_rows;
+  uint32_t row0, across;  // this lane's first row (k where transposed) and where its pieces lie in a row, in bytes
+  uint32_t shift, inside; // of the stage that is in the registers: bytes to drop, rows of k that there are
+  bool odd;               // whether any of it has to be put in order
+
+  static constexpr uint32_t kRowStep = OP::kThreads / OP::kPieces;
 
   __device__ void init(const char* tile, int64_t row_stride, uint32_t n_rows_, uint32_t) {
     base = tile;
-    stride = row_stride;
+    stride = (uint32_t)row_stride;
     n_rows = n_rows_;
+    row0 = OP::row_of(threadIdx.x);
+    across = OP::piece_of(threadIdx.x) * 16;
   }
-  uint32_t k0, red;
-  __device__ void begin(char*, uint32_t k0_, uint32_t red_) {
-    k0 = k0_;
-    red = red_;
-  }
-  __device__ void part(int i) {
-    const uint32_t slot = threadIdx.x + i * OP::kThreads, row = OP::row_of(slot), piece = OP::piece_of(slot);
+  __device__ void load(uint32_t k0, uint32_t red) {
     if constexpr (!OP::kTrans) {
-      const char* p = base + (int64_t)(row < n_rows ? row : n_rows - 1) * stride + (int64_t)k0 * OP::kEs + piece * 16;
-      v[i] = k0 + OP::kStageK <= red ? load_raw<16>(p) : load_part<OP::kEs>(p, ((int64_t)red - k0) * OP::kEs - piece * 16);
-    } else {  // memory row = k, a piece holds 8 tile rows
-      const char* p = base + (int64_t)(k0 + row) * stride + piece * 16;
-      v[i] = k0 + OP::kStageK <= red && n_rows * 2 == OP::kPieces * 16 ? load_raw<16>(p)
-                 : load_part<OP::kEs>(p, k0 + row < red ? ((int64_t)n_rows - piece * 8) * 2 : 0);
+      const int left = (int)((red - k0) * OP::kEs) - (int)across;  // bytes of the row from this piece on
+      shift = left >= 16 ? 0 : left > 0 ? 16 - left : 16;
+      odd = k0 + OP::kStageK > red;
+      const uint32_t at = left >= 16 ? k0 * OP::kEs + across : red * OP::kEs - 16;
+      #pragma unroll
+      for (int i = 0; i < OP::kPer; i++) {
+        const uint32_t row = row0 + i * kRowStep;  // rows past the last repeat it; their results are dropped
+        v[i] = load_raw<16>(base + ((row < n_rows ? row : n_rows - 1) * stride + at));
+      }
+    } else {
+      const int left = (int)(n_rows * 2) - (int)across;
+      shift = left >= 16 ? 0 : left > 0 ? 16 - left : 0;  // columns past the last: their results are dropped
+      inside = red - k0 < OP::kStageK ? red - k0 : OP::kStageK;
+      odd = inside < OP::kStageK || n_rows * 2 < OP::kPieces * 16;
+      const char* from = base + (int64_t)k0 * stride + (left >= 16 ? (int)across : (int)(n_rows * 2) - 16);
+      #pragma unroll
+      for (int i = 0; i < OP::kPer; i++) {
+        const uint32_t row = row0 + i * kRowStep;
+        v[i] = load_raw<16>(from + (row < inside ? row : inside - 1) * stride);
+      }
     }
   }
-  __device__ void store(char* lds) const {
+  __device__ void store(char* lds) {
+    if (odd) {
+      #pragma unroll
+      for (int i = 0; i < OP::kPer; i++)
+        v[i] = shift_bytes(v[i], OP::kTrans && row0 + i * kRowStep >= inside ? 16 : shift);
+    }
     #pragma unroll
     for (int i = 0; i < OP::kPer; i++) *(u32x4*)(lds + (threadIdx.x + i * OP::kThreads) * 16) = v[i];
   }
@@ -380,78 +414,95 @@ __global__ __launch_bounds__(S::kThreads) void etha_matmul_kernel(const MatmulAr
     sp.init(tile.p, a.p_stride, n_rows < S::BM ? n_rows : S::BM, tile.red);
     sq.init(tile.q, a.q_stride, n_cols < S::BN ? n_cols : S::BN, tile.red);
   }
-  uint32_t next = 0;  // k of the first stage that is not on its way yet
-  const auto begin = [&](char* to) {
-    sp.begin(to, next, tile.red);
-    sq.begin(to + OpP::kBytes, next, tile.red);
-    next += kStageK;
-  };
-  constexpr int kParts = OpP::kPer + OpQ::kPer;
-  const auto part = [&](int t) {
-    if (t < OpP::kPer) sp.part(t);
-    else sq.part(t - OpP::kPer);
-  };
-  const auto load = [&](char* to) {
-    begin(to);
-    #pragma unroll
-    for (int t = 0; t < kParts; t++) part(t);
-  };
-  u32x4 fp[2][kFm], fq[2][kFn];
-  // fragments to read in a row of matrix instructions: done well before the barrier waits for them
-  constexpr int kReads = kFm + kFn, kReadRows = kFm * 3 / 4 > 0 ? kFm * 3 / 4 : 1, kReadsRow = (kReads + kReadRows - 1) / kReadRows;
+  constexpr int kReads = kFm + kFn;
+  u32x4 fp[kDirect ? 2 : 1][kFm], fq[kDirect ? 2 : 1][kFn];
   const auto read = [&](int set, const char* from, int half, int t) {
     if (t < kFn) fq[set][t] = OpQ::fragment(from + OpP::kBytes, wc + t * 16, half * 4);
     else fp[set][t - kFn] = OpP::fragment(from, wr + (t - kFn) * 16, half * 4);
   };
   typename E::acc acc[kFm][kFn] = {};
-  if (tile.red) {
-    load(lds);
-    if constexpr (kDirect) {
+  if constexpr (kDirect) {
+    constexpr int kParts = OpP::kPer + OpQ::kPer;
+    // fragments to read in a row of matrix instructions: done well before the barrier waits for them
+    constexpr int kReadRows = kFm * 3 / 4 > 0 ? kFm * 3 / 4 : 1, kReadsRow = (kReads + kReadRows - 1) / kReadRows;
+    uint32_t next = 0;  // k of the first stage that is not on its way yet
+    const auto begin = [&](char* to) {
+      sp.begin(to, next, tile.red);
+      sq.begin(to + OpP::kBytes, next, tile.red);
+      next += kStageK;
+    };
+    const auto part = [&](int t) {
+      if (t < OpP::kPer) sp.part(t);
+      else sq.part(t - OpP::kPer);
+    };
+    if (tile.red) {
       #pragma unroll
-      for (int s = 1; s < kStages; s++) load(lds + s * kBytes);
+      for (int s = 0; s < kStages; s++) {
+        begin(lds + s * kBytes);
+        #pragma unroll
+        for (int t = 0; t < kParts; t++) part(t);
+      }
       wait_stage<(kStages - 1) * kParts>();
-    } else {
-      sp.store(lds);
-      sq.store(lds + OpP::kBytes);
-      load(nullptr);
-      __syncthreads();
+      #pragma unroll
+      for (int t = 0; t < kReads; t++) read(0, lds, 0, t);
+      uint32_t use = 0;
+      for (uint32_t k = 0; k < tile.red; k += kStageK) {
+        const uint32_t then = use + kBytes == sizeof(lds) ? 0 : use + kBytes;
+        #pragma unroll
+        for (int h = 0; h < 2; h++) {
+          if (h == 1) {
+            wait_stage<(kStages - 2) * kParts>();
+            begin(lds + use);  // past the end of k it brings zeros: the count of loads stays the same
+          }
+          // a row of matrix instructions, the next half's fragments and the loads of a stage further on, in turn: issued
+          // in a row each of them would hold up the others
+          #pragma unroll
+          for (int i = 0; i < kFm; i++) {
+            #pragma unroll
+            for (int t = i * kReadsRow; t < (i + 1) * kReadsRow && t < kReads; t++) read(h ^ 1, lds + (h ? then : use), h ^ 1, t);
+            #pragma unroll
+            for (int j = 0; j < kFn; j++) acc[i][j] = E::mfma(fq[h][j], fp[h][i], acc[i][j]);
+            if (h == 1) {
+              #pragma unroll
+              for (int t = i * kParts / kFm; t < (i + 1) * kParts / kFm; t++) part(t);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+          }
+        }
+        use = then;
+      }
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no load into this LDS outlives the workgroup
     }
-    #pragma unroll
-    for (int t = 0; t < kReads; t++) read(0, lds, 0, t);
+  } else if (tile.red) {
+    sp.load(0, tile.red);
+    sq.load(0, tile.red);
+    sp.store(lds);
+    sq.store(lds + OpP::kBytes);
+    __syncthreads();
     uint32_t use = 0;
     for (uint32_t k = 0; k < tile.red; k += kStageK) {
-      const uint32_t then = use + kBytes == sizeof(lds) ? 0 : use + kBytes;
+      const uint32_t then = use ^ kBytes;
+      const bool more = k + kStageK < tile.red;
+      if (more) {
+        sp.load(k + kStageK, tile.red);
+        sq.load(k + kStageK, tile.red);
+      }
       #pragma unroll
       for (int h = 0; h < 2; h++) {
-        if (h == 1) {
-          if constexpr (kDirect) {
-            wait_stage<(kStages - 2) * kParts>();
-            begin(lds + use);
-          } else {
-            sp.store(lds + then);
-            sq.store(lds + then + OpP::kBytes);
-            __syncthreads();
-            begin(nullptr);
-          }
-        }
-        // a row of matrix instructions, the next half's fragments and the loads of a stage further on, in turn: issued in
-        // a row each of them would hold up the others
         #pragma unroll
-        for (int i = 0; i < kFm; i++) {
+        for (int t = 0; t < kReads; t++) read(0, lds + use, h, t);
+        #pragma unroll
+        for (int i = 0; i < kFm; i++)
           #pragma unroll
-          for (int t = i * kReadsRow; t < (i + 1) * kReadsRow && t < kReads; t++) read(h ^ 1, lds + (h ? then : use), h ^ 1, t);
-          #pragma unroll
-          for (int j = 0; j < kFn; j++) acc[i][j] = E::mfma(fq[h][j], fp[h][i], acc[i][j]);
-          if (h == 1) {
-            #pragma unroll
-            for (int t = i * kParts / kFm; t < (i + 1) * kParts / kFm; t++) part(t);
-          }
-          __builtin_amdgcn_sched_barrier(0);
-        }
+          for (int j = 0; j < kFn; j++) acc[i][j] = E::mfma(fq[0][j], fp[0][i], acc[i][j]);
       }
+      if (more) {
+        sp.store(lds + then);
+        sq.store(lds + then + OpP::kBytes);
+      }
+      __syncthreads();
       use = then;
     }
-    if constexpr (kDirect) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no load into this LDS outlives the workgroup
   }
   // a lane holds row (lane & 15) and four consecutive columns of each 16 x 16 block
   const uint32_t row_first = tile.row0 + wr + (lane & 15), col_first = tile.col0 + wc + (lane >> 4) * 4;
@@ -525,6 +576,61 @@ __global__ __launch_bounds__(S::kThreads) void etha_matmul_kernel(const MatmulAr
   };
   if (tile.row0 + S::BM <= tile.row_end && tile.col0 + S::BN <= a.cols) store_tile(std::true_type{});
   else store_tile(std::false_type{});
+}
+
+// ---- rows shorter than 16 bytes ------------------------------------------------------------------------------------
+// A work-item an element: nothing here is worth a tile.
+template <typename E>
+__device__ inline typename std::conditional<E::kEs == 1, int, float>::type element(const char* p) {
+  if constexpr (E::kEs == 1) return *(const int8_t*)p;
+  else if constexpr (std::is_same_v<E, ElemBF16>) return BF16::to_f32(*(const uint16_t*)p);
+  else return F16::to_f32(*(const uint16_t*)p);
+}
+
+template <typename E, uint32_t KIND, typename D>
+__global__ __launch_bounds__(256) void etha_matmul_short_kernel(const MatmulArgs a) {
+  constexpr bool kTransP = KIND == kGroupReduce, kTransQ = KIND == kGroupReduce || KIND == kGroupRowsT;
+  const uint64_t groups = KIND == kGroupReduce ? a.n_groups : 1, count = groups * a.rows * a.cols;
+  for (uint64_t id = (uint64_t)blockIdx.x * 256 + threadIdx.x; id < count; id += (uint64_t)gridDim.x * 256) {
+    const uint32_t col = (uint32_t)(id % a.cols);
+    const uint64_t row = id / a.cols % a.rows;
+    const uint32_t g = (uint32_t)(id / a.cols / a.rows);
+    const char *p = a.p, *q = a.q;
+    uint32_t red = a.red;
+    int64_t out = (int64_t)g * a.out_group_stride;
+    if constexpr (KIND == kGroupReduce) {
+      int lo = 0;
+      for (uint32_t i = 0; i <= g; i++) {
+        const int v = clamped(a.offsets, i, a.red);
+        lo = v > lo ? v : lo;
+      }
+      const int hi = clamped(a.offsets, g + 1, a.red);
+      red = hi > lo ? hi - lo : 0;
+      p += (int64_t)lo * a.p_stride;
+      q += (int64_t)lo * a.q_stride;
+    } else if constexpr (KIND != kPlain) {
+      uint32_t e = 0;  // the entries up to the row's own, which the largest so far never passes before
+      while (e <= a.n_groups && (uint64_t)clamped(a.offsets, e, a.rows) <= row) e++;
+      if (e == 0 || e > a.n_groups) {  // rows of no group
+        if (!a.zero_rest) continue;
+        red = 0;
+      } else {
+        q += (int64_t)(e - 1) * a.q_group_stride;
+      }
+    }
+    p += kTransP ? (int64_t)row * E::kEs : (int64_t)row * a.p_stride;
+    q += kTransQ ? (int64_t)col * E::kEs : (int64_t)col * a.q_stride;
+    typename std::conditional<E::kEs == 1, int, float>::type sum = 0;
+    for (uint32_t k = 0; k < red; k++)
+      sum += element<E>(p + (kTransP ? (int64_t)k * a.p_stride : (int64_t)k * E::kEs)) *
+             element<E>(q + (kTransQ ? (int64_t)k * a.q_stride : (int64_t)k * E::kEs));
+    float v = (float)sum;
+    if constexpr (E::kEs == 1) {
+      v *= a.row_scale[row] * a.col_scale[col];
+      if (a.bias) v += a.bias[col];
+    }
+    ((typename D::bits*)a.out)[out + (int64_t)row * a.out_stride + col] = D::from_f32(v);
+  }
 }
 
 // ---- few rows --------------------------------------------------------------------------------------------------------
@@ -737,6 +843,8 @@ int check_sizes(const char* what, uint64_t rows, uint64_t cols, uint64_t red, ui
 
 // Whether an operand's tiles can be brought straight into LDS, see DirectStage.  `across`: elements of a row of memory
 // where it lies transposed; rows that overlap (a broadcast gradient) would leave what is past the end of k within the tile.
+constexpr uint32_t kMostStride = 1u << 23;  // bytes between rows: offsets within a tile of 256 of them have 32 bits
+
 bool is_direct(const void* base, int64_t stride, int64_t group_stride, uint64_t k_bytes, bool trans, uint64_t across) {
   return !(((uintptr_t)base | (uint64_t)stride | (uint64_t)group_stride) & 15) && stride >= 0 && stride < 1 << 22 &&
          (trans ? (uint64_t)stride >= across * 2 : !(k_bytes & 15));
@@ -767,6 +875,11 @@ int launch_matmul(const char* what, const MatmulArgs& a, void* stream) {
 }
 
 
+template <typename E, uint32_t KIND, typename D, typename S>
+int launch_shape(const char* what, const MatmulArgs& a, bool direct, void* stream) {
+  return direct ? launch_matmul<E, KIND, D, S, DirectStage>(what, a, stream) : launch_matmul<E, KIND, D, S, RegisterStage>(what, a, stream);
+}
+
 template <typename E, uint32_t KIND, typename D, typename SX, int MT>
 int launch_few(const char* what, const FewArgs& few, void* stream) {
   const uint64_t blocks = row_tiles_of(few.m, KIND, MT * 16) * (((uint64_t)few.m.cols + kFewCols - 1) / kFewCols);
@@ -794,12 +907,19 @@ double tile_cost(const MatmulArgs& a, uint32_t kind, int es, int bm, int bn, int
 
 template <typename E, uint32_t KIND, typename D>
 int shaped_matmul(const char* what, const MatmulArgs& a, bool direct, void* stream) {
+  const uint64_t p_row = (uint64_t)(KIND == kGroupReduce ? a.rows : a.red) * E::kEs;
+  const uint64_t q_row = (uint64_t)(KIND == kGroupReduce || KIND == kGroupRowsT ? a.cols : a.red) * E::kEs;
+  if (!direct && (p_row < 16 || q_row < 16)) {
+    const uint64_t blocks = ((KIND == kGroupReduce ? a.n_groups : 1ull) * a.rows * a.cols + 255) / 256;
+    hipLaunchKernelGGL((etha_matmul_short_kernel<E, KIND, D>), dim3((uint32_t)(blocks < 1u << 20 ? blocks : 1u << 20)), dim3(256), 0,
+                       (hipStream_t)stream, a);
+    return launched("etha_matmul_short_kernel");
+  }
   if constexpr (KIND == kGroupReduce) {
     // the tall reduction pays for the large tile from about a stage or two of rows on, if there are tiles for every CU
     const uint64_t tiles = row_tiles_of(a, KIND, ShapeL::BM) * (((uint64_t)a.cols + ShapeL::BN - 1) / ShapeL::BN);
-    if (!direct) return launch_matmul<E, KIND, D, ShapeM, RegisterStage>(what, a, stream);
-    if (tiles >= 192 && a.red / a.n_groups >= 96) return launch_matmul<E, KIND, D, ShapeL, DirectStage>(what, a, stream);
-    return launch_matmul<E, KIND, D, ShapeM, DirectStage>(what, a, stream);
+    if (tiles >= 192 && a.red / a.n_groups >= 96) return launch_shape<E, KIND, D, ShapeL>(what, a, direct, stream);
+    return launch_shape<E, KIND, D, ShapeM>(what, a, direct, stream);
   } else {
     double cost[6];
     const double none = 1e30;
@@ -809,7 +929,7 @@ int shaped_matmul(const char* what, const MatmulArgs& a, bool direct, void* stre
     cost[2] = few ? tile_cost(a, KIND, E::kEs, 64, kFewCols, 256, 6000) : none;
     cost[3] = tile_cost(a, KIND, E::kEs, ShapeS::BM, ShapeS::BN, 512, 4600);
     cost[4] = tile_cost(a, KIND, E::kEs, ShapeM::BM, ShapeM::BN, 512, 5200);
-    cost[5] = direct ? tile_cost(a, KIND, E::kEs, ShapeL::BM, ShapeL::BN, 256, 4600) : none;
+    cost[5] = tile_cost(a, KIND, E::kEs, ShapeL::BM, ShapeL::BN, 256, 4600);
     int best = 0;
     for (int i = 1; i < 6; i++)
       if (cost[i] < cost[best]) best = i;
@@ -820,17 +940,19 @@ int shaped_matmul(const char* what, const MatmulArgs& a, bool direct, void* stre
       if (best == 1) return launch_few<E, KIND, D, void, 2>(what, args, stream);
       if (best == 2) return launch_few<E, KIND, D, void, 4>(what, args, stream);
     }
-    if (best == 5) return launch_matmul<E, KIND, D, ShapeL, DirectStage>(what, a, stream);
-    if (best == 4)
-      return direct ? launch_matmul<E, KIND, D, ShapeM, DirectStage>(what, a, stream) : launch_matmul<E, KIND, D, ShapeM, RegisterStage>(what, a, stream);
-    return direct ? launch_matmul<E, KIND, D, ShapeS, DirectStage>(what, a, stream) : launch_matmul<E, KIND, D, ShapeS, RegisterStage>(what, a, stream);
+    if (best == 5) return launch_shape<E, KIND, D, ShapeL>(what, a, direct, stream);
+    if (best == 4) return launch_shape<E, KIND, D, ShapeM>(what, a, direct, stream);
+    return launch_shape<E, KIND, D, ShapeS>(what, a, direct, stream);
   }
 }
 
 template <typename E, uint32_t KIND>
 int run_matmul(const char* what, const MatmulArgs& a, uint32_t out_dtype, void* stream) {
   constexpr bool kTransP = KIND == kGroupReduce, kTransQ = KIND == kGroupReduce || KIND == kGroupRowsT;
+  if (a.p_stride < 0 || a.q_stride < 0 || a.p_stride > kMostStride || a.q_stride > kMostStride)
+    return fail(ETHA_ERR_UNSUPPORTED, "%s: rows have to lie at most %u bytes apart", what, kMostStride);
   const uint64_t k_bytes = (uint64_t)a.red * E::kEs;
+  if (KIND != kGroupReduce && k_bytes > 1u << 30) return fail(ETHA_ERR_UNSUPPORTED, "%s: sums over at most 2^30 bytes of a row", what);
   const bool direct = is_direct(a.p, a.p_stride, 0, k_bytes, kTransP, a.rows) &&
                       is_direct(a.q, a.q_stride, a.q_group_stride, k_bytes, kTransQ, a.cols);
   if (out_dtype == ETHA_F32) return shaped_matmul<E, KIND, F32>(what, a, direct, stream);

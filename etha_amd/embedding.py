@@ -35,7 +35,7 @@ def _lookup(tokens, weight, scale, first_row, dtype, out):
         dtype = dtype or weight.dtype
         out_code = code_of("embedding", dtype)
         device = check_device("embedding", weight, tokens)
-        out = torch.empty((*tokens.shape, width), dtype=dtype, device=device)
+        out = weight.new_empty((*tokens.shape, width), dtype=dtype)
         out_stride = width
     else:
         if dtype is not None and dtype != out.dtype:
@@ -100,7 +100,7 @@ def embedding_grad(grad: torch.Tensor, tokens: torch.Tensor, n_rows: int, *, sca
         dtype = dtype or grad.dtype
         out_code = code_of("embedding_grad", dtype)
         device = check_device("embedding_grad", grad, tokens)
-        out = torch.empty((n_rows, width), dtype=dtype, device=device)
+        out = grad.new_empty((n_rows, width), dtype=dtype)
         out_stride = width
     else:
         if dtype is not None and dtype != out.dtype:
@@ -109,7 +109,7 @@ def embedding_grad(grad: torch.Tensor, tokens: torch.Tensor, n_rows: int, *, sca
         out_code = DTYPE_CODES[out.dtype]
         device = check_device("embedding_grad", grad, tokens, out)
     nbytes = _native.embedding_grad_workspace(n_tokens, n_rows, width, grad_code)
-    workspace = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+    workspace = grad.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
     call(device, "etha_embedding_grad", grad.data_ptr(), grad_code, grad_stride, source.data_ptr(),
          token_code, n_tokens, n_rows, width, first_row, scale, out.data_ptr(), out_code, out_stride, int(accumulate),
          workspace.data_ptr() if nbytes else None, nbytes)

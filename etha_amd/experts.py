@@ -11,7 +11,7 @@ from __future__ import annotations
 import torch
 
 from . import _native
-from ._operands import DTYPE_CODES, call, check_device, check_out, code_of, readable_rows, refuse_captured_backward
+from ._operands import DTYPE_CODES, MOST_STRIDE, call, check_device, check_out, code_of, readable_rows, refuse_captured_backward
 
 _OPERANDS = {torch.bfloat16: _native.BF16, torch.float16: _native.F16}
 
@@ -19,22 +19,29 @@ _OPERANDS = {torch.bfloat16: _native.BF16, torch.float16: _native.F16}
 def _check(what: str, weight: torch.Tensor | None, offsets: torch.Tensor, *rows: torch.Tensor) -> None:
     if offsets.dim() != 1 or offsets.dtype != torch.int32 or offsets.numel() < 1:
         raise ValueError(f"{what}: offsets are {offsets.dtype} {tuple(offsets.shape)}, not int32 [experts + 1]")
-    if weight is not None and weight.dim() != 3:
-        raise ValueError(f"{what}: weight has {weight.dim()} dims, not [experts, out, in]")
-    if weight is not None and weight.shape[0] != offsets.numel() - 1:
-        raise ValueError(f"{what}: {weight.shape[0]} experts and {offsets.numel()} offsets")
+    dtype = rows[0].dtype
+    same = dtype in _OPERANDS
+    if weight is not None:
+        if weight.dim() != 3:
+            raise ValueError(f"{what}: weight has {weight.dim()} dims, not [experts, out, in]")
+        if weight.shape[0] != offsets.numel() - 1:
+            raise ValueError(f"{what}: {weight.shape[0]} experts and {offsets.numel()} offsets")
+        same = same and weight.dtype == dtype
     for t in rows:
         if t.dim() != 2:
             raise ValueError(f"{what}: rows have {t.dim()} dims, not 2")
-    dtypes = {t.dtype for t in (*rows, *(() if weight is None else (weight,)))}
-    if len(dtypes) != 1 or next(iter(dtypes)) not in _OPERANDS:
-        raise ValueError(f"{what}: operands are {', '.join(sorted(map(str, dtypes)))}; all bfloat16 or all float16 are supported")
+        same = same and t.dtype == dtype
+    if not same:
+        dtypes = {str(t.dtype) for t in (*rows, *(() if weight is None else (weight,)))}
+        raise ValueError(f"{what}: operands are {', '.join(sorted(dtypes))}; all bfloat16 or all float16 are supported")
 
 
 def _matrices(what: str, weight: torch.Tensor) -> tuple[torch.Tensor, int, int]:
     """Row and matrix stride of a weight whose rows are contiguous."""
     if weight.stride(2) != 1 and weight.shape[2] > 1:
         raise ValueError(f"{what}: the rows of weight have to be contiguous")
+    if weight.stride(1) * 2 > MOST_STRIDE:
+        weight = weight.contiguous()
     return weight, weight.stride(1), weight.stride(0)
 
 
@@ -44,7 +51,7 @@ def _product(what, x, weight, offsets, transposed, out):
     cols, red = (k, n) if transposed else (n, k)
     if x.shape[1] != red:
         raise ValueError(f"{what}: rows of {x.shape[1]} elements and a weight of {tuple(weight.shape)}")
-    source, stride = readable_rows(x)
+    source, stride = readable_rows(x, MOST_STRIDE)
     weight, w_stride, w_group = _matrices(what, weight)
     offsets = offsets if offsets.is_contiguous() else offsets.contiguous()
     rows = x.shape[0]
@@ -53,7 +60,7 @@ def _product(what, x, weight, offsets, transposed, out):
         out_stride = check_out(what, out, (rows, cols), DTYPE_CODES, x, weight, offsets)
     device = check_device(what, x, weight, offsets, out)
     if fresh:
-        out, out_stride = torch.empty((rows, cols), dtype=x.dtype, device=device), cols
+        out, out_stride = x.new_empty((rows, cols)), cols
     call(device, "etha_grouped_matmul", source.data_ptr(), _OPERANDS[x.dtype], rows, stride,
          weight.data_ptr(), experts, cols, red, w_stride, w_group, int(transposed), offsets.data_ptr(), out.data_ptr(),
          DTYPE_CODES[out.dtype], out_stride, int(fresh))
@@ -106,8 +113,8 @@ def grouped_linear_grad_weight(grad: torch.Tensor, x: torch.Tensor, offsets: tor
     if grad.shape[0] != x.shape[0]:
         raise ValueError(f"{what}: {grad.shape[0]} rows of grad and {x.shape[0]} of x")
     experts, n, k = offsets.numel() - 1, grad.shape[1], x.shape[1]
-    g, g_stride = readable_rows(grad)
-    r, r_stride = readable_rows(x)
+    g, g_stride = readable_rows(grad, MOST_STRIDE)
+    r, r_stride = readable_rows(x, MOST_STRIDE)
     offsets = offsets if offsets.is_contiguous() else offsets.contiguous()
     if out is None:
         dtype = dtype or x.dtype
@@ -118,7 +125,7 @@ def grouped_linear_grad_weight(grad: torch.Tensor, x: torch.Tensor, offsets: tor
         check_out(what, out, (experts, n, k), DTYPE_CODES, grad, x, offsets)
     device = check_device(what, x, grad, offsets, out)
     if out is None:
-        out = torch.empty((experts, n, k), dtype=dtype, device=device)
+        out = x.new_empty((experts, n, k), dtype=dtype)
     call(device, "etha_grouped_matmul_reduce", g.data_ptr(), r.data_ptr(), _OPERANDS[x.dtype],
          x.shape[0], g_stride, r_stride, experts, n, k, offsets.data_ptr(), out.data_ptr(), DTYPE_CODES[out.dtype], out.stride(1),
          out.stride(0))

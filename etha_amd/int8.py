@@ -11,7 +11,7 @@ from __future__ import annotations
 import torch
 
 from . import _native
-from ._operands import DTYPE_CODES, call, check_device, check_out, code_of, readable_rows, refuse_grad
+from ._operands import DTYPE_CODES, MOST_STRIDE, call, check_device, check_out, code_of, readable_rows, refuse_grad
 
 INT8_MAX_WIDTH = 131071  # ETHA_INT8_MAX_WIDTH
 
@@ -39,9 +39,9 @@ def quantize_rows(x: torch.Tensor, *, values: torch.Tensor | None = None,
     rows = x.numel() // width if width else x.shape[:-1].numel()
     source, stride = readable_rows(x)
     if values is None:
-        values, values_stride = torch.empty(x.shape, dtype=torch.int8, device=device), width
+        values, values_stride = x.new_empty(x.shape, dtype=torch.int8), width
     if scales is None:
-        scales = torch.empty(x.shape[:-1], dtype=torch.float32, device=device)
+        scales = x.new_empty(x.shape[:-1], dtype=torch.float32)
     call(device, "etha_quantize_rows", source.data_ptr(), code, rows, width, stride,
          values.data_ptr(), values_stride, scales.data_ptr())
     return values, scales
@@ -64,7 +64,7 @@ def _weight_operands(what, x, weight, weight_scales, bias):
     weight_scales = _check_scales(what, "weight_scales", weight_scales, (channels,))
     if bias is not None:
         bias = _check_scales(what, "bias", bias, (channels,))
-    weight, stride = readable_rows(weight)
+    weight, stride = readable_rows(weight, MOST_STRIDE)
     rows = x.numel() // width if width else x.shape[:-1].numel()
     return weight, stride, weight_scales, bias, channels, width, rows
 
@@ -82,13 +82,13 @@ def int8_matmul(x: torch.Tensor, x_scales: torch.Tensor, weight: torch.Tensor, w
     refuse_grad(what, x_scales, weight_scales, bias)
     weight, w_stride, weight_scales, bias, channels, width, rows = _weight_operands(what, x, weight, weight_scales, bias)
     x_scales = _check_scales(what, "x_scales", x_scales, x.shape[:-1])
-    source, stride = readable_rows(x)
+    source, stride = readable_rows(x, MOST_STRIDE)
     if out is not None:
         out_stride = check_out(what, out, (*x.shape[:-1], channels), DTYPE_CODES, x, x_scales, weight, weight_scales, bias)
     device = check_device(what, x, x_scales, weight, weight_scales, bias, out)
     if out is None:
         code_of(what, dtype)
-        out, out_stride = torch.empty((*x.shape[:-1], channels), dtype=dtype, device=device), channels
+        out, out_stride = x.new_empty((*x.shape[:-1], channels), dtype=dtype), channels
     call(device, "etha_int8_matmul", source.data_ptr(), x_scales.data_ptr(), rows, stride,
          weight.data_ptr(), weight_scales.data_ptr(), channels, w_stride, width, None if bias is None else bias.data_ptr(),
          out.data_ptr(), DTYPE_CODES[out.dtype], out_stride)
@@ -113,9 +113,9 @@ def int8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scales: torch.Tens
     if out is None:
         dtype = dtype or x.dtype
         code_of(what, dtype)
-        out, out_stride = torch.empty((*x.shape[:-1], channels), dtype=dtype, device=device), channels
+        out, out_stride = x.new_empty((*x.shape[:-1], channels), dtype=dtype), channels
     nbytes = _native.int8_linear_workspace(rows, channels, width)
-    workspace = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+    workspace = x.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
     call(device, "etha_int8_linear", source.data_ptr(), x_code, rows, stride, weight.data_ptr(),
          weight_scales.data_ptr(), channels, w_stride, width, None if bias is None else bias.data_ptr(), out.data_ptr(),
          DTYPE_CODES[out.dtype], out_stride, workspace.data_ptr() if nbytes else None, nbytes)

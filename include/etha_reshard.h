@@ -325,6 +325,7 @@ int etha_ipc_close(void* opened_ptr);
  * reference, which leaves them to the framework on either side of it.
  *  - tensors are given by address and strides in elements of their own type; the last dimension is contiguous; rows
  *    may start at any multiple of the element size.  Types are ETHA_F32, ETHA_BF16 and ETHA_F16 unless said otherwise.
+ *    Operands of products have rows at most 8 MiB apart.
  *  - sums are held in fp32 (32-bit integers for 8-bit products) and rounded once.
  *  - results do not depend on timing: the same call on the same values gives the same bits.
  *  - launches are asynchronous on `stream` of the current device and can be captured into a graph; nothing is allocated.

@@ -107,6 +107,7 @@ def test_entry_points_refuse_what_they_cannot_take():
     assert mul(m=1 << 31) == nat.ERR_UNSUPPORTED
     for name in ("x", "w", "off", "o"):
         assert mul(**{name: None}) == nat.ERR_INVALID
+    assert mul(xs=(1 << 22) + 8) == nat.ERR_UNSUPPORTED and mul(ws=-8) == nat.ERR_UNSUPPORTED
     assert mul(m=0) == 0 and mul(n=0) == 0
     red = lambda **k: lib.etha_grouped_matmul_reduce(*{**dict(g=0x1000, x=0x1000, d=nat.F16, m=4, gs=8, xs=8, e=2, n=8, k=8, off=0x1000,
                                                               o=0x1000, od=nat.F32, os=8, og=64, st=None), **k}.values())
@@ -209,6 +210,19 @@ def test_views(gpu_device):
         check_rows(grouped_linear(many, weight, offsets), many, weight, offsets)
         same = weight[:1].expand(2, 128, 256)  # one matrix for all experts
         check_rows(grouped_linear(x, same, offsets), x, same, offsets)
+
+
+@pytest.mark.gpu
+def test_rows_far_apart(gpu_device):
+    """Rows 8 MiB apart are read where they lie, rows further apart are copied first."""
+    gen = torch.Generator(device=gpu_device).manual_seed(15)
+    x, weight, offsets, grad = case(gen, [130, 0, 140], 72, 96, torch.bfloat16, gpu_device)
+    for apart in (1 << 22, (1 << 22) + 8):
+        far = torch.empty(270, apart, dtype=torch.bfloat16, device=gpu_device)[:, 3:99]
+        far.copy_(x)
+        check_rows(grouped_linear(far, weight, offsets), x, weight, offsets)
+        check_weight(grouped_linear_grad_weight(grad, far, offsets), grad, x, offsets)
+        del far
 
 
 @pytest.mark.gpu
