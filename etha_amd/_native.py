@@ -158,8 +158,9 @@ _SIGNATURES = {
                                  c_void_p, c_uint32, c_int64, c_void_p, c_uint64, c_void_p]),
     "etha_grouped_matmul": (c_int, [c_void_p, c_uint32, c_uint64, c_int64, c_void_p, c_uint64, c_uint64, c_uint64, c_int64, c_int64,
                                     c_int, c_void_p, c_void_p, c_uint32, c_int64, c_int, c_void_p]),
+    "etha_grouped_matmul_reduce_workspace": (c_int, [c_uint64, c_uint64, c_uint64, c_uint64, POINTER(c_uint64)]),
     "etha_grouped_matmul_reduce": (c_int, [c_void_p, c_void_p, c_uint32, c_uint64, c_int64, c_int64, c_uint64, c_uint64, c_uint64,
-                                           c_void_p, c_void_p, c_uint32, c_int64, c_int64, c_void_p]),
+                                           c_void_p, c_void_p, c_uint32, c_int64, c_int64, c_void_p, c_uint64, c_void_p]),
 }
 
 _lib = None
@@ -436,6 +437,14 @@ def int8_linear_workspace(rows: int, cols: int, width: int) -> int:
     """Bytes of workspace that ``etha_int8_linear`` needs for these sizes."""
     out = c_uint64()
     _check("etha_int8_linear_workspace", lib().etha_int8_linear_workspace(rows, cols, width, byref(out)))
+    return out.value
+
+
+def grouped_matmul_reduce_workspace(rows: int, n_groups: int, out_rows: int, out_cols: int) -> int:
+    """Bytes of workspace that ``etha_grouped_matmul_reduce`` needs for these sizes."""
+    out = c_uint64()
+    _check("etha_grouped_matmul_reduce_workspace",
+           lib().etha_grouped_matmul_reduce_workspace(rows, n_groups, out_rows, out_cols, byref(out)))
     return out.value
 
 

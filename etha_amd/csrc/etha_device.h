@@ -56,6 +56,38 @@ __device__ inline void store_raw(void* p, typename Raw<BYTES>::type v) {
   else *(any*)p = v;
 }
 
+// 16 bytes at p of which `left` exist; the others read as zero
+template <int ES>
+__device__ inline u32x4 load_part(const char* p, int64_t left) {
+  if (left >= 16) return load_raw<16>(p);
+  u32x4 v = {0, 0, 0, 0};
+  if (left <= 0) return v;
+  if constexpr (ES == 2) {
+    #pragma unroll
+    for (int i = 0; i < 8; i++)
+      if (2 * i < left) v[i >> 1] |= (uint32_t)*(const uint16_t*)(p + 2 * i) << (16 * (i & 1));
+  } else if constexpr (ES == 4) {
+    #pragma unroll
+    for (int i = 0; i < 4; i++)
+      if (4 * i < left) v[i] = *(const uint32_t*)(p + 4 * i);
+  } else {
+    #pragma unroll
+    for (int i = 0; i < 16; i++)
+      if (i < left) v[i >> 2] |= (uint32_t)*(const uint8_t*)(p + i) << (8 * (i & 3));
+  }
+  return v;
+}
+
+// The elements of 16 bytes as fp32
+template <typename T, int N>
+__device__ inline void raw_to_f32(float (&out)[N], u32x4 raw) {
+  static_assert(N * sizeof(typename T::bits) == 16, "one vector");
+  typename T::bits e[N];
+  __builtin_memcpy(e, &raw, 16);
+  #pragma unroll
+  for (int i = 0; i < N; i++) out[i] = T::to_f32(e[i]);
+}
+
 // N consecutive elements of type T as fp32; `n` of them exist (the rest read as zero)
 template <typename T, int N, bool NT = false>
 __device__ inline void load_f32(float (&out)[N], const typename T::bits* p, int64_t n) {
@@ -108,9 +140,11 @@ __device__ inline uint32_t largest_bits(const float (&v)[8], uint32_t top) {
   }
   return top;
 }
-__device__ inline uint32_t wave_max(uint32_t v) {
+// the largest of each group of LANES lanes, in all of them
+template <int LANES>
+__device__ inline uint32_t group_max(uint32_t v) {
   #pragma unroll
-  for (int d = 32; d; d >>= 1) {
+  for (int d = LANES / 2; d; d >>= 1) {
     const uint32_t o = __shfl_xor(v, d);
     v = o > v ? o : v;
   }

@@ -65,6 +65,8 @@ struct MatmulArgs {
   const float* row_scale;                      // 8 bits
   const float* col_scale;
   const float* bias;
+  uint32_t splits;                             // kGroupReduce: parts that a group's rows are cut into, each with an output
+  int64_t split_stride;                        // of its own, in elements
 };
 
 // ---- groups --------------------------------------------------------------------------------------------------------
@@ -236,24 +238,6 @@ struct DirectStage {
   }
 };
 
-// 16 bytes at p of which `left` exist; the others read as zero
-template <int ES>
-__device__ inline u32x4 load_part(const char* p, int64_t left) {
-  if (left >= 16) return load_raw<16>(p);
-  u32x4 v = {0, 0, 0, 0};
-  if (left <= 0) return v;
-  if constexpr (ES == 2) {
-    #pragma unroll
-    for (int i = 0; i < 8; i++)
-      if (2 * i < left) v[i >> 1] |= (uint32_t)*(const uint16_t*)(p + 2 * i) << (16 * (i & 1));
-  } else {
-    #pragma unroll
-    for (int i = 0; i < 16; i++)
-      if (i < left) v[i >> 2] |= (uint32_t)*(const uint8_t*)(p + i) << (8 * (i & 3));
-  }
-  return v;
-}
-
 // n bytes (0 to 16) dropped at the low end, zeros in at the high end
 __device__ inline u32x4 shift_bytes(u32x4 v, uint32_t n) {
   uint64_t lo = (uint64_t)v.y << 32 | v.x, hi = (uint64_t)v.w << 32 | v.z;
@@ -351,6 +335,7 @@ struct Tile {
 template <typename E, uint32_t KIND, typename S>
 __device__ inline Tile locate(const MatmulArgs& a) {
   constexpr bool kTransP = KIND == kGroupReduce, kTransQ = KIND == kGroupReduce || KIND == kGroupRowsT;
+  constexpr uint32_t kStageK = kStageBytes / E::kEs;
   Tile t = {};
   t.there = true;
   uint32_t id = blockIdx.x;
@@ -377,10 +362,17 @@ __device__ inline Tile locate(const MatmulArgs& a) {
   if constexpr (KIND == kGroupReduce) {
     uint32_t lo, hi;
     group_bounds(a, group, &lo, &hi);
+    if (a.splits > 1) {  // this part's stages
+      const uint32_t part = ((hi - lo + kStageK - 1) / kStageK + a.splits - 1) / a.splits * kStageK;
+      const uint64_t from = (uint64_t)lo + (uint64_t)blockIdx.y * part;
+      lo = from < hi ? (uint32_t)from : hi;
+      hi = hi - lo > part ? lo + part : hi;
+      t.out += (int64_t)blockIdx.y * a.split_stride;
+    }
     t.red = hi - lo;
     t.p += (int64_t)lo * a.p_stride;
     t.q += (int64_t)lo * a.q_stride;
-    t.out = (int64_t)group * a.out_group_stride;
+    t.out += (int64_t)group * a.out_group_stride;
   } else if constexpr (KIND != kPlain) {
     const GroupTile g = find_tile<S::BM>(a, row_id);
     t.there = g.found;
@@ -750,7 +742,7 @@ __global__ __launch_bounds__(kFewThreads) void etha_few_rows_kernel(const FewArg
           load_f32<SX, 8>(v, rows + (int64_t)(row0 + m) * few.x_stride + k, (int64_t)red - k);
           top = largest_bits(v, top);
         }
-        top = wave_max(top);
+        top = group_max<64>(top);
         if (lane == 0) s_top[m][wave] = top;
       }
     __syncthreads();
@@ -826,6 +818,101 @@ __global__ __launch_bounds__(kFewThreads) void etha_few_rows_kernel(const FewArg
   }
 }
 
+// A few rows against matrices that lie transposed (the gradient of the rows): the same stream.  A workgroup takes 64 columns,
+// which are 128 bytes of a row of memory, and each wave every eighth run of 64 rows of k; the transposing LDS load turns
+// them.  Pieces that reach over the end of a row or of k are handled as RegisterStage does it.
+constexpr int kFewColsT = 64;
+
+template <typename E, typename D>
+__global__ __launch_bounds__(kFewThreads) void etha_few_rows_transposed_kernel(const MatmulArgs a) {
+  typedef Operand<E, true, kFewColsT, 128> OpQ;  // for the layouts of the LDS tiles
+  typedef Operand<E, false, 16, 128> OpP;
+  constexpr uint32_t kRun = 64;
+  __shared__ __align__(1024) char s_tile[kFewWaves][OpQ::kBytes + OpP::kBytes];  // the wave's own until the last barrier
+  const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t col_tiles = (a.cols + kFewColsT - 1) / kFewColsT;
+  const uint32_t col0 = blockIdx.x % col_tiles * kFewColsT;
+  const GroupTile g = find_tile<16>(a, blockIdx.x / col_tiles);
+  if (!g.found) return;
+  const uint32_t row0 = g.lo + g.tile * 16, n_rows = g.hi - row0 < 16 ? g.hi - row0 : 16;
+  const uint32_t n_cols = a.cols - col0 < kFewColsT ? a.cols - col0 : kFewColsT;
+  const uint32_t red = g.group == a.n_groups ? 0 : a.red;
+  const char* q = a.q + (g.group == a.n_groups ? 0 : (int64_t)g.group * a.q_group_stride) + (int64_t)col0 * 2;
+  const char* p = a.p + (int64_t)row0 * a.p_stride;
+  char* tile = s_tile[wave];
+  const uint32_t row = lane >> 3, piece = (lane & 7) * 16;  // of 8 rows of 128 bytes, in memory
+  const int left_q = (int)(n_cols * 2) - (int)piece;
+  const int at_q = left_q >= 16 ? (int)piece : (int)(n_cols * 2) - 16;
+  const uint32_t shift_q = left_q >= 16 || left_q <= 0 ? 0 : 16 - left_q;
+  const uint32_t prow[2] = {row < n_rows ? row : n_rows - 1, row + 8 < n_rows ? row + 8 : n_rows - 1};
+  f32x4 acc[4] = {};
+  for (uint32_t k0 = wave * kRun; k0 < red; k0 += kFewWaves * kRun) {
+    const uint32_t inside = red - k0 < kRun ? red - k0 : kRun;
+    const int left_p = (int)((red - k0) * 2) - (int)piece;
+    const uint32_t at_p = left_p >= 16 ? k0 * 2 + piece : red * 2 - 16;
+    const uint32_t shift_p = left_p >= 16 ? 0 : left_p > 0 ? 16 - left_p : 16;
+    u32x4 vq[8], vp[2];
+    #pragma unroll
+    for (uint32_t i = 0; i < 8; i++)
+      vq[i] = load_raw<16, true>(q + (int64_t)(k0 + (i * 8 + row < inside ? i * 8 + row : inside - 1)) * a.q_stride + at_q);
+    #pragma unroll
+    for (int i = 0; i < 2; i++) vp[i] = load_raw<16>(p + (int64_t)prow[i] * a.p_stride + at_p);
+    if (inside < kRun || n_cols < kFewColsT) {
+      #pragma unroll
+      for (uint32_t i = 0; i < 8; i++) vq[i] = shift_bytes(vq[i], i * 8 + row >= inside ? 16 : shift_q);
+      #pragma unroll
+      for (int i = 0; i < 2; i++) vp[i] = shift_bytes(vp[i], shift_p);
+    }
+    #pragma unroll
+    for (uint32_t i = 0; i < 8; i++) *(u32x4*)(tile + (i * 8 + row) * 128 + OpQ::swizzle(i * 8 + row, lane & 7) * 16) = vq[i];
+    #pragma unroll
+    for (uint32_t i = 0; i < 2; i++) *(u32x4*)(tile + OpQ::kBytes + (i * 8 + row) * 128 + OpP::swizzle(i * 8 + row, lane & 7) * 16) = vp[i];
+    #pragma unroll
+    for (int h = 0; h < 2; h++) {
+      const u32x4 fp = OpP::fragment(tile + OpQ::kBytes, 0, h * 4);
+      #pragma unroll
+      for (int j = 0; j < 4; j++) acc[j] = E::mfma(OpQ::fragment(tile, j * 16, h * 4), fp, acc[j]);
+    }
+  }
+  float* sums = (float*)tile;
+  #pragma unroll
+  for (int j = 0; j < 4; j++)
+    #pragma unroll
+    for (int c = 0; c < 4; c++) sums[j * 256 + lane * 4 + c] = acc[j][c];
+  __syncthreads();
+  #pragma unroll
+  for (int e = 0; e < 2; e++) {
+    const uint32_t t = threadIdx.x + e * kFewThreads;
+    const uint32_t out_row = row0 + (t >> 2 & 15), col = col0 + (t >> 8) * 16 + (t >> 6 & 3) * 4 + (t & 3);
+    if (out_row >= g.hi || col >= a.cols) continue;
+    float sum = ((const float*)s_tile[0])[t];
+    #pragma unroll
+    for (int i = 1; i < kFewWaves; i++) sum += ((const float*)s_tile[i])[t];
+    ((typename D::bits*)a.out)[(int64_t)out_row * a.out_stride + col] = D::from_f32(sum);
+  }
+}
+
+// The parts of a sum over a group's rows, added up in their order; four columns a work-item.
+template <typename D>
+__global__ __launch_bounds__(256) void etha_join_parts_kernel(const float* parts, uint32_t splits, int64_t split_stride, uint64_t rows,
+                                                              uint32_t group_rows, uint32_t cols, typename D::bits* out, int64_t out_stride,
+                                                              int64_t out_group_stride) {
+  const uint32_t vecs = (cols + 3) / 4;
+  for (uint64_t id = (uint64_t)blockIdx.x * 256 + threadIdx.x; id < rows * vecs; id += (uint64_t)gridDim.x * 256) {
+    const uint64_t row = id / vecs;
+    const uint32_t col = (uint32_t)(id % vecs) * 4;
+    const int64_t left = (int64_t)cols - col;
+    float sum[4] = {}, v[4];
+    #pragma unroll 4
+    for (uint32_t s = 0; s < splits; s++) {
+      load_f32<F32, 4>(v, (const uint32_t*)parts + s * split_stride + (int64_t)row * cols + col, left);
+      #pragma unroll
+      for (int i = 0; i < 4; i++) sum[i] += v[i];
+    }
+    store_f32<D, 4>(out + (int64_t)(row / group_rows) * out_group_stride + (int64_t)(row % group_rows) * out_stride + col, sum, left);
+  }
+}
+
 int launched(const char* name) {
   g_kernel_launches.fetch_add(1, std::memory_order_relaxed);
   const hipError_t e = hipGetLastError();
@@ -870,7 +957,7 @@ int launch_matmul(const char* what, const MatmulArgs& a, void* stream) {
   const uint64_t col_tiles = ((uint64_t)a.cols + S::BN - 1) / S::BN, blocks = row_tiles * col_tiles;
   if (blocks >= 1ull << 22) return fail(ETHA_ERR_UNSUPPORTED, "%s: the product is too large for one call", what);
   if (!blocks) return ETHA_OK;
-  hipLaunchKernelGGL((etha_matmul_kernel<E, KIND, D, S, STAGE>), dim3((uint32_t)blocks), dim3(S::kThreads), 0, (hipStream_t)stream, a);
+  hipLaunchKernelGGL((etha_matmul_kernel<E, KIND, D, S, STAGE>), dim3((uint32_t)blocks, a.splits > 1 ? a.splits : 1), dim3(S::kThreads), 0, (hipStream_t)stream, a);
   return launched("etha_matmul_kernel");
 }
 
@@ -918,13 +1005,14 @@ int shaped_matmul(const char* what, const MatmulArgs& a, bool direct, void* stre
   if constexpr (KIND == kGroupReduce) {
     // the tall reduction pays for the large tile from about a stage or two of rows on, if there are tiles for every CU
     const uint64_t tiles = row_tiles_of(a, KIND, ShapeL::BM) * (((uint64_t)a.cols + ShapeL::BN - 1) / ShapeL::BN);
-    if (tiles >= 192 && a.red / a.n_groups >= 96) return launch_shape<E, KIND, D, ShapeL>(what, a, direct, stream);
+    if (a.splits < 2 && tiles >= 192 && a.red / a.n_groups >= 96) return launch_shape<E, KIND, D, ShapeL>(what, a, direct, stream);
     return launch_shape<E, KIND, D, ShapeM>(what, a, direct, stream);
   } else {
     double cost[6];
     const double none = 1e30;
-    const bool few = KIND != kGroupRowsT;
-    cost[0] = few ? tile_cost(a, KIND, E::kEs, 16, kFewCols, 512, 6000) : none;
+    constexpr bool few = KIND != kGroupRowsT;
+    cost[0] = tile_cost(a, KIND, E::kEs, 16, few ? kFewCols : kFewColsT, 512, 6000);
+    if (!few && (p_row < 16 || q_row < 16)) cost[0] = none;  // its loads begin 16 bytes before the end of a row
     cost[1] = few ? tile_cost(a, KIND, E::kEs, 32, kFewCols, 512, 6000) : none;
     cost[2] = few ? tile_cost(a, KIND, E::kEs, 64, kFewCols, 256, 6000) : none;
     cost[3] = tile_cost(a, KIND, E::kEs, ShapeS::BM, ShapeS::BN, 512, 4600);
@@ -939,6 +1027,14 @@ int shaped_matmul(const char* what, const MatmulArgs& a, bool direct, void* stre
       if (best == 0) return launch_few<E, KIND, D, void, 1>(what, args, stream);
       if (best == 1) return launch_few<E, KIND, D, void, 2>(what, args, stream);
       if (best == 2) return launch_few<E, KIND, D, void, 4>(what, args, stream);
+    }
+    if constexpr (KIND == kGroupRowsT) {
+      if (best == 0) {
+        const uint64_t blocks = row_tiles_of(a, KIND, 16) * (((uint64_t)a.cols + kFewColsT - 1) / kFewColsT);
+        if (blocks >= 1ull << 22) return fail(ETHA_ERR_UNSUPPORTED, "%s: the product is too large for one call", what);
+        hipLaunchKernelGGL((etha_few_rows_transposed_kernel<E, D>), dim3((uint32_t)blocks), dim3(kFewThreads), 0, (hipStream_t)stream, a);
+        return launched("etha_few_rows_transposed_kernel");
+      }
     }
     if (best == 5) return launch_shape<E, KIND, D, ShapeL>(what, a, direct, stream);
     if (best == 4) return launch_shape<E, KIND, D, ShapeM>(what, a, direct, stream);
@@ -970,6 +1066,18 @@ bool is_few(uint64_t rows, uint64_t cols, uint64_t width) {
   return padded <= kFewLds && (rows == 1 || (rows <= kFewConverted && cols <= 8192 && padded <= kFewThreads * 8));
 }
 uint64_t padded_width(uint64_t width) { return (width + 15) / 16 * 16; }
+
+// Parts that the sum over a group's rows is cut into where its tiles are too few for the chip: about two workgroups a CU,
+// each with at least four stages of an even group's rows.
+uint32_t reduce_splits(uint64_t rows, uint64_t n_groups, uint64_t out_rows, uint64_t out_cols) {
+  if (!n_groups || !out_rows || !out_cols) return 1;
+  const uint64_t tiles = n_groups * ((out_rows + ShapeM::BM - 1) / ShapeM::BM) * ((out_cols + ShapeM::BN - 1) / ShapeM::BN);
+  const uint64_t stages = rows / n_groups / 64;
+  if (tiles > 192 || stages < 8 || out_rows * 2 < 16 || out_cols * 2 < 16) return 1;
+  const uint64_t by_tiles = (512 + tiles - 1) / tiles, by_stages = stages / 4;
+  const uint64_t splits = by_tiles < by_stages ? by_tiles : by_stages;
+  return (uint32_t)(splits < 64 ? splits : 64);
+}
 
 template <uint32_t KIND>
 int run_grouped(const char* what, const MatmulArgs& a, uint32_t dtype, uint32_t out_dtype, void* stream) {
@@ -1085,9 +1193,19 @@ int etha_grouped_matmul(const void* x, uint32_t dtype, uint64_t rows, int64_t x_
                       : run_grouped<kGroupRows>("etha_grouped_matmul", a, dtype, out_dtype, stream);
 }
 
+int etha_grouped_matmul_reduce_workspace(uint64_t rows, uint64_t n_groups, uint64_t out_rows, uint64_t out_cols, uint64_t* bytes) {
+  if (!bytes) return fail(ETHA_ERR_INVALID, "etha_grouped_matmul_reduce_workspace: null result");
+  const int rc = check_sizes("etha_grouped_matmul_reduce_workspace", out_rows, out_cols, rows, (1ull << 31) - 1);
+  if (rc != ETHA_OK) return rc;
+  const uint64_t splits = reduce_splits(rows, n_groups, out_rows, out_cols);
+  *bytes = splits < 2 ? 0 : splits * n_groups * out_rows * out_cols * 4;
+  return ETHA_OK;
+}
+
 int etha_grouped_matmul_reduce(const void* grad, const void* x, uint32_t dtype, uint64_t rows, int64_t grad_stride, int64_t x_stride,
                                uint64_t n_groups, uint64_t out_rows, uint64_t out_cols, const int32_t* offsets, void* out,
-                               uint32_t out_dtype, int64_t out_stride, int64_t out_group_stride, void* stream) {
+                               uint32_t out_dtype, int64_t out_stride, int64_t out_group_stride, void* workspace,
+                               uint64_t workspace_bytes, void* stream) {
   int rc = check_groups("etha_grouped_matmul_reduce", offsets, n_groups, dtype, out_dtype);
   if (rc == ETHA_OK) rc = check_sizes("etha_grouped_matmul_reduce", out_rows, out_cols, rows, (1ull << 31) - 1);
   if (rc != ETHA_OK) return rc;
@@ -1106,7 +1224,27 @@ int etha_grouped_matmul_reduce(const void* grad, const void* x, uint32_t dtype, 
   a.red = (uint32_t)rows;
   a.offsets = offsets;
   a.n_groups = (uint32_t)n_groups;
-  return run_grouped<kGroupReduce>("etha_grouped_matmul_reduce", a, dtype, out_dtype, stream);
+  const uint32_t splits = reduce_splits(rows, n_groups, out_rows, out_cols);
+  if (splits < 2) return run_grouped<kGroupReduce>("etha_grouped_matmul_reduce", a, dtype, out_dtype, stream);
+  const uint64_t elements = n_groups * out_rows * out_cols;
+  if (!workspace || workspace_bytes < splits * elements * 4 || ((uintptr_t)workspace & 15))
+    return fail(ETHA_ERR_INVALID, "etha_grouped_matmul_reduce: the workspace has to hold %llu bytes at a 16-byte address",
+                (unsigned long long)(splits * elements * 4));
+  a.out = workspace;
+  a.out_stride = (int64_t)out_cols;
+  a.out_group_stride = (int64_t)(out_rows * out_cols);
+  a.splits = splits;
+  a.split_stride = (int64_t)elements;
+  rc = run_grouped<kGroupReduce>("etha_grouped_matmul_reduce", a, dtype, ETHA_F32, stream);
+  if (rc != ETHA_OK) return rc;
+  const uint64_t blocks = (n_groups * out_rows * ((out_cols + 3) / 4) + 255) / 256;
+  with_type(out_dtype, [&](auto d) {
+    typedef decltype(d) D;
+    hipLaunchKernelGGL((etha_join_parts_kernel<D>), dim3((uint32_t)(blocks < 1u << 20 ? blocks : 1u << 20)), dim3(256), 0, (hipStream_t)stream,
+                       (const float*)workspace, splits, (int64_t)elements, n_groups * out_rows, (uint32_t)out_rows, (uint32_t)out_cols,
+                       (typename D::bits*)out, out_stride, out_group_stride);
+  });
+  return launched("etha_join_parts_kernel");
 }
 
 }  // extern "C"

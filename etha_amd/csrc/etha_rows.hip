@@ -299,20 +299,58 @@ struct GradArgs {
   float scale;
 };
 
-template <typename D, int N>
-__device__ inline void write_row(const GradArgs& a, uint32_t row, uint64_t col, float (&acc)[N]) {
-  typename D::bits* p = (typename D::bits*)a.out + (int64_t)row * a.out_stride + col;
-  const int64_t left = (int64_t)(a.width - col);
-  float v[N];
-  if (a.accumulate) {
-    load_f32<D, N>(v, p, left);
+// The columns of a lane.  Vectors that would reach over the end of a row begin earlier, at `at`, so that no load branches:
+// their first columns are the neighbour's too and come out the same there.  Rows shorter than a vector (`narrow`) are read
+// by elements.
+template <int N>
+struct Columns {
+  uint64_t own, at;
+  bool inside, narrow;
+  __device__ Columns(uint64_t col, uint64_t width) {
+    own = col;
+    inside = col < width;
+    narrow = width < N;
+    at = narrow ? 0 : col + N <= width ? col : width - N;
+  }
+};
+
+// `count` of K rows of a gradient (the rest repeat the first), all loads on their way at once
+template <typename S, int N, int K, typename ROW>
+__device__ inline void load_rows(u32x4 (&raw)[K], const GradArgs& a, const Columns<N>& c, uint32_t count, ROW&& row) {
+  if (!c.narrow) {
     #pragma unroll
-    for (int i = 0; i < N; i++) v[i] += acc[i] * a.scale;
+    for (int u = 0; u < K; u++)
+      raw[u] = load_raw<16, true>((const typename S::bits*)a.grad + (int64_t)row((uint32_t)u < count ? u : 0) * a.grad_stride + c.at);
   } else {
     #pragma unroll
-    for (int i = 0; i < N; i++) v[i] = acc[i] * a.scale;
+    for (int u = 0; u < K; u++)
+      raw[u] = load_part<sizeof(typename S::bits)>(
+          (const char*)((const typename S::bits*)a.grad + (int64_t)row((uint32_t)u < count ? u : 0) * a.grad_stride),
+          (int64_t)a.width * (int64_t)sizeof(typename S::bits));
   }
-  store_f32<D, N, true>(p, v, left);
+}
+
+template <typename D, int N>
+__device__ inline void write_row(const GradArgs& a, uint32_t row, const Columns<N>& c, float (&acc)[N]) {
+  if (!c.inside) return;
+  typename D::bits* p = (typename D::bits*)a.out + (int64_t)row * a.out_stride + c.at;
+  float v[N];
+  if (c.own == c.at && !c.narrow) {
+    if (a.accumulate) load_f32<D, N>(v, p, N);
+    #pragma unroll
+    for (int i = 0; i < N; i++) v[i] = a.accumulate ? v[i] + acc[i] * a.scale : acc[i] * a.scale;
+    store_f32<D, N, true>(p, v, N);
+  } else {  // the columns that are this lane's alone
+    #pragma unroll
+    for (int i = 0; i < N; i++)
+      if (c.at + i >= c.own && c.at + i < a.width) p[i] = D::from_f32(a.accumulate ? D::to_f32(p[i]) + acc[i] * a.scale : acc[i] * a.scale);
+  }
+}
+
+// a piece of a row that crosses chunks, in the workspace
+template <int N>
+__device__ inline void store_piece(float* piece, const GradArgs& a, const Columns<N>& c, const float (&acc)[N]) {
+  if (c.inside) store_f32<F32, N>((uint32_t*)piece + c.at, acc, c.narrow ? (int64_t)a.width : N);
 }
 
 constexpr int kGradWaves = 4, kGradAhead = 8;
@@ -348,51 +386,44 @@ __global__ __launch_bounds__(kGradWaves* kWave) void etha_embedding_grad_kernel(
   }
   const uint64_t unit = (uint64_t)blockIdx.x * kGradWaves + wave;
   const uint32_t j = (uint32_t)(unit / a.n_cols);
-  const uint64_t col = (unit % a.n_cols * 64 + lane) * N;
   if (j >= a.n_chunks) return;
+  const Columns<N> c((unit % a.n_cols * 64 + lane) * N, a.width);
   const uint64_t begin = (uint64_t)j * a.chunk, end = begin + a.chunk < a.n ? begin + a.chunk : a.n;
   uint32_t cur = a.keys[begin];
   if (cur >= a.n_rows) return;  // other shards' tokens sort behind all rows
   bool open_left = begin && a.keys[begin - 1] == cur;
-  const bool inside = col < a.width;
-  const int64_t left = inside ? (int64_t)(a.width - col) : 0;
   float acc[N] = {};
-  float* part = a.partial + (uint64_t)j * 2 * a.width + col;
+  float* piece = a.partial + (uint64_t)j * 2 * a.width;
   for (uint64_t at = begin; at < end; at += 64) {
     const uint32_t key = at + lane < end ? a.keys[at + lane] : a.n_rows;
     const uint32_t pos = at + lane < end ? a.pos[at + lane] : 0;
-    const int n = __popcll(__ballot(key < a.n_rows));
-    for (int i = 0; i < n; i += kGradAhead) {
-      float v[kGradAhead][N];
+    const uint32_t n = (uint32_t)__popcll(__ballot(key < a.n_rows));
+    for (uint32_t i = 0; i < n; i += kGradAhead) {
+      u32x4 raw[kGradAhead];
+      load_rows<S, N>(raw, a, c, n - i, [&](uint32_t u) { return (uint32_t)__builtin_amdgcn_readlane(pos, i + u); });
       #pragma unroll
-      for (int u = 0; u < kGradAhead; u++) {
-        const uint32_t p = __builtin_amdgcn_readlane(pos, i + u < n ? i + u : i);
-        load_f32<S, N, true>(v[u], (const typename S::bits*)a.grad + (int64_t)p * a.grad_stride + col, i + u < n ? left : 0);
-      }
-      #pragma unroll
-      for (int u = 0; u < kGradAhead; u++) {
+      for (uint32_t u = 0; u < kGradAhead; u++) {
         if (i + u >= n) break;
         const uint32_t k = __builtin_amdgcn_readlane(key, i + u);
         if (k != cur) {
-          if (inside) {
-            if (open_left) store_f32<F32, N>((uint32_t*)part, acc, left);
-            else write_row<D, N>(a, cur, col, acc);
-          }
+          if (open_left) store_piece(piece, a, c, acc);
+          else write_row<D, N>(a, cur, c, acc);
           open_left = false;
           cur = k;
           #pragma unroll
           for (int e = 0; e < N; e++) acc[e] = 0.f;
         }
+        float v[N];
+        raw_to_f32<S>(v, raw[u]);
         #pragma unroll
-        for (int e = 0; e < N; e++) acc[e] += v[u][e];
+        for (int e = 0; e < N; e++) acc[e] += v[e];
       }
     }
     if (n < 64) break;
   }
-  if (!inside) return;
-  if (open_left) store_f32<F32, N>((uint32_t*)part, acc, left);
-  else if (end < a.n && a.keys[end] == cur) store_f32<F32, N>((uint32_t*)(part + a.width), acc, left);
-  else write_row<D, N>(a, cur, col, acc);
+  if (open_left) store_piece(piece, a, c, acc);
+  else if (end < a.n && a.keys[end] == cur) store_piece(piece + a.width, a, c, acc);
+  else write_row<D, N>(a, cur, c, acc);
 }
 
 // Few tokens: no sort and one launch.  A workgroup owns 16 rows and 64 vectors of columns; each wave picks the places of
@@ -414,7 +445,7 @@ __global__ __launch_bounds__(kGradWaves* kWave) void etha_embedding_grad_few_ker
   __shared__ uint16_t s_list[kGradWaves][kFewTokenRows][kFewTokens];
   const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const uint32_t row0 = (blockIdx.x * kGradWaves + wave) * kFewTokenRows;
-  const uint64_t col = ((uint64_t)blockIdx.y * 64 + lane) * N;
+  const Columns<N> c(((uint64_t)blockIdx.y * 64 + lane) * N, a.width);
   uint32_t row[kSteps];
   #pragma unroll
   for (uint32_t i = 0; i < kSteps; i++) row[i] = i * 64 + lane < a.n ? local_row(few.tokens, few.wide, i * 64 + lane, few.first, a.n_rows) : a.n_rows;
@@ -430,25 +461,23 @@ __global__ __launch_bounds__(kGradWaves* kWave) void etha_embedding_grad_few_ker
       count[r] += (uint32_t)__popcll(mask);
     }
   }
-  const int64_t left = col < a.width ? (int64_t)(a.width - col) : 0;
-  if (!left) return;
   #pragma unroll
   for (uint32_t r = 0; r < kFewTokenRows; r++) {
     if (row0 + r >= a.n_rows || (a.accumulate && !count[r])) continue;
     float acc[N] = {};
     for (uint32_t i = 0; i < count[r]; i += kGradAhead) {
-      float v[kGradAhead][N];
+      u32x4 raw[kGradAhead];
+      load_rows<S, N>(raw, a, c, count[r] - i, [&](uint32_t u) { return (uint32_t)s_list[wave][r][i + u]; });
       #pragma unroll
       for (uint32_t u = 0; u < kGradAhead; u++) {
-        const uint32_t p = s_list[wave][r][i + u < count[r] ? i + u : i];
-        load_f32<S, N, true>(v[u], (const typename S::bits*)a.grad + (int64_t)p * a.grad_stride + col, i + u < count[r] ? left : 0);
-      }
-      #pragma unroll
-      for (uint32_t u = 0; u < kGradAhead; u++)
+        if (i + u >= count[r]) break;
+        float v[N];
+        raw_to_f32<S>(v, raw[u]);
         #pragma unroll
-        for (int e = 0; e < N; e++) acc[e] += v[u][e];
+        for (int e = 0; e < N; e++) acc[e] += v[e];
+      }
     }
-    write_row<D, N>(a, row0 + r, col, acc);
+    write_row<D, N>(a, row0 + r, c, acc);
   }
 }
 
@@ -459,37 +488,49 @@ __global__ __launch_bounds__(kGradWaves* kWave) void etha_embedding_join_kernel(
   const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const uint64_t unit = (uint64_t)blockIdx.x * kGradWaves + wave;
   uint32_t j = (uint32_t)(unit / a.n_cols);
-  const uint64_t col = (unit % a.n_cols * 64 + lane) * N;
   if (j >= a.n_chunks) return;
-  const uint64_t begin = (uint64_t)j * a.chunk;
-  uint64_t end = begin + a.chunk;
+  const Columns<N> c((unit % a.n_cols * 64 + lane) * N, a.width);
+  const uint64_t begin = (uint64_t)j * a.chunk, end = begin + a.chunk;
   if (end >= a.n) return;
-  const uint32_t key = a.keys[end];
-  if (key >= a.n_rows || a.keys[end - 1] != key) return;          // nothing goes on behind this chunk
-  if (a.keys[begin] == key && begin && a.keys[begin - 1] == key) return;  // begun earlier
-  const int64_t left = col < a.width ? (int64_t)(a.width - col) : 0;  // all lanes stay: they look for the row's chunks together
+  const uint32_t key = a.keys[end], last = a.keys[end - 1], first = a.keys[begin], before = begin ? a.keys[begin - 1] : a.n_rows;
+  if (key >= a.n_rows || last != key) return;    // nothing goes on behind this chunk
+  if (first == key && before == key) return;     // begun earlier
+  constexpr int kAhead = N > 4 ? 4 : 8;
+  const int64_t left = c.narrow ? (int64_t)a.width : N;
   float acc[N];
-  load_f32<F32, N>(acc, (const uint32_t*)(a.partial + ((uint64_t)j * 2 + 1) * a.width + col), left);
+  load_f32<F32, N>(acc, (const uint32_t*)(a.partial + ((uint64_t)j * 2 + 1) * a.width + c.at), left);
   // the chunks behind this one that begin with the same row, 64 at a time
   for (;;) {
     const uint64_t start = (uint64_t)(j + 1 + lane) * a.chunk;
     const uint64_t same = __ballot(start < a.n && a.keys[start < a.n ? start : 0] == key);
     const uint32_t more = ~same ? __builtin_ctzll(~same) : 64;
-    for (uint32_t i = 0; i < more; i += kGradAhead) {
-      float v[kGradAhead][N];
-      #pragma unroll
-      for (uint32_t u = 0; u < kGradAhead; u++)
-        load_f32<F32, N>(v[u], (const uint32_t*)(a.partial + (uint64_t)(j + 1 + (i + u < more ? i + u : i)) * 2 * a.width + col),
-                         i + u < more ? left : 0);
-      #pragma unroll
-      for (uint32_t u = 0; u < kGradAhead; u++)
+    for (uint32_t i = 0; i < more; i += kAhead) {
+      u32x4 raw[kAhead][N / 4];
+      if (!c.narrow) {
         #pragma unroll
-        for (int e = 0; e < N; e++) acc[e] += v[u][e];
+        for (uint32_t u = 0; u < kAhead; u++)
+          #pragma unroll
+          for (int e = 0; e < N / 4; e++)
+            raw[u][e] = load_raw<16>(a.partial + (uint64_t)(j + 1 + (i + u < more ? i + u : i)) * 2 * a.width + c.at + e * 4);
+      } else {
+        #pragma unroll
+        for (uint32_t u = 0; u < kAhead; u++)
+          #pragma unroll
+          for (int e = 0; e < N / 4; e++)
+            raw[u][e] = load_part<4>((const char*)(a.partial + (uint64_t)(j + 1 + (i + u < more ? i + u : i)) * 2 * a.width + e * 4),
+                                     ((int64_t)a.width - e * 4) * 4);
+      }
+      #pragma unroll
+      for (uint32_t u = 0; u < kAhead; u++) {
+        if (i + u >= more) break;
+        #pragma unroll
+        for (int e = 0; e < N; e++) acc[e] += __builtin_bit_cast(float, (uint32_t)raw[u][e / 4][e % 4]);
+      }
     }
     j += more;
     if (more < 64) break;
   }
-  if (left) write_row<D, N>(a, key, col, acc);
+  write_row<D, N>(a, key, c, acc);
 }
 
 // ---- rows to 8 bits --------------------------------------------------------------------------------------------
@@ -502,28 +543,57 @@ struct QuantArgs {
   int64_t x_stride, values_stride;
 };
 
+// THREADS work-items a row.  The last 8 elements of a row whose width is no multiple of 8 overlap those before, so that no
+// load branches: both come out the same.  (Rows shorter than 8 go by elements.)
 template <typename S, int THREADS, int CHUNKS>
 __global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS) void etha_quantize_rows_kernel(const QuantArgs a) {
-  constexpr int kBlock = THREADS < 256 ? 256 : THREADS, kWaves = THREADS / kWave;
+  constexpr int kBlock = THREADS < 256 ? 256 : THREADS, kWaves = THREADS / kWave, kPieces = 8 * (int)sizeof(typename S::bits) / 16;
+  constexpr int kPer = 8 / kPieces;
   __shared__ uint32_t s_max[kBlock / kWave];
   const uint32_t tid = threadIdx.x % THREADS;
   const uint64_t row = (uint64_t)blockIdx.x * (kBlock / THREADS) + threadIdx.x / THREADS;
   const bool there = row < a.rows;
-  const typename S::bits* x = (const typename S::bits*)a.x + (int64_t)(there ? row : 0) * a.x_stride;
+  const typename S::bits* x = (const typename S::bits*)a.x + (int64_t)(there ? row : a.rows - 1) * a.x_stride;
   int8_t* out = a.values + (int64_t)row * a.values_stride;
-  const int64_t width = there ? (int64_t)a.width : 0;
-  float v[CHUNKS][8];
-  uint32_t top = 0;  // the largest magnitude by its bits: infinity above all numbers, NaN above infinity
-  for (int64_t base = 0; base < width; base += THREADS * CHUNKS * 8) {
+  const int64_t width = (int64_t)a.width, last = width - 8, span = (int64_t)THREADS * CHUNKS * 8;
+  u32x4 raw[CHUNKS][kPieces];
+  const auto load = [&](int64_t base) {
+    if (width >= 8) {
+      #pragma unroll
+      for (int c = 0; c < CHUNKS; c++) {
+        const int64_t at = base + ((int64_t)c * THREADS + tid) * 8;
+        #pragma unroll
+        for (int i = 0; i < kPieces; i++) raw[c][i] = load_raw<16, true>(x + (at < last ? at : last) + i * kPer);
+      }
+    } else {
+      #pragma unroll
+      for (int c = 0; c < CHUNKS; c++)
+        #pragma unroll
+        for (int i = 0; i < kPieces; i++)
+          raw[c][i] = load_part<sizeof(typename S::bits)>((const char*)(x + i * kPer), (width - i * kPer) * (int64_t)sizeof(typename S::bits));
+    }
+  };
+  const auto values = [&](int c, float (&v)[8]) {
+    #pragma unroll
+    for (int i = 0; i < kPieces; i++) {
+      float part[kPer];
+      raw_to_f32<S>(part, raw[c][i]);
+      #pragma unroll
+      for (int e = 0; e < kPer; e++) v[i * kPer + e] = part[e];
+    }
+  };
+  uint32_t top = 0;
+  for (int64_t base = 0; base < width; base += span) {
+    load(base);
     #pragma unroll
     for (int c = 0; c < CHUNKS; c++) {
-      const int64_t at = base + ((int64_t)c * THREADS + tid) * 8;
-      load_f32<S, 8, true>(v[c], x + at, width - at);
-      top = largest_bits(v[c], top);
+      float v[8];
+      values(c, v);
+      top = largest_bits(v, top);
     }
   }
-  top = wave_max(top);
-  if (kWaves > 1) {
+  top = group_max<THREADS < kWave ? THREADS : kWave>(top);
+  if constexpr (kWaves > 1) {
     if ((threadIdx.x & 63) == 0) s_max[threadIdx.x >> 6] = top;
     __syncthreads();
     #pragma unroll
@@ -531,19 +601,20 @@ __global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS) void etha_quantize_r
   }
   if (!there) return;
   const RowScale scale(top);
-  const bool again = width > (int64_t)THREADS * CHUNKS * 8;
-  for (int64_t base = 0; base < width; base += THREADS * CHUNKS * 8) {
+  for (int64_t base = 0; base < width; base += span) {
+    if (width > span) load(base);
     #pragma unroll
     for (int c = 0; c < CHUNKS; c++) {
       const int64_t at = base + ((int64_t)c * THREADS + tid) * 8;
       if (at >= width) continue;
-      if (again) load_f32<S, 8>(v[c], x + at, width - at);
-      const u32x2 packed = scale.pack(v[c]);
-      if (width - at >= 8) {
-        store_raw<8, true>(out + at, packed);
+      float v[8];
+      values(c, v);
+      const u32x2 packed = scale.pack(v);
+      if (width >= 8) {
+        store_raw<8, true>(out + (at < last ? at : last), packed);
       } else {
         for (int i = 0; i < 8; i++)
-          if (i < width - at) out[at + i] = (int8_t)(packed[i >> 2] >> (8 * (i & 3)));
+          if (i < width) out[i] = (int8_t)(packed[i >> 2] >> (8 * (i & 3)));
       }
     }
   }
@@ -583,7 +654,7 @@ GradPlan grad_plan(uint64_t n, uint64_t n_rows, uint64_t width, int es) {
   // chunks of 128 places, shorter while there would be fewer waves than the chip holds a few of per SIMD, longer where the
   // pieces of rows that cross chunks would need more than 2048 places in the workspace
   uint64_t chunk = 128;
-  while (chunk > 8 && (n + chunk - 1) / chunk * p.n_cols < 4096) chunk >>= 1;
+  while (chunk > 32 && (n + chunk - 1) / chunk * p.n_cols < 4096) chunk >>= 1;
   if ((n + chunk - 1) / chunk > 2048 && chunk == 128) chunk = ((n + 2047) / 2048 + 127) / 128 * 128;
   p.chunk = (uint32_t)chunk;
   p.n_chunks = (uint32_t)((n + chunk - 1) / chunk);
@@ -748,9 +819,13 @@ int etha_quantize_rows(const void* x, uint32_t dtype, uint64_t rows, uint64_t wi
   const QuantArgs a = {x, values, scales, rows, width, x_stride, values_stride};
   with_type(dtype, [&](auto s) {
     typedef decltype(s) S;
-    // a wave a row while the row fits its registers, else a workgroup a row, with no more registers than the row needs
+    // a wave (16 lanes for the narrowest) a row while the row fits its registers, else a workgroup a row, with no more registers than the row needs
     // (64128 rows of 4096 in fp32: 222 us with room for 4096, 236 us with room for 8192)
-    if (width <= 64 * 8 * 4)
+    if (width <= 16 * 8 * 4)
+      hipLaunchKernelGGL((etha_quantize_rows_kernel<S, 16, 4>), dim3((uint32_t)((rows + 15) / 16)), dim3(256), 0, (hipStream_t)stream, a);
+    else if (width <= 64 * 8 * 2)
+      hipLaunchKernelGGL((etha_quantize_rows_kernel<S, 64, 2>), dim3((uint32_t)((rows + 3) / 4)), dim3(256), 0, (hipStream_t)stream, a);
+    else if (width <= 64 * 8 * 4)
       hipLaunchKernelGGL((etha_quantize_rows_kernel<S, 64, 4>), dim3((uint32_t)((rows + 3) / 4)), dim3(256), 0, (hipStream_t)stream, a);
     else if (width <= 256 * 8 * 2)
       hipLaunchKernelGGL((etha_quantize_rows_kernel<S, 256, 2>), dim3((uint32_t)rows), dim3(256), 0, (hipStream_t)stream, a);

@@ -126,9 +126,11 @@ def grouped_linear_grad_weight(grad: torch.Tensor, x: torch.Tensor, offsets: tor
     device = check_device(what, x, grad, offsets, out)
     if out is None:
         out = x.new_empty((experts, n, k), dtype=dtype)
-    call(device, "etha_grouped_matmul_reduce", g.data_ptr(), r.data_ptr(), _OPERANDS[x.dtype],
-         x.shape[0], g_stride, r_stride, experts, n, k, offsets.data_ptr(), out.data_ptr(), DTYPE_CODES[out.dtype], out.stride(1),
-         out.stride(0))
+    nbytes = _native.grouped_matmul_reduce_workspace(x.shape[0], experts, n, k)
+    workspace = x.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
+    call(device, "etha_grouped_matmul_reduce", g.data_ptr(), r.data_ptr(), _OPERANDS[x.dtype], x.shape[0], g_stride, r_stride, experts,
+         n, k, offsets.data_ptr(), out.data_ptr(), DTYPE_CODES[out.dtype], out.stride(1), out.stride(0),
+         workspace.data_ptr() if nbytes else None, nbytes)
     return out
 
 

@@ -387,15 +387,18 @@ int etha_int8_linear(const void* x, uint32_t dtype, uint64_t rows, int64_t x_str
  * one (w_transposed): the forward product and the gradient of its rows.  Rows of no expert become zeros with zero_rest
  * and are left as they are without.
  * etha_grouped_matmul_reduce: out[e] = grad[rows of e]^T * x[rows of e], the gradient of the weights, [out_rows, out_cols]
- * for each expert; zeros for an expert without rows.
+ * for each expert; zeros for an expert without rows.  Its workspace (16-byte aligned, at least the bytes that
+ * etha_grouped_matmul_reduce_workspace names, which may be none) may be used again once the launches have finished.
  * Operands are ETHA_BF16 or ETHA_F16.
  */
 int etha_grouped_matmul(const void* x, uint32_t dtype, uint64_t rows, int64_t x_stride, const void* w, uint64_t n_groups,
                         uint64_t cols, uint64_t red, int64_t w_stride, int64_t w_group_stride, int w_transposed,
                         const int32_t* offsets, void* out, uint32_t out_dtype, int64_t out_stride, int zero_rest, void* stream);
+int etha_grouped_matmul_reduce_workspace(uint64_t rows, uint64_t n_groups, uint64_t out_rows, uint64_t out_cols, uint64_t* bytes);
 int etha_grouped_matmul_reduce(const void* grad, const void* x, uint32_t dtype, uint64_t rows, int64_t grad_stride, int64_t x_stride,
                                uint64_t n_groups, uint64_t out_rows, uint64_t out_cols, const int32_t* offsets, void* out,
-                               uint32_t out_dtype, int64_t out_stride, int64_t out_group_stride, void* stream);
+                               uint32_t out_dtype, int64_t out_stride, int64_t out_group_stride, void* workspace,
+                               uint64_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -110,7 +110,10 @@ def test_entry_points_refuse_what_they_cannot_take():
     assert mul(xs=(1 << 22) + 8) == nat.ERR_UNSUPPORTED and mul(ws=-8) == nat.ERR_UNSUPPORTED
     assert mul(m=0) == 0 and mul(n=0) == 0
     red = lambda **k: lib.etha_grouped_matmul_reduce(*{**dict(g=0x1000, x=0x1000, d=nat.F16, m=4, gs=8, xs=8, e=2, n=8, k=8, off=0x1000,
-                                                              o=0x1000, od=nat.F32, os=8, og=64, st=None), **k}.values())
+                                                              o=0x1000, od=nat.F32, os=8, og=64, wk=None, wb=0, st=None), **k}.values())
+    assert red(m=4096) == nat.ERR_INVALID and b"workspace" in lib.etha_last_error()
+    assert red(m=4096, wk=0x1004, wb=1 << 30) == nat.ERR_INVALID and red(m=4096, wk=0x1000, wb=64) == nat.ERR_INVALID
+    assert nat.grouped_matmul_reduce_workspace(4, 2, 8, 8) == 0 and nat.grouped_matmul_reduce_workspace(4096, 2, 8, 8) % (2 * 8 * 8 * 4) == 0
     assert red(d=nat.I8) == nat.ERR_UNSUPPORTED and red(od=nat.F64) == nat.ERR_UNSUPPORTED
     for name in ("g", "x", "off", "o"):
         assert red(**{name: None}) == nat.ERR_INVALID
@@ -132,6 +135,12 @@ CASES = [  # sizes of the groups, out, in, rows before the first and behind the 
     ([257, 600], 256, 512, 0, 0),
     ([40, 70, 10], 768, 1024, 0, 0),
     ([700, 1, 323], 384, 320, 0, 256),
+    ([3000], 130, 72, 2, 1),      # few tiles and many rows: the sum over the rows is cut
+    ([5, 1500, 0, 2600], 33, 47, 0, 9),
+    ([1, 0, 6, 2], 700, 330, 0, 0),  # few rows, a long sum for the gradient of the rows
+    ([16, 17], 1029, 65, 1, 0),
+    ([9], 12, 7, 0, 0),           # rows shorter than 16 bytes
+    ([140, 30], 5, 300, 0, 3),
 ]
 
 
