@@ -976,19 +976,24 @@ int launch_few(const char* what, const FewArgs& few, void* stream) {
 }
 
 // What a choice of tiles costs, in microseconds, by what bounded the shapes where they were measured: a workgroup takes in
-// its operands at about 45 GB/s, all of them together at about 11 TB/s, and the matrices come from memory at `gbs`.  A rule
-// on sizes alone; the rows of a group are taken as even, half a tile a group as lost.
-double tile_cost(const MatmulArgs& a, uint32_t kind, int es, int bm, int bn, int resident, double gbs) {
+// its operands at about 45 GB/s and needs `fixed` to begin and to write its results, all of them together take in `tbs`, and
+// the matrices come from memory at `gbs`.  A rule on sizes alone; the rows of a group are taken as even, half a tile a group
+// as lost.
+struct TileCost {
+  int bm, bn, resident;
+  double fixed, tbs, gbs;
+};
+double tile_cost(const MatmulArgs& a, uint32_t kind, int es, const TileCost& t) {
   const double k_bytes = (double)a.red * es;
   const double groups = kind == kPlain ? 1 : a.n_groups < a.rows ? (a.n_groups ? a.n_groups : 1) : a.rows;
-  const double high = a.rows / groups < bm ? a.rows / groups : bm;  // rows of a tile that there are
-  double row_tiles = kind == kPlain ? (double)((a.rows + bm - 1) / bm) : a.rows / (double)bm + groups / 2;
+  const double high = a.rows / groups < t.bm ? a.rows / groups : t.bm;  // rows of a tile that there are
+  double row_tiles = kind == kPlain ? (double)((a.rows + t.bm - 1) / t.bm) : a.rows / (double)t.bm + groups / 2;
   if (row_tiles < groups) row_tiles = groups;
-  const double tiles = row_tiles * ((a.cols + bn - 1) / bn), bytes = (high + bn) * k_bytes;
-  const double rounds = (double)(uint64_t)((tiles + resident - 1) / resident);
-  double us = rounds * bytes / 45e3;
-  if (tiles * bytes / 11e6 > us) us = tiles * bytes / 11e6;
-  if (groups * a.cols * k_bytes / gbs / 1e3 > us) us = groups * a.cols * k_bytes / gbs / 1e3;
+  const double tiles = row_tiles * ((a.cols + t.bn - 1) / t.bn), bytes = (high + t.bn) * k_bytes;
+  const double rounds = (double)(uint64_t)((tiles + t.resident - 1) / t.resident);
+  double us = rounds * (bytes / 45e3 + t.fixed);
+  if (tiles * bytes / t.tbs / 1e6 + t.fixed > us) us = tiles * bytes / t.tbs / 1e6 + t.fixed;
+  if (groups * a.cols * k_bytes / t.gbs / 1e3 > us) us = groups * a.cols * k_bytes / t.gbs / 1e3;
   return us;
 }
 
@@ -1003,21 +1008,26 @@ int shaped_matmul(const char* what, const MatmulArgs& a, bool direct, void* stre
     return launched("etha_matmul_short_kernel");
   }
   if constexpr (KIND == kGroupReduce) {
-    // the tall reduction pays for the large tile from about a stage or two of rows on, if there are tiles for every CU
+    // the large tile wherever there are enough of them for every CU, also for few rows, where all there is to do is writing
+    // the results (16 rows, 8 x [3584, 4096]: 53 us, 63 us with the middle one)
     const uint64_t tiles = row_tiles_of(a, KIND, ShapeL::BM) * (((uint64_t)a.cols + ShapeL::BN - 1) / ShapeL::BN);
-    if (a.splits < 2 && tiles >= 192 && a.red / a.n_groups >= 96) return launch_shape<E, KIND, D, ShapeL>(what, a, direct, stream);
+    if (a.splits < 2 && tiles >= 192) return launch_shape<E, KIND, D, ShapeL>(what, a, direct, stream);
     return launch_shape<E, KIND, D, ShapeM>(what, a, direct, stream);
   } else {
     double cost[6];
     const double none = 1e30;
     constexpr bool few = KIND != kGroupRowsT;
-    cost[0] = tile_cost(a, KIND, E::kEs, 16, few ? kFewCols : kFewColsT, 512, 6000);
+    const TileCost shapes[6] = {
+        few ? TileCost{16, kFewCols, 512, 2, 11, 6000} : TileCost{16, kFewColsT, 512, 2, 7, 6000},
+        {32, kFewCols, 512, 2, 11, 6000},
+        {64, kFewCols, 256, 2, 11, 6000},
+        {ShapeS::BM, ShapeS::BN, 512, 3, 11, 4600},
+        {ShapeM::BM, ShapeM::BN, 512, 4, 11, 5200},
+        {ShapeL::BM, ShapeL::BN, 256, 8, 11, 4600},
+    };
+    for (int i = 0; i < 6; i++) cost[i] = tile_cost(a, KIND, E::kEs, shapes[i]);
+    if (!few) cost[1] = cost[2] = none;
     if (!few && (p_row < 16 || q_row < 16)) cost[0] = none;  // its loads begin 16 bytes before the end of a row
-    cost[1] = few ? tile_cost(a, KIND, E::kEs, 32, kFewCols, 512, 6000) : none;
-    cost[2] = few ? tile_cost(a, KIND, E::kEs, 64, kFewCols, 256, 6000) : none;
-    cost[3] = tile_cost(a, KIND, E::kEs, ShapeS::BM, ShapeS::BN, 512, 4600);
-    cost[4] = tile_cost(a, KIND, E::kEs, ShapeM::BM, ShapeM::BN, 512, 5200);
-    cost[5] = tile_cost(a, KIND, E::kEs, ShapeL::BM, ShapeL::BN, 256, 4600);
     int best = 0;
     for (int i = 1; i < 6; i++)
       if (cost[i] < cost[best]) best = i;
@@ -1068,13 +1078,13 @@ bool is_few(uint64_t rows, uint64_t cols, uint64_t width) {
 uint64_t padded_width(uint64_t width) { return (width + 15) / 16 * 16; }
 
 // Parts that the sum over a group's rows is cut into where its tiles are too few for the chip: about two workgroups a CU,
-// each with at least four stages of an even group's rows.
+// each with at least two stages of an even group's rows (groups are uneven, the longest one is what is waited for).
 uint32_t reduce_splits(uint64_t rows, uint64_t n_groups, uint64_t out_rows, uint64_t out_cols) {
   if (!n_groups || !out_rows || !out_cols) return 1;
   const uint64_t tiles = n_groups * ((out_rows + ShapeM::BM - 1) / ShapeM::BM) * ((out_cols + ShapeM::BN - 1) / ShapeM::BN);
   const uint64_t stages = rows / n_groups / 64;
-  if (tiles > 192 || stages < 8 || out_rows * 2 < 16 || out_cols * 2 < 16) return 1;
-  const uint64_t by_tiles = (512 + tiles - 1) / tiles, by_stages = stages / 4;
+  if (tiles > 192 || stages < 4 || out_rows * 2 < 16 || out_cols * 2 < 16) return 1;
+  const uint64_t by_tiles = (512 + tiles - 1) / tiles, by_stages = stages / 2;
   const uint64_t splits = by_tiles < by_stages ? by_tiles : by_stages;
   return (uint32_t)(splits < 64 ? splits : 64);
 }
