@@ -31,7 +31,7 @@ def quantize_rows(x: torch.Tensor, *, values: torch.Tensor | None = None,
     if values is not None:
         values_stride = check_out("quantize_rows", values, x.shape, (torch.int8,), x, scales)
     if scales is not None:
-        check_out("quantize_rows", scales, x.shape[:-1], (torch.float32,), x)
+        check_out("quantize_rows", scales.unsqueeze(-1), (*x.shape[:-1], 1), (torch.float32,), x)
         if not scales.is_contiguous():
             raise ValueError("quantize_rows: scales have to be contiguous")
     device = check_device("quantize_rows", x, values, scales)

@@ -86,7 +86,7 @@ def test_entry_points_refuse_what_they_cannot_take():
     rows = lambda **k: lib.etha_quantize_rows(*{**dict(x=0x1000, d=nat.F32, r=4, w=4, xs=4, v=0x1000, vs=4, s=0x1000, st=None), **k}.values())
     assert rows(d=nat.I8) == nat.ERR_UNSUPPORTED
     assert rows(x=None) == nat.ERR_INVALID and rows(v=None) == nat.ERR_INVALID and rows(s=None) == nat.ERR_INVALID
-    assert rows(r=(1 << 22) + 1) == nat.ERR_UNSUPPORTED
+    assert rows(r=1 << 31) == nat.ERR_UNSUPPORTED
     assert rows(r=0) == 0
     mul = lambda **k: lib.etha_int8_matmul(*{**dict(x=0x1000, xs=0x1000, m=4, xp=16, w=0x1000, ws=0x1000, n=4, wp=16, k=16, b=None, o=0x1000,
                                                     od=nat.BF16, op=4, st=None), **k}.values())
@@ -116,6 +116,23 @@ def test_rows(gpu_device, rows, width, dtype):
     gen = torch.Generator(device=gpu_device).manual_seed(rows * width)
     x = (torch.randn(rows, width, generator=gen, device=gpu_device) * 3).to(dtype)
     check_rows(x, *quantize_rows(x))
+
+
+@pytest.mark.gpu
+def test_more_rows_than_a_launch_takes(gpu_device):
+    x = torch.randn((1 << 21) + 5, 9, dtype=torch.bfloat16, device=gpu_device)[:, :8]  # 18 bytes between rows
+    values, scales = quantize_rows(x)
+    for part in (slice(0, 4), slice((1 << 21) - 4, None)):
+        check_rows(x[part], values[part], scales[part])
+
+
+@pytest.mark.gpu
+def test_one_row_into_a_given_scale(gpu_device):
+    x = torch.randn(77, device=gpu_device)
+    scale = torch.empty((), device=gpu_device)
+    values, got = quantize_rows(x, scales=scale)
+    assert got is scale
+    check_rows(x[None], values[None], got[None])
 
 
 @pytest.mark.gpu
