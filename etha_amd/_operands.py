@@ -57,8 +57,7 @@ def readable_rows(t: torch.Tensor, most: int | None = None) -> tuple[torch.Tenso
     distance in elements."""
     stride = row_stride(t)
     if stride is None or (most is not None and stride * t.element_size() > most):
-        t = t.contiguous()
-        stride = row_stride(t)
+        return t.contiguous(), t.shape[-1]  # a single row counts as contiguous, whatever its stride says
     return t, stride
 
 

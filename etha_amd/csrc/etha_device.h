@@ -201,6 +201,4 @@ inline void with_type(uint32_t dtype, F&& f) {
   else f(etha_device::F16{});
 }
 
-
-
 #endif  // ETHA_DEVICE_H

@@ -961,7 +961,6 @@ int launch_matmul(const char* what, const MatmulArgs& a, void* stream) {
   return launched("etha_matmul_kernel");
 }
 
-
 template <typename E, uint32_t KIND, typename D, typename S>
 int launch_shape(const char* what, const MatmulArgs& a, bool direct, void* stream) {
   return direct ? launch_matmul<E, KIND, D, S, DirectStage>(what, a, stream) : launch_matmul<E, KIND, D, S, RegisterStage>(what, a, stream);

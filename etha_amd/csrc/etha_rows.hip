@@ -331,7 +331,7 @@ __device__ inline void load_rows(u32x4 (&raw)[K], const GradArgs& a, const Colum
 }
 
 // Stored through the caches, unlike the rows of zeros: a wave here writes 1 KB of one row, its neighbours the rest at other
-// times, and the lines are put together in L2 (16381 tokens of 4096 into 128256 rows 321 us, 343 us around the caches; 4 tokens
+// times, and the lines are put together in L2 (65536 tokens of 4096 into 128256 rows 321 us, 343 us around the caches; 4 tokens
 // into 20480 x 2809 fp32 34 us, 70 us).
 template <typename D, int N>
 __device__ inline void write_row(const GradArgs& a, uint32_t row, const Columns<N>& c, float (&acc)[N]) {
@@ -642,6 +642,12 @@ int check_tokens(const char* what, const void* tokens, uint32_t token_dtype, uin
   return ETHA_OK;
 }
 
+// Of a gradient, whose sort has every workgroup add up the counts of all others: here they are some hundred gigabytes of L2.
+int check_gradient_tokens(const char* what, uint64_t n_tokens) {
+  if (n_tokens > 1ull << 26) return fail(ETHA_ERR_UNSUPPORTED, "%s: %llu tokens; at most 2^26", what, (unsigned long long)n_tokens);
+  return ETHA_OK;
+}
+
 // Column blocks, chunk length and workspace of a gradient call: a rule on sizes alone.
 struct GradPlan {
   uint32_t n_cols, chunk, n_chunks;
@@ -725,7 +731,8 @@ int etha_embedding(const void* tokens, uint32_t token_dtype, uint64_t n_tokens, 
 }
 
 int etha_embedding_grad_workspace(uint64_t n_tokens, uint64_t n_rows, uint64_t width, uint32_t grad_dtype, uint64_t* bytes) {
-  const int rc = check_tokens("etha_embedding_grad_workspace", &n_tokens, ETHA_I32, n_tokens, n_rows, width);
+  int rc = check_tokens("etha_embedding_grad_workspace", &n_tokens, ETHA_I32, n_tokens, n_rows, width);
+  if (rc == ETHA_OK) rc = check_gradient_tokens("etha_embedding_grad_workspace", n_tokens);
   if (rc != ETHA_OK) return rc;
   if (!bytes) return fail(ETHA_ERR_INVALID, "etha_embedding_grad_workspace: null result");
   if (!es_of(grad_dtype)) return fail(ETHA_ERR_UNSUPPORTED, "etha_embedding_grad_workspace: element types are f32, bf16 and f16");
@@ -738,6 +745,7 @@ int etha_embedding_grad(const void* grad, uint32_t grad_dtype, int64_t grad_stri
                         uint32_t out_dtype, int64_t out_stride, int accumulate, void* workspace, uint64_t workspace_bytes,
                         void* stream) {
   int rc = check_tokens("etha_embedding_grad", tokens, token_dtype, n_tokens, n_rows, width);
+  if (rc == ETHA_OK) rc = check_gradient_tokens("etha_embedding_grad", n_tokens);
   if (rc != ETHA_OK) return rc;
   const int es = es_of(grad_dtype);
   if (!es || !es_of(out_dtype)) return fail(ETHA_ERR_UNSUPPORTED, "etha_embedding_grad: element types are f32, bf16 and f16");

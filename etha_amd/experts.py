@@ -41,7 +41,7 @@ def _matrices(what: str, weight: torch.Tensor) -> tuple[torch.Tensor, int, int]:
     if weight.stride(2) != 1 and weight.shape[2] > 1:
         raise ValueError(f"{what}: the rows of weight have to be contiguous")
     if weight.stride(1) * 2 > MOST_STRIDE:
-        weight = weight.contiguous()
+        return weight.contiguous(), weight.shape[2], weight.shape[1] * weight.shape[2]
     return weight, weight.stride(1), weight.stride(0)
 
 

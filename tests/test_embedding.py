@@ -107,10 +107,14 @@ def test_entry_points_refuse_what_they_cannot_take():
     assert grad(ws=0x1004) == nat.ERR_INVALID
     assert grad(g=None) == nat.ERR_INVALID
     assert grad(r=0) == 0 and grad(n=0, a=1) == 0
+    assert grad(n=(1 << 26) + 1) == nat.ERR_UNSUPPORTED
     need = nat.embedding_grad_workspace
     assert need(0, 8, 4, nat.F32) == 0 and need(4000, 8, 4, nat.F32) > 0
     with pytest.raises(nat.EthaNativeError):
         need(1, 8, 4, nat.I32)
+    assert need(1 << 26, 8, 4, nat.F32) > 0
+    with pytest.raises(nat.EthaNativeError):
+        need((1 << 26) + 1, 8, 4, nat.F32)
 
 
 # ---- lookup ---------------------------------------------------------------------------------------------------------
@@ -286,6 +290,43 @@ def test_capture_and_streams(gpu_device):
         eager_rows, eager_total = embedding(ids, weight, scale=2.0), embedding_grad(grad, ids, 300)
         torch.cuda.synchronize()
         assert torch.equal(rows, eager_rows) and torch.equal(total, eager_total)
+
+
+@pytest.mark.gpu
+def test_two_graphs_replayed_in_turn(gpu_device):
+    """Each graph has a workspace of its own, also where they share a pool."""
+    ids = [torch.randint(0, 40, (n,), device=gpu_device) for n in (9000, 12000)]
+    grad = [torch.randn(i.numel(), 72, device=gpu_device) for i in ids]
+    graphs, totals, pool = [], [], None
+    for i, g in zip(ids, grad):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, pool=pool):
+            totals.append(embedding_grad(g, i, 40))
+        pool = pool or graph.pool()
+        graphs.append(graph)
+    for order in ((0, 1), (1, 0), (0, 0, 1)):
+        for k in order:
+            ids[k].copy_(torch.randint(0, 40, ids[k].shape, device=gpu_device))
+            graphs[k].replay()
+            eager = embedding_grad(grad[k], ids[k], 40)
+            torch.cuda.synchronize()
+            assert torch.equal(totals[k], eager)
+
+
+@pytest.mark.gpu
+def test_two_streams_at_once(gpu_device):
+    ids = torch.randint(0, 500, (2, 30000), device=gpu_device)
+    grad = torch.randn(2, 30000, 136, device=gpu_device)
+    want = [embedding_grad(g, i, 500) for g, i in zip(grad, ids)]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(5):
+        for k, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                got[k].append(embedding_grad(grad[k], ids[k], 500))
+    torch.cuda.synchronize()
+    assert all(torch.equal(g, want[k]) for k in (0, 1) for g in got[k])
 
 
 @pytest.mark.gpu

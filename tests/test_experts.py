@@ -235,6 +235,17 @@ def test_rows_far_apart(gpu_device):
 
 
 @pytest.mark.gpu
+def test_a_single_row_whatever_its_stride(gpu_device):
+    gen = torch.Generator(device=gpu_device).manual_seed(16)
+    x, weight, offsets, grad = case(gen, [0, 1], 1, 96, torch.bfloat16, gpu_device)
+    far = torch.as_strided(x, x.shape, (1 << 30, 1))
+    check_rows(grouped_linear(far, weight, offsets), x, weight, offsets)
+    check_weight(grouped_linear_grad_weight(grad, far, offsets), grad, x, offsets)
+    matrices = torch.as_strided(weight, weight.shape, (96, 1 << 30, 1))  # one row each
+    check_rows(grouped_linear(x, matrices, offsets), x, weight, offsets)
+
+
+@pytest.mark.gpu
 def test_nan_stays_in_its_group(gpu_device):
     gen = torch.Generator(device=gpu_device).manual_seed(6)
     for sizes in ([3, 5, 2], [130, 70, 40]):

@@ -216,6 +216,14 @@ def test_product_at_the_end_of_32_bits(gpu_device):
 
 
 @pytest.mark.gpu
+def test_a_single_row_whatever_its_stride(gpu_device):
+    gen = torch.Generator(device=gpu_device).manual_seed(10)
+    x, xs, w, ws = operands(gen, 1, 1, 200, gpu_device)
+    far = lambda t: torch.as_strided(t, t.shape, (1 << 30, 1))
+    check_product(int8_matmul(far(x), xs, far(w), ws), x, xs, w, ws, None)
+
+
+@pytest.mark.gpu
 def test_product_of_views(gpu_device):
     gen = torch.Generator(device=gpu_device).manual_seed(9)
     for m in (3, 70, 300):
