@@ -63,6 +63,9 @@ def readable_rows(t: torch.Tensor, most: int | None = None) -> tuple[torch.Tenso
 
 def _byte_range(t: torch.Tensor) -> tuple[int, int]:
     """First byte and the byte behind the last that the elements of ``t`` lie in."""
+    if t.is_contiguous():
+        at = t.data_ptr()
+        return at, at + t.numel() * t.element_size()
     lo = hi = 0
     for size, step in zip(t.shape, t.stride()):
         lo += min(0, (size - 1) * step)
@@ -73,16 +76,19 @@ def _byte_range(t: torch.Tensor) -> tuple[int, int]:
 
 def check_out(what: str, out: torch.Tensor, shape, dtypes, *inputs: torch.Tensor | None) -> int:
     """Checks an output that the caller passes; returns its row stride."""
-    if tuple(out.shape) != tuple(shape):
+    if out.shape != shape:
         raise ValueError(f"{what}: out has shape {tuple(out.shape)}, not {tuple(shape)}")
     if out.dtype not in dtypes:
         raise ValueError(f"{what}: out is {out.dtype}")
     if out.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{what}: out requires a gradient")
-    stride = row_stride(out)
-    rows = out.numel() // out.shape[-1] if out.dim() and out.shape[-1] else 0
-    if stride is None or (rows > 1 and stride < out.shape[-1]):
-        raise ValueError(f"{what}: the rows of out have to be contiguous, apart and at one distance")
+    if out.dim() and out.is_contiguous():
+        stride = shape[-1]
+    else:
+        stride = row_stride(out)
+        rows = out.numel() // out.shape[-1] if out.dim() and out.shape[-1] else 0
+        if stride is None or (rows > 1 and stride < out.shape[-1]):
+            raise ValueError(f"{what}: the rows of out have to be contiguous, apart and at one distance")
     if out.numel():
         lo, hi = _byte_range(out)
         for t in inputs:
