@@ -73,38 +73,20 @@ __global__ __launch_bounds__(256) void etha_embedding_kernel(const LookupArgs a)
 }
 
 // ---- sorting tokens by row ---------------------------------------------------------------------------------------
-// A stable radix sort of (row, position), digits of up to 9 bits, so that a row's positions come in their own order
-// and the sums that follow do not depend on timing.  A wave ranks 64 keys at a time: the lanes with the same digit
-// find each other with one ballot per digit bit, and the wave's running count of the digit lies in LDS.
-constexpr int kMaxBins = 512;
-constexpr uint32_t kOneBlockThreads = 1024, kOneBlockTokens = 8192;
-constexpr uint32_t kSortThreads = 256;
-// Tokens of a workgroup where there are more: every workgroup adds up the counts of all of them, so they get longer where
-// there would be more than 256 (65536 tokens: a pass takes 11 us with 64 workgroups, 29 us with 16).
-constexpr uint32_t sort_tokens(uint64_t n) { return n <= 256 * 1024 ? 1024 : 4096; }
+// Tokens row by row, a row's positions in their own order, so that the sums that follow do not depend on timing.  One launch:
+// a workgroup owns every 2^groups_log2-th row (frequent tokens lie close together) and looks through all tokens, a wave
+// through a run of them.  It counts those of each of its rows, wave by wave, and those of the workgroups before it, which
+// says where its own begin, and notes which they are; then every wave puts its tokens where the counts say.  Lanes whose
+// tokens have the same row find each other with one ballot per bit.  What bounds it is the looking, some 10 instructions for
+// 64 tokens: 57984 tokens of 21716 rows 20 us, 6965 of 6676 rows 7 us (a radix sort of two passes, with four launches, took
+// 29 us and the gaps between them; one in a single workgroup 17 us for the latter; runs of rows instead of every 256th, with
+// the tokens looked through twice, 57 us for the former).
+constexpr uint32_t kSortThreads = 1024, kSortWaves = kSortThreads / kWave, kSortNoted = 1024;
+constexpr int kSortBinsLog2 = 10;
+constexpr int kSortGroupsLog2 = 8;
 
-__device__ inline uint64_t same_digit(uint32_t digit, int bits) {
-  uint64_t mask = ~0ull;
-  for (int b = 0; b < bits; b++) {
-    const uint64_t ones = __ballot((digit >> b) & 1);
-    mask &= (digit >> b) & 1 ? ones : ~ones;
-  }
-  return mask;
-}
-
-// Rank of this lane's key among the wave's earlier keys of the same digit; `counts` (the wave's own, in LDS) goes on.
-__device__ inline uint32_t rank_in_wave(volatile uint16_t* counts, uint32_t digit, int bits) {
-  const uint32_t lane = threadIdx.x & 63;
-  const uint64_t mask = same_digit(digit, bits);
-  const uint32_t before = counts[digit];
-  __builtin_amdgcn_wave_barrier();
-  if ((mask >> lane) == 1) counts[digit] = (uint16_t)(before + __popcll(mask));  // the highest lane of the digit
-  __builtin_amdgcn_wave_barrier();
-  return before + __popcll(mask & ((1ull << lane) - 1));
-}
-
-// Exclusive sum over the workgroup's work-items; `sums` holds one word per wave.
-__device__ inline uint32_t scan_block(uint32_t v, uint32_t* sums) {
+// Exclusive sum over the workgroup's work-items and the sum of all; `sums` holds one word per wave.
+__device__ inline uint32_t scan_block(uint32_t v, uint32_t* sums, uint32_t* all) {
   const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   uint32_t inc = v;
   #pragma unroll
@@ -114,170 +96,108 @@ __device__ inline uint32_t scan_block(uint32_t v, uint32_t* sums) {
   }
   if (lane == 63) sums[wave] = inc;
   __syncthreads();
-  uint32_t base = 0;
-  for (uint32_t w = 0; w < wave; w++) base += sums[w];
+  uint32_t base = 0, total = 0;
+  #pragma unroll
+  for (uint32_t w = 0; w < kSortWaves; w++) {
+    base += w < wave ? sums[w] : 0;
+    total += sums[w];
+  }
   __syncthreads();
+  *all = total;
   return base + inc - v;
 }
 
-// Up to kOneBlockTokens tokens: all passes in one workgroup.
-__global__ __launch_bounds__(kOneBlockThreads) void etha_sort_tokens_kernel(const void* tokens, uint32_t wide, uint32_t n, int64_t first,
-                                                                          uint32_t n_rows, int passes, int bits, uint32_t* keys_out,
-                                                                          uint32_t* pos_out) {
-  constexpr uint32_t kWaves = kOneBlockThreads / kWave, kItems = kOneBlockTokens / kOneBlockThreads;
-  __shared__ uint32_t s_key[kOneBlockTokens];
-  __shared__ uint16_t s_pos[kOneBlockTokens];
-  __shared__ uint16_t s_count[kWaves][kMaxBins];
-  __shared__ uint32_t s_base[kMaxBins];
-  __shared__ uint32_t s_sums[kWaves];
-  const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const uint32_t items = (n + kOneBlockThreads - 1) / kOneBlockThreads;  // per work-item, at most kItems
-  const uint32_t at0 = wave * items * 64 + lane;
-  uint32_t key[kItems], pos[kItems];
-  #pragma unroll
-  for (uint32_t i = 0; i < kItems; i++) {
-    const uint32_t p = at0 + i * 64;
-    pos[i] = p;
-    key[i] = 0xffffffffu;  // behind the last token: sorts behind everything
-    if (i < items && p < n) key[i] = local_row(tokens, wide, p, first, n_rows);
-  }
-  const uint32_t bins = 1u << bits;
-  for (int pass = 0; pass < passes; pass++) {
-    const int shift = pass * bits;
-    for (uint32_t i = tid; i < kWaves * kMaxBins; i += kOneBlockThreads) (&s_count[0][0])[i] = 0;
-    __syncthreads();
-    uint32_t rank[kItems];
-    #pragma unroll
-    for (uint32_t i = 0; i < kItems; i++)
-      if (i < items) rank[i] = rank_in_wave(s_count[wave], (key[i] >> shift) & (bins - 1), bits);
-    __syncthreads();
-    uint32_t total = 0;
-    if (tid < bins)
-      for (uint32_t w = 0; w < kWaves; w++) {
-        const uint32_t c = s_count[w][tid];
-        s_count[w][tid] = (uint16_t)total;
-        total += c;
-      }
-    const uint32_t base = scan_block(total, s_sums);
-    if (tid < bins) s_base[tid] = base;
-    __syncthreads();
-    #pragma unroll
-    for (uint32_t i = 0; i < kItems; i++)
-      if (i < items) {
-        const uint32_t digit = (key[i] >> shift) & (bins - 1);
-        const uint32_t to = s_base[digit] + s_count[wave][digit] + rank[i];
-        s_key[to] = key[i];
-        s_pos[to] = (uint16_t)pos[i];
-      }
-    __syncthreads();
-    #pragma unroll
-    for (uint32_t i = 0; i < kItems; i++)
-      if (i < items) {
-        key[i] = s_key[at0 + i * 64];
-        pos[i] = s_pos[at0 + i * 64];
-      }
-    __syncthreads();
-  }
-  #pragma unroll
-  for (uint32_t i = 0; i < kItems; i++) {
-    const uint32_t p = at0 + i * 64;
-    if (i < items && p < n) {
-      keys_out[p] = key[i];
-      pos_out[p] = pos[i];
-    }
-  }
-}
-
 struct SortArgs {
-  const void* tokens;     // first pass: keys come from the tokens, positions are the places themselves
-  const uint32_t* keys_in;
-  const uint32_t* pos_in;
-  uint32_t* keys_out;
-  uint32_t* pos_out;
-  uint32_t* hist;         // [block][bin]
-  uint64_t n;
+  const void* tokens;
+  uint32_t* keys;  // tokens of other shards come last, as row n_rows and without a position
+  uint32_t* pos;
+  uint32_t* used;  // tokens of each row
+  uint32_t n, n_rows;
   int64_t first;
-  uint32_t n_rows, wide;
-  int shift, bits;
+  int groups_log2, bins_log2;  // workgroups, rows of one
 };
 
-__device__ inline uint32_t sort_key(const SortArgs& a, uint64_t p) {
-  if (p >= a.n) return 0xffffffffu;
-  return a.keys_in ? a.keys_in[p] : local_row(a.tokens, a.wide, p, a.first, a.n_rows);
-}
-
-template <uint32_t TOKENS>
-__global__ __launch_bounds__(kSortThreads) void etha_sort_count_kernel(const SortArgs a) {
-  __shared__ uint32_t s_count[kMaxBins];
-  const uint32_t bins = 1u << a.bits;
-  for (uint32_t i = threadIdx.x; i < bins; i += kSortThreads) s_count[i] = 0;
+template <typename T>
+__global__ __launch_bounds__(kSortThreads) void etha_sort_tokens_kernel(const SortArgs a) {
+  constexpr uint32_t kAhead = 8;
+  __shared__ uint32_t s_count[kSortWaves << kSortBinsLog2];  // [wave][row]
+  __shared__ uint32_t s_noted[kSortWaves][kSortNoted];
+  __shared__ uint32_t s_sums[kSortWaves];
+  const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), bins = 1u << a.bins_log2;
+  const uint32_t group = blockIdx.x, groups = 1u << a.groups_log2;
+  const T* tokens = (const T*)a.tokens;
+  for (uint32_t i = tid; i < kSortWaves << a.bins_log2; i += kSortThreads) s_count[i] = 0;
   __syncthreads();
-  const uint64_t base = (uint64_t)blockIdx.x * TOKENS;
-  for (uint32_t i = threadIdx.x; i < TOKENS; i += kSortThreads)
-    if (base + i < a.n) atomicAdd(&s_count[(sort_key(a, base + i) >> a.shift) & (bins - 1)], 1u);
-  __syncthreads();
-  for (uint32_t i = threadIdx.x; i < bins; i += kSortThreads) a.hist[(uint64_t)blockIdx.x * bins + i] = s_count[i];
-}
-
-template <uint32_t TOKENS>
-__global__ __launch_bounds__(kSortThreads) void etha_sort_scatter_kernel(const SortArgs a) {
-  constexpr uint32_t kWaves = kSortThreads / kWave, kItems = TOKENS / kSortThreads;
-  constexpr uint32_t kBinsPer = kMaxBins / kSortThreads;
-  __shared__ uint16_t s_count[kWaves][kMaxBins];
-  __shared__ uint32_t s_base[kMaxBins];
-  __shared__ uint32_t s_sums[kWaves];
-  const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, bins = 1u << a.bits;
-  for (uint32_t i = tid; i < kWaves * kMaxBins; i += kSortThreads) (&s_count[0][0])[i] = 0;
-  // where this block's keys of each bin begin: all keys of lower bins, then the earlier blocks' of this bin
-  uint32_t before[kBinsPer], total[kBinsPer], sum = 0;
-  #pragma unroll
-  for (uint32_t j = 0; j < kBinsPer; j++) {
-    const uint32_t bin = tid * kBinsPer + j;
-    before[j] = total[j] = 0;
-    if (bin < bins) {
-      #pragma unroll 8
-      for (uint32_t b = 0; b < gridDim.x; b++) {
-        const uint32_t c = a.hist[(uint64_t)b * bins + bin];
-        before[j] += b < blockIdx.x ? c : 0;
-        total[j] += c;
-      }
+  uint32_t* count = s_count + (wave << a.bins_log2);
+  uint32_t* noted = s_noted[wave];
+  const uint32_t per = (a.n + kSortThreads - 1) / kSortThreads * kWave, lo = wave * per < a.n ? wave * per : a.n;
+  const uint32_t hi = a.n - lo < per ? a.n : lo + per;
+  // a row, or something from n_rows on; unsigned: an id far below `first` must not wrap into the shard
+  const auto row_of = [&](T id) {
+    const uint64_t r = (uint64_t)(int64_t)id - (uint64_t)a.first;
+    return (int64_t)id >= a.first && r < a.n_rows ? (uint32_t)r : a.n_rows;
+  };
+  uint32_t lower = 0, n_noted = 0;
+  const auto look = [&](T id, bool there, uint32_t p) {
+    const uint32_t row = row_of(id), of = row & (groups - 1);
+    const bool inside = there && row < a.n_rows, mine = inside && of == group;
+    lower += (uint32_t)__popcll(__ballot(inside && of < group));
+    const uint64_t mask = __ballot(mine);
+    if (!mask) return;
+    if (mine) {
+      atomicAdd(&count[row >> a.groups_log2], 1u);
+      const uint32_t at = n_noted + (uint32_t)__popcll(mask & ((1ull << lane) - 1));
+      if (at < kSortNoted) noted[at] = p;
     }
-    sum += total[j];
+    n_noted += (uint32_t)__popcll(mask);
+  };
+  uint32_t at = lo;
+  for (; at + kAhead * kWave <= hi; at += kAhead * kWave) {
+    T id[kAhead];
+    #pragma unroll
+    for (uint32_t u = 0; u < kAhead; u++) id[u] = tokens[at + u * kWave + lane];
+    #pragma unroll
+    for (uint32_t u = 0; u < kAhead; u++) look(id[u], true, at + u * kWave + lane);
   }
-  uint32_t base = scan_block(sum, s_sums);
-  #pragma unroll
-  for (uint32_t j = 0; j < kBinsPer; j++) {
-    const uint32_t bin = tid * kBinsPer + j;
-    if (bin < bins) s_base[bin] = base + before[j];
-    base += total[j];
-  }
-  __syncthreads();
-  const uint64_t at0 = (uint64_t)blockIdx.x * TOKENS + wave * (kItems * 64) + lane;
-  uint32_t key[kItems], rank[kItems];
-  #pragma unroll
-  for (uint32_t i = 0; i < kItems; i++) key[i] = sort_key(a, at0 + i * 64);
-  #pragma unroll
-  for (uint32_t i = 0; i < kItems; i++) rank[i] = rank_in_wave(s_count[wave], (key[i] >> a.shift) & (bins - 1), a.bits);
-  __syncthreads();
-  for (uint32_t bin = tid; bin < bins; bin += kSortThreads) {
-    uint32_t sofar = 0;
-    for (uint32_t w = 0; w < kWaves; w++) {
-      const uint32_t c = s_count[w][bin];
-      s_count[w][bin] = (uint16_t)sofar;
-      sofar += c;
+  for (; at < hi; at += kWave) look(tokens[at + lane < hi ? at + lane : hi - 1], at + lane < hi, at + lane);
+  scan_block(lane ? 0 : lower, s_sums, &lower);  // (its barriers stand between the counts and their use, too)
+  uint32_t total = 0, inside;
+  if (tid < bins)
+    for (uint32_t w = 0; w < kSortWaves; w++) total += s_count[(w << a.bins_log2) + tid];
+  if (tid < bins && (tid << a.groups_log2 | group) < a.n_rows) a.used[tid << a.groups_log2 | group] = total;
+  uint32_t to = lower + scan_block(total, s_sums, &inside);
+  if (tid < bins)
+    for (uint32_t w = 0; w < kSortWaves; w++) {
+      const uint32_t c = s_count[(w << a.bins_log2) + tid];
+      s_count[(w << a.bins_log2) + tid] = to;
+      to += c;
     }
-  }
   __syncthreads();
-  #pragma unroll
-  for (uint32_t i = 0; i < kItems; i++) {
-    const uint64_t p = at0 + i * 64;
-    if (p < a.n) {
-      const uint32_t digit = (key[i] >> a.shift) & (bins - 1);
-      const uint32_t to = s_base[digit] + s_count[wave][digit] + rank[i];
-      a.keys_out[to] = key[i];
-      a.pos_out[to] = a.pos_in ? a.pos_in[p] : (uint32_t)p;
+  // the wave's own tokens in their order: those noted, or all of them once more where there were too many
+  volatile uint32_t* place = count;
+  const bool all = n_noted > kSortNoted;
+  const uint32_t steps = all ? hi - lo : n_noted;
+  for (uint32_t i = lane; i < (steps + kWave - 1) / kWave * kWave; i += kWave) {
+    const uint32_t p = i < steps ? (all ? lo + i : noted[i]) : a.n;
+    const uint32_t row = p < a.n ? row_of(tokens[p]) : a.n_rows, bin = row >> a.groups_log2;
+    const bool here = row < a.n_rows && (row & (groups - 1)) == group;
+    uint64_t same = __ballot(here);
+    if (!same) continue;
+    for (int b = 0; b < a.bins_log2; b++) {
+      const uint64_t ones = __ballot((bin >> b) & 1);
+      same &= (bin >> b) & 1 ? ones : ~ones;
     }
+    if (here) {
+      const uint32_t before = place[bin], rank = (uint32_t)__popcll(same & ((1ull << lane) - 1));
+      __builtin_amdgcn_wave_barrier();
+      if ((same >> lane) == 1) place[bin] = before + rank + 1;  // the highest lane of the row
+      a.keys[before + rank] = row;
+      a.pos[before + rank] = p;
+    }
+    __builtin_amdgcn_wave_barrier();
   }
+  if (group == groups - 1)
+    for (uint32_t i = lower + inside + tid; i < a.n; i += kSortThreads) a.keys[i] = a.n_rows;
 }
 
 // ---- gradient of the lookup ----------------------------------------------------------------------------------------
@@ -291,6 +211,7 @@ struct GradArgs {
   void* out;
   const uint32_t* keys;  // sorted
   const uint32_t* pos;
+  const uint32_t* used;  // tokens of each row
   float* partial;        // [chunk][2][width]
   uint64_t n, width;
   int64_t grad_stride, out_stride;
@@ -356,9 +277,12 @@ __device__ inline void store_piece(float* piece, const GradArgs& a, const Column
   if (c.inside) store_f32<F32, N>((uint32_t*)piece + c.at, acc, c.narrow ? (int64_t)a.width : N);
 }
 
-constexpr int kGradWaves = 4, kGradAhead = 8;
+// Rows whose loads are on their way at once: 16 in the sums of sorted tokens (20928 x 768: 50 us, 55 us with 8), 8 for few
+// tokens, of which most rows have one (509 of 1001 columns: 10.6 us, 12.2 us with 16) and in the join.
+constexpr int kGradWaves = 4, kSumAhead = 16, kFewAhead = 8, kJoinAhead = 8;
 // Rows that a workgroup looks through for ones without tokens: one a wave, so that they are written in address order by
-// workgroups that live as shortly as a copy's (128256 x 4096 in bf16: 327 us with 4 rows, 357 us with 64).
+// workgroups that live as shortly as a copy's (65536 tokens into 128256 x 4096 in bf16: 311 us with 4 rows, 326 us with 64;
+// 20928 into 52352 x 768 fp32: 50 us, 62 us).
 constexpr uint32_t kZeroRows = 4;
 
 template <typename S>
@@ -370,13 +294,7 @@ __global__ __launch_bounds__(kGradWaves* kWave) void etha_embedding_grad_kernel(
   const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   if (blockIdx.x >= a.sum_blocks) {  // rows without a token
     const uint64_t row0 = (uint64_t)(blockIdx.x - a.sum_blocks) * kZeroRows;
-    uint64_t lo = 0, hi = a.n;
-    const uint32_t mine = (uint32_t)(row0 + lane);
-    while (lo < hi) {
-      const uint64_t mid = (lo + hi) >> 1;
-      if (a.keys[mid] < mine) lo = mid + 1; else hi = mid;
-    }
-    const bool empty = lane < kZeroRows && row0 + lane < a.n_rows && !(lo < a.n && a.keys[lo] == mine);
+    const bool empty = lane < kZeroRows && row0 + lane < a.n_rows && !a.used[row0 + lane];
     uint64_t todo = __ballot(empty);
     constexpr int M = 16 / (int)sizeof(typename D::bits);
     const float zero[M] = {};
@@ -401,11 +319,11 @@ __global__ __launch_bounds__(kGradWaves* kWave) void etha_embedding_grad_kernel(
     const uint32_t key = at + lane < end ? a.keys[at + lane] : a.n_rows;
     const uint32_t pos = at + lane < end ? a.pos[at + lane] : 0;
     const uint32_t n = (uint32_t)__popcll(__ballot(key < a.n_rows));
-    for (uint32_t i = 0; i < n; i += kGradAhead) {
-      u32x4 raw[kGradAhead];
+    for (uint32_t i = 0; i < n; i += kSumAhead) {
+      u32x4 raw[kSumAhead];
       load_rows<S, N>(raw, a, c, n - i, [&](uint32_t u) { return (uint32_t)__builtin_amdgcn_readlane(pos, i + u); });
       #pragma unroll
-      for (uint32_t u = 0; u < kGradAhead; u++) {
+      for (uint32_t u = 0; u < kSumAhead; u++) {
         if (i + u >= n) break;
         const uint32_t k = __builtin_amdgcn_readlane(key, i + u);
         if (k != cur) {
@@ -468,11 +386,11 @@ __global__ __launch_bounds__(kGradWaves* kWave) void etha_embedding_grad_few_ker
   for (uint32_t r = 0; r < kFewTokenRows; r++) {
     if (row0 + r >= a.n_rows || (a.accumulate && !count[r])) continue;
     float acc[N] = {};
-    for (uint32_t i = 0; i < count[r]; i += kGradAhead) {
-      u32x4 raw[kGradAhead];
+    for (uint32_t i = 0; i < count[r]; i += kFewAhead) {
+      u32x4 raw[kFewAhead];
       load_rows<S, N>(raw, a, c, count[r] - i, [&](uint32_t u) { return (uint32_t)s_list[wave][r][i + u]; });
       #pragma unroll
-      for (uint32_t u = 0; u < kGradAhead; u++) {
+      for (uint32_t u = 0; u < kFewAhead; u++) {
         if (i + u >= count[r]) break;
         float v[N];
         raw_to_f32<S>(v, raw[u]);
@@ -498,7 +416,6 @@ __global__ __launch_bounds__(kGradWaves* kWave) void etha_embedding_join_kernel(
   const uint32_t key = a.keys[end], last = a.keys[end - 1], first = a.keys[begin], before = begin ? a.keys[begin - 1] : a.n_rows;
   if (key >= a.n_rows || last != key) return;    // nothing goes on behind this chunk
   if (first == key && before == key) return;     // begun earlier
-  constexpr int kAhead = N > 4 ? 4 : 8;
   const int64_t left = c.narrow ? (int64_t)a.width : N;
   float acc[N];
   load_f32<F32, N>(acc, (const uint32_t*)(a.partial + ((uint64_t)j * 2 + 1) * a.width + c.at), left);
@@ -507,24 +424,24 @@ __global__ __launch_bounds__(kGradWaves* kWave) void etha_embedding_join_kernel(
     const uint64_t start = (uint64_t)(j + 1 + lane) * a.chunk;
     const uint64_t same = __ballot(start < a.n && a.keys[start < a.n ? start : 0] == key);
     const uint32_t more = ~same ? __builtin_ctzll(~same) : 64;
-    for (uint32_t i = 0; i < more; i += kAhead) {
-      u32x4 raw[kAhead][N / 4];
+    for (uint32_t i = 0; i < more; i += kJoinAhead) {
+      u32x4 raw[kJoinAhead][N / 4];
       if (!c.narrow) {
         #pragma unroll
-        for (uint32_t u = 0; u < kAhead; u++)
+        for (uint32_t u = 0; u < kJoinAhead; u++)
           #pragma unroll
           for (int e = 0; e < N / 4; e++)
             raw[u][e] = load_raw<16>(a.partial + (uint64_t)(j + 1 + (i + u < more ? i + u : i)) * 2 * a.width + c.at + e * 4);
       } else {
         #pragma unroll
-        for (uint32_t u = 0; u < kAhead; u++)
+        for (uint32_t u = 0; u < kJoinAhead; u++)
           #pragma unroll
           for (int e = 0; e < N / 4; e++)
             raw[u][e] = load_part<4>((const char*)(a.partial + (uint64_t)(j + 1 + (i + u < more ? i + u : i)) * 2 * a.width + e * 4),
                                      ((int64_t)a.width - e * 4) * 4);
       }
       #pragma unroll
-      for (uint32_t u = 0; u < kAhead; u++) {
+      for (uint32_t u = 0; u < kJoinAhead; u++) {
         if (i + u >= more) break;
         #pragma unroll
         for (int e = 0; e < N; e++) acc[e] += __builtin_bit_cast(float, (uint32_t)raw[u][e / 4][e % 4]);
@@ -642,38 +559,44 @@ int check_tokens(const char* what, const void* tokens, uint32_t token_dtype, uin
   return ETHA_OK;
 }
 
-// Of a gradient, whose sort has every workgroup add up the counts of all others: here they are some hundred gigabytes of L2.
-int check_gradient_tokens(const char* what, uint64_t n_tokens) {
-  if (n_tokens > 1ull << 26) return fail(ETHA_ERR_UNSUPPORTED, "%s: %llu tokens; at most 2^26", what, (unsigned long long)n_tokens);
+// Workgroups of the sort: one a CU, more where a workgroup's rows would need more LDS than there is.
+int sort_groups_log2(uint64_t n_rows) {
+  const int rows = log2_up(n_rows);
+  return rows < kSortGroupsLog2 ? rows : rows - kSortGroupsLog2 > kSortBinsLog2 ? rows - kSortBinsLog2 : kSortGroupsLog2;
+}
+// Each of them looks through all tokens: 2^36 looks are some 50 ms.
+int check_gradient_tokens(const char* what, uint64_t n_tokens, uint64_t n_rows) {
+  if (n_tokens > 1ull << 26 || (n_tokens > kFewTokens && n_tokens << sort_groups_log2(n_rows) > 1ull << 36))
+    return fail(ETHA_ERR_UNSUPPORTED, "%s: %llu tokens of %llu rows; at most 2^26 tokens, or 2^46 over the rows where those are more than 2^20",
+                what, (unsigned long long)n_tokens, (unsigned long long)n_rows);
   return ETHA_OK;
 }
 
 // Column blocks, chunk length and workspace of a gradient call: a rule on sizes alone.
 struct GradPlan {
   uint32_t n_cols, chunk, n_chunks;
-  int passes, bits;
-  uint32_t sort_blocks;
-  uint64_t keys_bytes, hist_bytes, partial_bytes;
-  uint64_t total() const { return 4 * keys_bytes + hist_bytes + partial_bytes; }
+  int groups_log2, bins_log2;
+  uint64_t keys_bytes, used_bytes, partial_bytes;
+  uint64_t total() const { return 2 * keys_bytes + used_bytes + partial_bytes; }
 };
 GradPlan grad_plan(uint64_t n, uint64_t n_rows, uint64_t width, int es) {
   GradPlan p = {};
   const uint64_t per = 64 * (16 / es);
   p.n_cols = (uint32_t)((width + per - 1) / per);
-  // chunks of 128 places, shorter while there would be fewer waves than the chip holds a few of per SIMD, longer where the
-  // pieces of rows that cross chunks would need more than 2048 places in the workspace
+  // chunks of 128 places, shorter while there would be fewer waves than the chip holds a few of per SIMD (16 places where that
+  // is still less than two waves a SIMD: 6965 tokens of 76 columns 23 us, 28 us with 32; 57984 of 128 columns 56 us, 48 us with
+  // 32), longer where the pieces of rows that cross chunks would need more than 2048 places in the workspace
   uint64_t chunk = 128;
   while (chunk > 32 && (n + chunk - 1) / chunk * p.n_cols < 4096) chunk >>= 1;
+  if (chunk == 32 && (n + 15) / 16 * p.n_cols < 2048) chunk = 16;
   if ((n + chunk - 1) / chunk > 2048 && chunk == 128) chunk = ((n + 2047) / 2048 + 127) / 128 * 128;
   p.chunk = (uint32_t)chunk;
   p.n_chunks = (uint32_t)((n + chunk - 1) / chunk);
-  const int bits = log2_up(n_rows + 1);
-  p.passes = bits ? (bits + 8) / 9 : 1;
-  p.bits = bits ? (bits + p.passes - 1) / p.passes : 1;
-  p.sort_blocks = n <= kOneBlockTokens ? 0 : (uint32_t)((n + sort_tokens(n) - 1) / sort_tokens(n));
+  p.groups_log2 = sort_groups_log2(n_rows);
+  p.bins_log2 = log2_up(n_rows) - p.groups_log2;
   const auto up = [](uint64_t b) { return (b + 255) / 256 * 256; };
   p.keys_bytes = up(n * 4);
-  p.hist_bytes = up((uint64_t)p.sort_blocks * (1u << p.bits) * 4);
+  p.used_bytes = up(n_rows * 4);
   p.partial_bytes = up((uint64_t)p.n_chunks * 2 * width * 4);
   return p;
 }
@@ -732,7 +655,7 @@ int etha_embedding(const void* tokens, uint32_t token_dtype, uint64_t n_tokens, 
 
 int etha_embedding_grad_workspace(uint64_t n_tokens, uint64_t n_rows, uint64_t width, uint32_t grad_dtype, uint64_t* bytes) {
   int rc = check_tokens("etha_embedding_grad_workspace", &n_tokens, ETHA_I32, n_tokens, n_rows, width);
-  if (rc == ETHA_OK) rc = check_gradient_tokens("etha_embedding_grad_workspace", n_tokens);
+  if (rc == ETHA_OK) rc = check_gradient_tokens("etha_embedding_grad_workspace", n_tokens, n_rows);
   if (rc != ETHA_OK) return rc;
   if (!bytes) return fail(ETHA_ERR_INVALID, "etha_embedding_grad_workspace: null result");
   if (!es_of(grad_dtype)) return fail(ETHA_ERR_UNSUPPORTED, "etha_embedding_grad_workspace: element types are f32, bf16 and f16");
@@ -745,7 +668,7 @@ int etha_embedding_grad(const void* grad, uint32_t grad_dtype, int64_t grad_stri
                         uint32_t out_dtype, int64_t out_stride, int accumulate, void* workspace, uint64_t workspace_bytes,
                         void* stream) {
   int rc = check_tokens("etha_embedding_grad", tokens, token_dtype, n_tokens, n_rows, width);
-  if (rc == ETHA_OK) rc = check_gradient_tokens("etha_embedding_grad", n_tokens);
+  if (rc == ETHA_OK) rc = check_gradient_tokens("etha_embedding_grad", n_tokens, n_rows);
   if (rc != ETHA_OK) return rc;
   const int es = es_of(grad_dtype);
   if (!es || !es_of(out_dtype)) return fail(ETHA_ERR_UNSUPPORTED, "etha_embedding_grad: element types are f32, bf16 and f16");
@@ -780,43 +703,16 @@ int etha_embedding_grad(const void* grad, uint32_t grad_dtype, int64_t grad_stri
     if (!workspace || workspace_bytes < p.total() || ((uintptr_t)workspace & 15))
       return fail(ETHA_ERR_INVALID, "etha_embedding_grad: the workspace has to hold %llu bytes at a 16-byte address",
                   (unsigned long long)p.total());
-    uint32_t* keys[2] = {(uint32_t*)workspace, (uint32_t*)((char*)workspace + p.keys_bytes)};
-    uint32_t* pos[2] = {(uint32_t*)((char*)workspace + 2 * p.keys_bytes), (uint32_t*)((char*)workspace + 3 * p.keys_bytes)};
-    int at = 0;
-    if (!p.sort_blocks) {
-      hipLaunchKernelGGL(etha_sort_tokens_kernel, dim3(1), dim3(kOneBlockThreads), 0, (hipStream_t)stream, tokens,
-                         (uint32_t)(token_dtype == ETHA_I64), (uint32_t)n_tokens, first_row, (uint32_t)n_rows, p.passes, p.bits,
-                         keys[0], pos[0]);
-      if ((rc = launched("etha_sort_tokens_kernel")) != ETHA_OK) return rc;
-    } else {
-      SortArgs s = {};
-      s.tokens = tokens;
-      s.wide = token_dtype == ETHA_I64;
-      s.n = n_tokens;
-      s.first = first_row;
-      s.n_rows = (uint32_t)n_rows;
-      s.bits = p.bits;
-      s.hist = (uint32_t*)((char*)workspace + 4 * p.keys_bytes);
-      for (int pass = 0; pass < p.passes; pass++) {
-        s.shift = pass * p.bits;
-        s.keys_in = pass ? keys[at ^ 1] : nullptr;
-        s.pos_in = pass ? pos[at ^ 1] : nullptr;
-        s.keys_out = keys[at];
-        s.pos_out = pos[at];
-        const bool wide_blocks = sort_tokens(n_tokens) == 4096;
-        const auto count = wide_blocks ? etha_sort_count_kernel<4096> : etha_sort_count_kernel<1024>;
-        const auto scatter = wide_blocks ? etha_sort_scatter_kernel<4096> : etha_sort_scatter_kernel<1024>;
-        hipLaunchKernelGGL(count, dim3(p.sort_blocks), dim3(kSortThreads), 0, (hipStream_t)stream, s);
-        if ((rc = launched("etha_sort_count_kernel")) != ETHA_OK) return rc;
-        hipLaunchKernelGGL(scatter, dim3(p.sort_blocks), dim3(kSortThreads), 0, (hipStream_t)stream, s);
-        if ((rc = launched("etha_sort_scatter_kernel")) != ETHA_OK) return rc;
-        at ^= 1;
-      }
-      at ^= 1;
-    }
-    g.keys = keys[at];
-    g.pos = pos[at];
-    g.partial = (float*)((char*)workspace + 4 * p.keys_bytes + p.hist_bytes);
+    SortArgs sort = {tokens, (uint32_t*)workspace, nullptr, nullptr, (uint32_t)n_tokens, (uint32_t)n_rows, first_row, p.groups_log2, p.bins_log2};
+    sort.pos = (uint32_t*)((char*)sort.keys + p.keys_bytes);
+    sort.used = (uint32_t*)((char*)sort.pos + p.keys_bytes);
+    const auto kernel = token_dtype == ETHA_I64 ? etha_sort_tokens_kernel<int64_t> : etha_sort_tokens_kernel<int32_t>;
+    hipLaunchKernelGGL(kernel, dim3(1u << p.groups_log2), dim3(kSortThreads), 0, (hipStream_t)stream, sort);
+    if ((rc = launched("etha_sort_tokens_kernel")) != ETHA_OK) return rc;
+    g.keys = sort.keys;
+    g.pos = sort.pos;
+    g.used = sort.used;
+    g.partial = (float*)((char*)sort.used + p.used_bytes);
     g.chunk = p.chunk;
     g.n_chunks = p.n_chunks;
     g.n_cols = p.n_cols;

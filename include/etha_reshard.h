@@ -345,7 +345,8 @@ int etha_embedding(const void* tokens, uint32_t token_dtype, uint64_t n_tokens, 
  * Gradient of the lookup: out[r,:] = scale * sum of grad[t,:] over the tokens of row r, in the order of t (pieces of a
  * frequent row are summed apart and joined in order); zeros for a row without tokens.  With accumulate the sum is added
  * to out (one rounding) and rows without tokens are left as they are.  The workspace (16-byte aligned, at least the
- * bytes that etha_embedding_grad_workspace names) may be used again once the launches have finished.  At most 2^26 tokens.
+ * bytes that etha_embedding_grad_workspace names) may be used again once the launches have finished.  At most 2^26 tokens, and
+ * 2^46 / n_rows of them where there are more than 2^20 rows.
  */
 int etha_embedding_grad_workspace(uint64_t n_tokens, uint64_t n_rows, uint64_t width, uint32_t grad_dtype, uint64_t* bytes);
 int etha_embedding_grad(const void* grad, uint32_t grad_dtype, int64_t grad_stride, const void* tokens, uint32_t token_dtype,

@@ -107,7 +107,7 @@ def test_entry_points_refuse_what_they_cannot_take():
     assert grad(ws=0x1004) == nat.ERR_INVALID
     assert grad(g=None) == nat.ERR_INVALID
     assert grad(r=0) == 0 and grad(n=0, a=1) == 0
-    assert grad(n=(1 << 26) + 1) == nat.ERR_UNSUPPORTED
+    assert grad(n=(1 << 26) + 1) == nat.ERR_UNSUPPORTED and grad(n=(1 << 21) + 1, r=1 << 25) == nat.ERR_UNSUPPORTED
     need = nat.embedding_grad_workspace
     assert need(0, 8, 4, nat.F32) == 0 and need(4000, 8, 4, nat.F32) > 0
     with pytest.raises(nat.EthaNativeError):
