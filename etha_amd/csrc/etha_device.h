@@ -5,6 +5,7 @@
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
+#include <type_traits>
 
 #include "etha_reshard.h"
 
@@ -160,11 +161,12 @@ struct RowScale {
   __device__ explicit RowScale(uint32_t top) {
     scale = __builtin_bit_cast(float, top) * (1.f / 127.f);
     none = !(scale > 0.f) || top >= 0x7f800000u;  // a row of zeros, or one that holds an infinity or NaN
-    // a scale below the smallest normal number may have no finite inverse: the quotient is formed by division there
-    tiny = scale < 1.2e-38f;
+    // a scale below the smallest normal number may have no finite inverse, and half of one below twice that may be no
+    // number: the quotient is formed by division there
+    tiny = scale < 2.4e-38f;
     inverse = 1.f / scale;
   }
-  // near: x / scale, give or take a few roundings
+  // x / scale rounded; near: x / scale, give or take a few roundings
   __device__ uint32_t value(float x, float near) const {
     float q = __builtin_rintf(near);
     const float r = __builtin_fmaf(-q, scale, x);
@@ -173,19 +175,51 @@ struct RowScale {
     if (twice > scale || (twice == scale && ((int)q & 1))) q += (r > 0.f) ? 1.f : -1.f;
     return (uint32_t)(int)__builtin_fmaxf(-127.f, __builtin_fminf(127.f, q)) & 255u;
   }
+  // bytes 0 of eight words
+  static __device__ u32x2 low_bytes(const float (&t)[8]) {
+    u32x2 w;
+    #pragma unroll
+    for (int i = 0; i < 2; i++) {
+      const auto bits = [&](int e) { return __builtin_bit_cast(uint32_t, t[4 * i + e]); };
+      w[i] = __builtin_amdgcn_perm(__builtin_amdgcn_perm(bits(3), bits(2), 0x0c0c0400), __builtin_amdgcn_perm(bits(1), bits(0), 0x0c0c0400),
+                                   0x05040100);
+    }
+    return w;
+  }
+  // Eight elements that came from type T.  Added to 1.5 * 2^23 a product is rounded to an integer, which the low byte of the
+  // sum holds.  It is the wrong one only where what is left of x * inverse, which is off by at most 127 * 2^-24 < 2^-17, lies
+  // within 2e-5 of one half: seldom in any of a wave's elements, but for bf16, whose few bits make such quotients common.
+  // There, and otherwise, r says whether it is off by one; exact ties are left to the general way.  (56732 rows of 1024 in
+  // fp16: 37 us, 40 us without the first way, 43 us the general way alone; 23040 rows of 2496 in bf16: 48 us, 54 us alone.)
+  template <typename T>
   __device__ u32x2 pack(const float (&v)[8]) const {
     u32x2 w = {0, 0};
     if (none) return w;
-    float near[8];
-    if (tiny) {
+    if (!tiny) {
+      constexpr float kRound = 12582912.f;
+      float t[8];
+      if constexpr (!std::is_same_v<T, BF16>) {
+        float left = 0.f;
+        #pragma unroll
+        for (int i = 0; i < 8; i++) {
+          t[i] = __builtin_fmaf(v[i], inverse, kRound);
+          left = __builtin_fmaxf(left, __builtin_fabsf(__builtin_fmaf(v[i], inverse, kRound - t[i])));
+        }
+        if (__ballot(left > 0.49998f) == 0) return low_bytes(t);
+      }
+      const float half = 0.5f * scale;
+      bool tie = false;
       #pragma unroll
-      for (int i = 0; i < 8; i++) near[i] = v[i] / scale;
-    } else {
-      #pragma unroll
-      for (int i = 0; i < 8; i++) near[i] = v[i] * inverse;
+      for (int i = 0; i < 8; i++) {
+        const float sum = __builtin_fmaf(v[i], inverse, kRound);
+        const float r = __builtin_fmaf(kRound - sum, scale, v[i]);
+        t[i] = sum + (__builtin_fabsf(r) > half ? __builtin_copysignf(1.f, r) : 0.f);
+        tie |= __builtin_fabsf(r) == half;
+      }
+      if (__ballot(tie) == 0) return low_bytes(t);
     }
     #pragma unroll
-    for (int i = 0; i < 8; i++) w[i >> 2] |= value(v[i], near[i]) << (8 * (i & 3));
+    for (int i = 0; i < 8; i++) w[i >> 2] |= value(v[i], tiny ? v[i] / scale : v[i] * inverse) << (8 * (i & 3));
     return w;
   }
 };

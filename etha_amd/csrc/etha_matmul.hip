@@ -753,11 +753,11 @@ __global__ __launch_bounds__(kFewThreads) void etha_few_rows_kernel(const FewArg
         #pragma unroll
         for (int i = 0; i < kFewWaves; i++) top = s_top[m][i] > top ? s_top[m][i] : top;
         const RowScale scale(top);
-        if (k0 < pitch - 32) *(u32x2*)(s_x + m * pitch + k0) = scale.pack(kept[m]);  // past the end of k: zeros
+        if (k0 < pitch - 32) *(u32x2*)(s_x + m * pitch + k0) = scale.pack<SX>(kept[m]);  // past the end of k: zeros
         for (uint32_t k = k0 + kFewThreads * 8; k < pitch - 32; k += kFewThreads * 8) {
           float v[8];
           load_f32<SX, 8>(v, rows + (int64_t)(row0 + m) * few.x_stride + k, (int64_t)red - k);
-          *(u32x2*)(s_x + m * pitch + k) = scale.pack(v);
+          *(u32x2*)(s_x + m * pitch + k) = scale.pack<SX>(v);
         }
       }
     __syncthreads();
@@ -1068,7 +1068,7 @@ int run_matmul(const char* what, const MatmulArgs& a, uint32_t out_dtype, void* 
 bool is_out(uint32_t dtype) { return dtype == ETHA_F32 || dtype == ETHA_BF16 || dtype == ETHA_F16; }
 
 // Rows that the few-rows kernel converts itself.  Every 16 columns convert them again while their part of the matrix
-// arrives: one row costs less than a launch (14336 x 4096: 14.2 us, 16.5 us with a launch of its own), further rows do where
+// arrives: one row costs less than a launch (14336 x 4096: 13.2 us, 16.5 us with a launch of its own), further rows do where
 // the workgroups are all resident and a row fits the registers (1024 x 4096: 9.5 us for 4 rows, 13 us; 14336 x 4096: 24 us).
 bool is_few(uint64_t rows, uint64_t cols, uint64_t width) {
   const uint64_t padded = (width + 127) / 128 * 128;

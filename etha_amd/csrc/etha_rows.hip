@@ -529,7 +529,7 @@ __global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS) void etha_quantize_r
       if (at >= width) continue;
       float v[8];
       values(c, v);
-      const u32x2 packed = scale.pack(v);
+      const u32x2 packed = scale.pack<S>(v);
       if (width >= 8) {
         store_raw<8, true>(out + (at < last ? at : last), packed);
       } else {
@@ -605,8 +605,8 @@ int quantize_launch(const QuantArgs& a, uint32_t dtype, hipStream_t stream) {
   with_type(dtype, [&](auto s) {
     typedef decltype(s) S;
     // a wave (16 lanes for the narrowest: 45913 rows of 102 in bf16 6 us, 36 us with a wave) a row while the row fits its
-    // registers, else a workgroup a row, with no more registers than the row needs (64128 rows of 4096 in fp32: 219 us with
-    // room for 4096, 236 us with room for 8192)
+    // registers, else a workgroup a row, with no more registers than the row needs (64128 rows of 4096 in fp32: 215 us with
+    // room for 4096, some 15 us more with room for 8192)
     if (a.width <= 16 * 8 * 4)
       hipLaunchKernelGGL((etha_quantize_rows_kernel<S, 16, 4>), dim3((uint32_t)((a.rows + 15) / 16)), dim3(256), 0, stream, a);
     else if (a.width <= 64 * 8 * 2)

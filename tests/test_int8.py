@@ -148,6 +148,27 @@ def test_rounding_of_halves(gpu_device):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("power", [-127, -126, -125, -100, 0, 100])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16], ids=str)
+def test_rounding_next_to_halves(gpu_device, dtype, power):
+    """Quotients within a few units of the last place of every half, and on it where it is a number; the last column is the
+    row's largest magnitude and sets its scale."""
+    if dtype == torch.float16 and power != 0:
+        pytest.skip("out of the range of float16")
+    gen = torch.Generator().manual_seed(4)
+    top = (torch.rand(64, 1, generator=gen).double() + 1) * 100 * 2.0 ** power
+    scale = (top.float() * (torch.ones(()) / 127)).double()
+    x = ((torch.arange(-126, 126).double() + 0.5) * scale).to(dtype)
+    bits = x.view(torch.int32 if dtype == torch.float32 else torch.int16)
+    nudged = [(bits + k).view(dtype) for k in (-2, -1, 0, 1, 2)]
+    x = torch.cat([*nudged, top.to(dtype)], 1)
+    assert bool((x.abs().amax(1) == x[:, -1].abs()).all())
+    for columns in (slice(None), slice(0, None, 5), slice(4, None, 41)):  # alone in their waves, or together
+        part = torch.cat([x[:, columns], x[:, -1:]], 1).to(gpu_device)
+        check_rows(part, *quantize_rows(part))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("width", [40, 3000, 9000, 40000])
 def test_rows_with_zeros_infinities_and_nan(gpu_device, width):
     x = torch.randn(8, width, device=gpu_device)
