@@ -601,24 +601,32 @@ GradPlan grad_plan(uint64_t n, uint64_t n_rows, uint64_t width, int es) {
   return p;
 }
 
+template <typename S, int THREADS, int CHUNKS>
+void quantize_with(const QuantArgs& a, hipStream_t stream) {
+  constexpr int kBlock = THREADS < 256 ? 256 : THREADS, kRows = kBlock / THREADS;
+  hipLaunchKernelGGL((etha_quantize_rows_kernel<S, THREADS, CHUNKS>), dim3((uint32_t)((a.rows + kRows - 1) / kRows)), dim3(kBlock), 0, stream, a);
+}
+
+// Part of a wave or a wave a row while the row fits its registers (narrow rows: 45913 of 102 in bf16 6 us, 36 us with a wave),
+// else a workgroup a row, always with little more room than the row needs (64128 rows of 4096 in fp32: 215 us with room for
+// 4096, some 15 us more with room for 8192).  16-bit rows go further in a wave: 49268 of 832 31 us with 32 lanes, 33 us with 64;
+// 23040 of 2496 36 us with a wave, 48 us with a workgroup; 32768 of 2700 59 us, 71 us; 64128 of 4096 143 us, 157 us, but 8192 of
+// 4096 28 us, 25 us.  fp32 does not: 49268 of 832 38 us with 32 lanes, 36 us; 8246 of 2453 22.3 us with a wave, 20.7 us.
 int quantize_launch(const QuantArgs& a, uint32_t dtype, hipStream_t stream) {
   with_type(dtype, [&](auto s) {
     typedef decltype(s) S;
-    // a wave (16 lanes for the narrowest: 45913 rows of 102 in bf16 6 us, 36 us with a wave) a row while the row fits its
-    // registers, else a workgroup a row, with no more registers than the row needs (64128 rows of 4096 in fp32: 215 us with
-    // room for 4096, some 15 us more with room for 8192)
-    if (a.width <= 16 * 8 * 4)
-      hipLaunchKernelGGL((etha_quantize_rows_kernel<S, 16, 4>), dim3((uint32_t)((a.rows + 15) / 16)), dim3(256), 0, stream, a);
-    else if (a.width <= 64 * 8 * 2)
-      hipLaunchKernelGGL((etha_quantize_rows_kernel<S, 64, 2>), dim3((uint32_t)((a.rows + 3) / 4)), dim3(256), 0, stream, a);
-    else if (a.width <= 64 * 8 * 4)
-      hipLaunchKernelGGL((etha_quantize_rows_kernel<S, 64, 4>), dim3((uint32_t)((a.rows + 3) / 4)), dim3(256), 0, stream, a);
-    else if (a.width <= 256 * 8 * 2)
-      hipLaunchKernelGGL((etha_quantize_rows_kernel<S, 256, 2>), dim3((uint32_t)a.rows), dim3(256), 0, stream, a);
-    else if (a.width <= 256 * 8 * 4)
-      hipLaunchKernelGGL((etha_quantize_rows_kernel<S, 256, 4>), dim3((uint32_t)a.rows), dim3(256), 0, stream, a);
-    else
-      hipLaunchKernelGGL((etha_quantize_rows_kernel<S, 1024, 4>), dim3((uint32_t)a.rows), dim3(1024), 0, stream, a);
+    if constexpr (sizeof(typename S::bits) == 2) {
+      if (a.width > 16 * 8 * 4 && a.width <= 32 * 8 * 4) return quantize_with<S, 32, 4>(a, stream);
+      if (a.width > 64 * 8 * 4 && a.width <= 64 * 8 * 5) return quantize_with<S, 64, 5>(a, stream);
+      if (a.width > 64 * 8 * 5 && a.width <= 64 * 8 * 8 && (a.width <= 64 * 8 * 7 || a.rows >= 32768)) return quantize_with<S, 64, 8>(a, stream);
+    } else {
+      if (a.width > 16 * 8 * 4 && a.width <= 64 * 8 * 2) return quantize_with<S, 64, 2>(a, stream);
+    }
+    if (a.width <= 16 * 8 * 4) return quantize_with<S, 16, 4>(a, stream);
+    if (a.width <= 64 * 8 * 4) return quantize_with<S, 64, 4>(a, stream);
+    if (a.width <= 256 * 8 * 2) return quantize_with<S, 256, 2>(a, stream);
+    if (a.width <= 256 * 8 * 4) return quantize_with<S, 256, 4>(a, stream);
+    return quantize_with<S, 1024, 4>(a, stream);
   });
   return launched("etha_quantize_rows_kernel");
 }

@@ -111,7 +111,8 @@ def test_entry_points_refuse_what_they_cannot_take():
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", DTYPES, ids=str)
 @pytest.mark.parametrize("rows,width", [(1, 1), (5, 7), (3, 64), (70, 511), (9, 1001), (6, 2048), (4, 2056), (130, 4096), (5, 8191),
-                                        (4, 8200), (3, 32768), (2, 33001)])
+                                        (4, 8200), (3, 32768), (2, 33001), (37, 700), (33, 1024), (11, 2300), (9, 2560), (7, 2561), (6, 3584),
+                                        (5, 3585), (32769, 3600)])
 def test_rows(gpu_device, rows, width, dtype):
     gen = torch.Generator(device=gpu_device).manual_seed(rows * width)
     x = (torch.randn(rows, width, generator=gen, device=gpu_device) * 3).to(dtype)
@@ -148,13 +149,10 @@ def test_rounding_of_halves(gpu_device):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("power", [-127, -126, -125, -100, 0, 100])
-@pytest.mark.parametrize("dtype", [torch.float32, torch.float16], ids=str)
+@pytest.mark.parametrize("dtype,power", [(torch.float16, 0), *((torch.float32, p) for p in (-127, -126, -125, -100, 0, 100))], ids=str)
 def test_rounding_next_to_halves(gpu_device, dtype, power):
     """Quotients within a few units of the last place of every half, and on it where it is a number; the last column is the
     row's largest magnitude and sets its scale."""
-    if dtype == torch.float16 and power != 0:
-        pytest.skip("out of the range of float16")
     gen = torch.Generator().manual_seed(4)
     top = (torch.rand(64, 1, generator=gen).double() + 1) * 100 * 2.0 ** power
     scale = (top.float() * (torch.ones(()) / 127)).double()
