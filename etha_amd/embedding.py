@@ -84,7 +84,7 @@ def embedding_grad(grad: torch.Tensor, tokens: torch.Tensor, n_rows: int, *, sca
 
     ``grad``: the gradient of the result, ``tokens.shape + (width,)``.  Rows without a token become zeros.  With ``out`` and
     ``accumulate=True`` the sums are added to ``out`` (micro-batches into one gradient) and rows without a token are not
-    touched.  The same inputs give the same bits.
+    touched.  The same inputs give the same bits.  The result is not part of a graph.
     """
     if grad.dim() != tokens.dim() + 1 or grad.shape[:-1] != tokens.shape:
         raise ValueError(f"embedding_grad: grad has shape {tuple(grad.shape)} for tokens of {tuple(tokens.shape)}")

@@ -136,6 +136,7 @@ def grouped_linear_grad_weight(grad: torch.Tensor, x: torch.Tensor, offsets: tor
 
 def grouped_linear_grad(grad: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor, *,
                         weight_dtype: torch.dtype | None = None) -> tuple[torch.Tensor, torch.Tensor]:
-    """Both gradients of :func:`grouped_linear`: of ``x``, and of ``weight`` in ``weight_dtype`` (default: the weight's)."""
+    """Both gradients of :func:`grouped_linear`: of ``x``, and of ``weight`` in ``weight_dtype`` (default: the weight's).  Neither
+    is part of a graph."""
     return (grouped_linear_grad_rows(grad, weight, offsets),
             grouped_linear_grad_weight(grad, x, offsets, dtype=weight_dtype or weight.dtype))
