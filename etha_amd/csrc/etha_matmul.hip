@@ -46,6 +46,12 @@ struct ElemI8 {
   }
 };
 
+// A sum of products of integers, which is exact, with its scales and bias: written as a fused operation, so that every kernel
+// gives the same bits.
+__device__ inline float scaled(float sum, float scale, bool with_bias, float bias) {
+  return with_bias ? __builtin_fmaf(sum, scale, bias) : sum * scale;
+}
+
 enum Kind : uint32_t {
   kPlain = 0,        // one product: P k-contiguous, Q k-contiguous
   kGroupRows = 1,    // rows of P belong to groups, a Q for each group, k-contiguous
@@ -525,10 +531,8 @@ __global__ __launch_bounds__(S::kThreads) void etha_matmul_kernel(const MatmulAr
       for (int j = 0; j < kFn; j++)
         #pragma unroll
         for (int c = 0; c < 4; c++) {
-          // the integer sum is exact; one product of scales, as the definition has it
           if constexpr (E::kEs == 1) {
-            v[j][c] = (float)acc[i][j][c] * (row_scale * col_scale[j][c]);
-            if (a.bias) v[j][c] += bias[j][c];
+            v[j][c] = scaled((float)acc[i][j][c], row_scale * col_scale[j][c], a.bias != nullptr, bias[j][c]);
           } else {
             v[j][c] = acc[i][j][c];
           }
@@ -618,8 +622,7 @@ __global__ __launch_bounds__(256) void etha_matmul_short_kernel(const MatmulArgs
              element<E>(q + (kTransQ ? (int64_t)k * a.q_stride : (int64_t)k * E::kEs));
     float v = (float)sum;
     if constexpr (E::kEs == 1) {
-      v *= a.row_scale[row] * a.col_scale[col];
-      if (a.bias) v += a.bias[col];
+      v = scaled(v, a.row_scale[row] * a.col_scale[col], a.bias != nullptr, a.bias ? a.bias[col] : 0.f);
     }
     ((typename D::bits*)a.out)[out + (int64_t)row * a.out_stride + col] = D::from_f32(v);
   }
@@ -635,7 +638,8 @@ __global__ __launch_bounds__(256) void etha_matmul_short_kernel(const MatmulArgs
 // lines of the matrix are on their way: one launch instead of two.
 // MT blocks of 16 rows share what is read of the matrix.
 constexpr int kFewCols = 16, kFewWaves = 8, kFewThreads = kFewWaves * 64;
-constexpr int kFewConverted = 4;     // rows that are converted here: every 16 columns read them again
+constexpr int kFewConverted = 16;    // rows that are converted here at most: every 16 columns read them again
+constexpr int kFewTogether = 4;      // rows up to which the whole workgroup converts each of them
 constexpr uint32_t kFewLds = 32768;  // bytes of converted rows at most
 
 struct FewArgs {
@@ -728,38 +732,59 @@ __global__ __launch_bounds__(kFewThreads) void etha_few_rows_kernel(const FewArg
   if (early) load(line);
   if constexpr (kConvert) {
     const typename SX::bits* rows = (const typename SX::bits*)few.x;
-    const uint32_t k0 = threadIdx.x * 8;
-    float kept[kFewConverted][8];  // the first 4096 of a row stay in registers, all rows' loads are on their way at once
-    #pragma unroll
-    for (uint32_t m = 0; m < kFewConverted; m++)
-      if (m < n_rows) load_f32<SX, 8>(kept[m], rows + (int64_t)(row0 + m) * few.x_stride + k0, (int64_t)red - k0);
-    #pragma unroll
-    for (uint32_t m = 0; m < kFewConverted; m++)
-      if (m < n_rows) {
-        uint32_t top = largest_bits(kept[m], 0);
-        for (uint32_t k = k0 + kFewThreads * 8; k < red; k += kFewThreads * 8) {
+    if (n_rows <= kFewTogether) {
+      const uint32_t k0 = threadIdx.x * 8;
+      float kept[kFewTogether][8];  // the first 4096 of a row stay in registers, all rows' loads are on their way at once
+      #pragma unroll
+      for (uint32_t m = 0; m < kFewTogether; m++)
+        if (m < n_rows) load_f32<SX, 8>(kept[m], rows + (int64_t)(row0 + m) * few.x_stride + k0, (int64_t)red - k0);
+      #pragma unroll
+      for (uint32_t m = 0; m < kFewTogether; m++)
+        if (m < n_rows) {
+          uint32_t top = largest_bits(kept[m], 0);
+          for (uint32_t k = k0 + kFewThreads * 8; k < red; k += kFewThreads * 8) {
+            float v[8];
+            load_f32<SX, 8>(v, rows + (int64_t)(row0 + m) * few.x_stride + k, (int64_t)red - k);
+            top = largest_bits(v, top);
+          }
+          top = group_max<64>(top);
+          if (lane == 0) s_top[m][wave] = top;
+        }
+      __syncthreads();
+      #pragma unroll
+      for (uint32_t m = 0; m < kFewTogether; m++)
+        if (m < n_rows) {
+          uint32_t top = 0;
+          #pragma unroll
+          for (int i = 0; i < kFewWaves; i++) top = s_top[m][i] > top ? s_top[m][i] : top;
+          const RowScale scale(top);
+          if (k0 < pitch - 32) *(u32x2*)(s_x + m * pitch + k0) = scale.pack<SX>(kept[m]);  // past the end of k: zeros
+          for (uint32_t k = k0 + kFewThreads * 8; k < pitch - 32; k += kFewThreads * 8) {
+            float v[8];
+            load_f32<SX, 8>(v, rows + (int64_t)(row0 + m) * few.x_stride + k, (int64_t)red - k);
+            *(u32x2*)(s_x + m * pitch + k) = scale.pack<SX>(v);
+          }
+        }
+    } else {
+      for (uint32_t m = wave; m < n_rows; m += kFewWaves) {  // a wave a row, which is read twice
+        const typename SX::bits* x = rows + (int64_t)(row0 + m) * few.x_stride;
+        uint32_t top = 0;
+        #pragma unroll 4
+        for (uint32_t k = lane * 8; k < red; k += 64 * 8) {
           float v[8];
-          load_f32<SX, 8>(v, rows + (int64_t)(row0 + m) * few.x_stride + k, (int64_t)red - k);
+          load_f32<SX, 8>(v, x + k, (int64_t)red - k);
           top = largest_bits(v, top);
         }
         top = group_max<64>(top);
-        if (lane == 0) s_top[m][wave] = top;
-      }
-    __syncthreads();
-    #pragma unroll
-    for (uint32_t m = 0; m < kFewConverted; m++)
-      if (m < n_rows) {
-        uint32_t top = 0;
-        #pragma unroll
-        for (int i = 0; i < kFewWaves; i++) top = s_top[m][i] > top ? s_top[m][i] : top;
+        if (lane < kFewWaves) s_top[m][lane] = top;
         const RowScale scale(top);
-        if (k0 < pitch - 32) *(u32x2*)(s_x + m * pitch + k0) = scale.pack<SX>(kept[m]);  // past the end of k: zeros
-        for (uint32_t k = k0 + kFewThreads * 8; k < pitch - 32; k += kFewThreads * 8) {
+        for (uint32_t k = lane * 8; k < pitch - 32; k += 64 * 8) {
           float v[8];
-          load_f32<SX, 8>(v, rows + (int64_t)(row0 + m) * few.x_stride + k, (int64_t)red - k);
+          load_f32<SX, 8>(v, x + k, (int64_t)red - k);
           *(u32x2*)(s_x + m * pitch + k) = scale.pack<SX>(v);
         }
       }
+    }
     __syncthreads();
   }
   if (early) {
@@ -811,8 +836,7 @@ __global__ __launch_bounds__(kFewThreads) void etha_few_rows_kernel(const FewArg
       } else {
         row_scale = a.row_scale[row];
       }
-      v *= row_scale * a.col_scale[col];
-      if (a.bias) v += a.bias[col];
+      v = scaled(v, row_scale * a.col_scale[col], a.bias != nullptr, a.bias ? a.bias[col] : 0.f);
     }
     ((typename D::bits*)a.out)[(int64_t)row * a.out_stride + col] = D::from_f32(v);
   }
@@ -1068,11 +1092,15 @@ int run_matmul(const char* what, const MatmulArgs& a, uint32_t out_dtype, void* 
 bool is_out(uint32_t dtype) { return dtype == ETHA_F32 || dtype == ETHA_BF16 || dtype == ETHA_F16; }
 
 // Rows that the few-rows kernel converts itself.  Every 16 columns convert them again while their part of the matrix
-// arrives: one row costs less than a launch (14336 x 4096: 13.2 us, 16.5 us with a launch of its own), further rows do where
-// the workgroups are all resident and a row fits the registers (1024 x 4096: 9.5 us for 4 rows, 13 us; 14336 x 4096: 24 us).
+// arrives, which is less than a launch where that is little (16 x 2048 x 2048: 9.5 to 12.3 us, 13.6 us with a launch of its
+// own; 8 x 4096 x 4096: 11.3 or 16.9 us, by how the workgroups come to lie on the CUs, 13.6 us) and the workgroups are all
+// resident or the rows short (8 x 14336 x 1024: 10.2 to 12.9 us, 13.5 us; 4 x 14336 x 2048: 14.9 us, 13.5 us); a single row
+// always is (14336 x 4096: 14.4 us, 16.5 us).
 bool is_few(uint64_t rows, uint64_t cols, uint64_t width) {
   const uint64_t padded = (width + 127) / 128 * 128;
-  return padded <= kFewLds && (rows == 1 || (rows <= kFewConverted && cols <= 8192 && padded <= kFewThreads * 8));
+  if (rows > kFewConverted || rows * padded > kFewLds) return false;
+  return rows == 1 || (rows * padded * ((cols + 4095) / 4096) <= kFewLds && (cols <= 8192 || padded <= 1024) &&
+                       (rows <= kFewTogether || padded <= 2048));
 }
 uint64_t padded_width(uint64_t width) { return (width + 15) / 16 * 16; }
 

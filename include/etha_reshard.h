@@ -364,7 +364,7 @@ int etha_quantize_rows(const void* x, uint32_t dtype, uint64_t rows, uint64_t wi
 
 /*
  * Product of 8-bit rows with a scale each: out[m,n] = x_scale[m] * w_scale[n] * sum_k x[m,k] * w[n,k] + bias[n] (bias:
- * fp32, may be NULL).  The sum is exact; width is at most ETHA_INT8_MAX_WIDTH, so that it stays within 32 bits.
+ * fp32, may be NULL; added in one fused operation).  The sum is exact; width is at most ETHA_INT8_MAX_WIDTH, so that it stays within 32 bits.
  */
 #define ETHA_INT8_MAX_WIDTH 131071u
 int etha_int8_matmul(const int8_t* x, const float* x_scale, uint64_t rows, int64_t x_stride, const int8_t* w, const float* w_scale,

@@ -263,7 +263,9 @@ def test_product_of_views(gpu_device):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", DTYPES, ids=str)
-@pytest.mark.parametrize("m,n,k", [(1, 515, 4096), (1, 64, 77), (1, 40, 33001), (2, 300, 4100), (4, 9000, 256), (3, 1000, 1001), (8, 512, 2048), (40, 200, 512), (300, 400, 640)])
+@pytest.mark.parametrize("m,n,k", [(1, 515, 4096), (1, 64, 77), (1, 40, 33001), (2, 300, 4100), (4, 9000, 256), (3, 1000, 1001), (8, 512, 2048), (40, 200, 512), (300, 400, 640),
+                                   (5, 70, 200), (7, 33, 4096), (9, 8200, 1000), (12, 9000, 1030), (16, 130, 2048), (16, 100, 2049), (16, 17, 5),
+                                   (17, 130, 512)])
 def test_linear(gpu_device, m, n, k, dtype):
     gen = torch.Generator(device=gpu_device).manual_seed(m * n + k)
     _, _, w, ws = operands(gen, 1, n, k, gpu_device)
@@ -283,7 +285,7 @@ def test_linear(gpu_device, m, n, k, dtype):
 @pytest.mark.gpu
 def test_a_poisoned_token_poisons_its_row_alone(gpu_device):
     gen = torch.Generator(device=gpu_device).manual_seed(5)
-    for m in (4, 100):
+    for m in (4, 12, 100):
         _, _, w, ws = operands(gen, 1, 70, 200, gpu_device)
         x = torch.randn(m, 200, generator=gen, device=gpu_device)
         x[2, 7] = float("nan")
