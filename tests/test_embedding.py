@@ -210,6 +210,27 @@ def test_gradient_of_repeated_tokens(gpu_device, tokens, id_of):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("tokens,rows", [(5000, 600000), (5000, 262144), (5000, 262145), (40000, 256), (40000, 257), (40000, 1024)])
+def test_gradient_by_number_of_rows(gpu_device, tokens, rows):
+    """From more rows than the workgroups that group the tokens have room for, to one row a workgroup."""
+    gen = torch.Generator(device=gpu_device).manual_seed(rows)
+    grad = torch.randn(tokens, 3, generator=gen, device=gpu_device)
+    ids = torch.randint(-5, rows + 5, (tokens,), generator=gen, device=gpu_device)
+    check_gradient(embedding_grad(grad, ids, rows), grad, ids, rows, 1.0, 0)
+
+
+@pytest.mark.gpu
+def test_gradient_of_a_padded_batch(gpu_device):
+    """One token half of the time in a part of the batch: some waves meet more of a workgroup's tokens than they can note."""
+    gen = torch.Generator(device=gpu_device).manual_seed(8)
+    grad = torch.randn(60000, 40, generator=gen, device=gpu_device).bfloat16()
+    ids = torch.randint(0, 3000, (60000,), generator=gen, device=gpu_device)
+    ids[20000:][torch.rand(40000, generator=gen, device=gpu_device) < 0.5] = 7
+    ids[50000:] = 7
+    check_gradient(embedding_grad(grad, ids, 3000, dtype=torch.float32), grad, ids, 3000, 1.0, 0)
+
+
+@pytest.mark.gpu
 def test_gradient_accumulates_and_leaves_the_rest(gpu_device):
     gen = torch.Generator(device=gpu_device).manual_seed(1)
     for tokens in (40, 10000):
