@@ -30,6 +30,15 @@ logger = logging.getLogger(__name__)
 HEARTBEAT_MAX_AGE = 5.0  # seconds (client.py:374)
 
 
+def _refresh(int8_weights) -> None:
+    """Waits for the conversion, because the agent's stream, which the next transfer is written on, does not."""
+    for weight in int8_weights:
+        weight.refresh()
+    for device in {weight.landing.device for weight in int8_weights}:
+        if device.type == "cuda":
+            torch.cuda.current_stream(device).synchronize()
+
+
 class BatchHandler:
     """Handle of one registered batch (``client.py:30-107``)."""
 
@@ -48,22 +57,14 @@ class BatchHandler:
         return client
 
     def transfer(self, transfer_type: Literal["send", "recv"], blocking: bool = False, timeout: float = 30.0) -> Completion:
-        """As the client's ``transfer``.  A blocking ``recv`` also converts the batch's 8-bit weights (on the current
-        stream); after one that does not block call :meth:`refresh_int8` once it has completed."""
-        msg = Transfer(batch_id=self.batch_id, transfer_type=transfer_type)
-        done = self.client._execute_command_with_semaphore(
-            msg, "transfer", context_id=f"batch_{self.batch_id}_{transfer_type}", blocking=blocking, timeout=timeout)
-        if blocking and transfer_type == "recv":
-            self.refresh_int8()
-        return done
+        """As the client's ``transfer``."""
+        return self.client._transfer(self.batch_id, transfer_type, f"batch_{self.batch_id}_{transfer_type}", blocking, timeout)
 
     def refresh_int8(self) -> None:
-        """Convert the batch's 8-bit weights from what the last transfer brought (no counterpart in the reference); waits
-        for it, because the agent's stream, which the next transfer is written on, does not."""
-        for weight in self.int8_weights:
-            weight.refresh()
-        for device in {weight.landing.device for weight in self.int8_weights}:
-            torch.cuda.current_stream(device).synchronize()
+        """Convert the batch's 8-bit weights from what the last transfer brought (no counterpart in the reference), on the
+        current stream.  A ``recv`` does so itself once its completion is acquired; this is for a caller that learns of
+        it in another way (``query_transfer_signal``)."""
+        _refresh(self.int8_weights)
 
     def query_transfer_signal(self, blocking: bool = True, timeout: float = 30.0) -> bool:
         return self.client.query_transfer_signal(self.batch_id, blocking=blocking, timeout=timeout)
@@ -72,6 +73,7 @@ class BatchHandler:
         if self._closed:
             return
         self._closed = True
+        self.client._int8_weights.pop(self.batch_id, None)
         msg = CleanupBatch(batch_id=self.batch_id)
         self.client._execute_command_with_semaphore(
             msg, "cleanup_batch", context_id=f"batch_{self.batch_id}", blocking=blocking, timeout=timeout)
@@ -103,6 +105,7 @@ class TensorBusClient:
         if lmdb_command_queue_path is None:
             lmdb_command_queue_path = os.environ.get("TENSOR_BUS_COMMAND_QUEUE_PATH")
         self.command_queue = CommandQueue(lmdb_command_queue_path)
+        self._int8_weights: dict[str, tuple[Int8Weight, ...]] = {}  # of the batches that have any
 
     # ---- plumbing ---------------------------------------------------------------------------
     def _read_state(self) -> dict | None:
@@ -131,11 +134,12 @@ class TensorBusClient:
         )
 
     def _execute_command_with_semaphore(self, command, command_type: str, context_id: str, blocking: bool = False,
-                                        timeout: float = 30.0) -> Completion:
+                                        timeout: float = 30.0, then=None) -> Completion:
         command.semaphore_name = generate_semaphore_name(command_type, context_id)
         command.timestamp = time.time()
         command.agent_rank = self.agent_rank
         sem = self.command_queue.enqueue(command)
+        sem.then = then
         if blocking:
             try:
                 sem.acquire(timeout=timeout)
@@ -169,8 +173,15 @@ class TensorBusClient:
 
     def transfer(self, batch_id: str, transfer_type: Literal["send", "recv"], blocking: bool = False,
                  timeout: float = 30.0) -> Completion:
-        msg = Transfer(batch_id=batch_id, transfer_type=transfer_type)
-        return self._execute_command_with_semaphore(msg, "transfer", context_id=batch_id, blocking=blocking, timeout=timeout)
+        """A ``recv`` also converts the batch's 8-bit weights, on the stream that is current when its completion is
+        acquired: within this call if it blocks, else in the returned completion's ``acquire``."""
+        return self._transfer(batch_id, transfer_type, batch_id, blocking, timeout)
+
+    def _transfer(self, batch_id: str, transfer_type: str, context_id: str, blocking: bool, timeout: float) -> Completion:
+        int8_weights = self._int8_weights.get(batch_id) if transfer_type == "recv" else None
+        return self._execute_command_with_semaphore(
+            Transfer(batch_id=batch_id, transfer_type=transfer_type), "transfer", context_id=context_id, blocking=blocking,
+            timeout=timeout, then=(lambda: _refresh(int8_weights)) if int8_weights else None)
 
     def query_transfer_signal(self, batch_id: str, blocking: bool = True, timeout: float = 30.0) -> bool:
         msg = QueryStatus(batch_id=batch_id, state_name="transfer_signal")
@@ -185,7 +196,7 @@ class TensorBusClient:
         """Register tensors across pairs; always blocks until every rank of the batch has registered.
 
         A receiving rank may register an :class:`~etha_amd.int8.Int8Weight`: its ``landing`` is the tensor that is filled,
-        and the handler converts it behind each transfer.
+        and a ``recv`` converts it (see :meth:`transfer`).
         """
         if not tensors:
             raise ValueError("tensors list cannot be empty")
@@ -204,6 +215,8 @@ class TensorBusClient:
             # memory and, as in the reference, the worker keeps its tensors alive for as long as the batch lives.
             for _, p in payloads:
                 release_local(p)
+        if int8_weights:
+            self._int8_weights[batch_id] = int8_weights
         unique_pair_names = list(dict.fromkeys(pair_name for _, pair_name in tensors))
         return BatchHandler(client=self, batch_id=batch_id, pair_names=unique_pair_names, int8_weights=int8_weights)
 

@@ -36,11 +36,17 @@ class Completion:
         self._conn = conn
         self.name = name
         self.result = None
+        self.then = None  # called once, by the acquire() that finds the command completed without an error
         self._done = False
 
     def acquire(self, timeout: float | None = None):
-        if self._done:
-            return
+        if not self._done:
+            self._receive(timeout)
+        if self.then is not None:
+            self.then()
+            self.then = None  # not before it has succeeded: a call that raised is made again
+
+    def _receive(self, timeout: float | None):
         if not self._conn.poll(timeout):
             raise BusyError(self.name)
         try:
@@ -49,6 +55,7 @@ class Completion:
             raise ConnectionError("agent closed the connection before completing the command") from e
         self._done = True
         if status == "error":
+            self.then = None
             exc_type, message = value
             raise {"ValueError": ValueError, "RuntimeError": RuntimeError, "KeyError": KeyError,
                    "NotImplementedError": NotImplementedError, "TimeoutError": TimeoutError}.get(exc_type, RuntimeError)(message)

@@ -244,31 +244,45 @@ class ReshardJob:
 
     # ------------------------------------------------------------------------------------------
     def run_send(self, merge_launches: bool = False, fanout: int = 1, drive: bool = True) -> None:
-        for buckets in self.send_buckets.values():
+        """The senders' half of a transfer.  If nothing is waiting for a peer behind it, targets in 8 bits are converted;
+        who steps the wire otherwise (``drive=False``, a peer process) calls :meth:`refresh_int8` when it is idle."""
+        self._half(self.send_buckets, merge_launches, fanout, drive)
+        self._refresh_if_idle()
+
+    def run_recv(self, merge_launches: bool = False, fanout: int = 1, drive: bool = True) -> None:
+        """The receivers' half of a transfer; targets in 8 bits as in :meth:`run_send`."""
+        self._half(self.recv_buckets, merge_launches, fanout, drive)
+        self._refresh_if_idle()
+
+    def _half(self, lists: dict[int, list], merge_launches: bool, fanout: int, drive: bool) -> None:
+        for buckets in lists.values():
             bucket_comm(buckets, self.max_in_flight, wire=self.wire, merge_launches=merge_launches, synchronize=False,
                         fanout=fanout, drive=drive)
 
-    def run_recv(self, merge_launches: bool = False, fanout: int = 1, drive: bool = True) -> None:
-        for buckets in self.recv_buckets.values():
-            bucket_comm(buckets, self.max_in_flight, wire=self.wire, merge_launches=merge_launches, synchronize=False,
-                        fanout=fanout, drive=drive)
+    def _refresh_if_idle(self) -> None:
+        if any(self.target_int8) and self.wire.idle():
+            self.refresh_int8()
+
+    def refresh_int8(self) -> None:
+        """Convert the targets in 8 bits from what lies in their landings, on the current stream."""
+        for weights in self.target_int8:
+            for weight in weights.values():
+                weight.refresh()
 
     def run(self, merge_launches: bool = False, synchronize: bool = True, fanout: int = 1) -> None:
         """One transfer: every source rank calls ``bucket_comm`` on its send list, then every target rank on its
         receive list.  With a ring pool the senders fill their slots and wait on the wire; the receivers' calls
         then move both sides along until every bucket has been unpacked.  Targets in 8 bits are converted behind it."""
         if self.wire.pool_mode == "ring":  # this process plays every rank: queue all pipelines, step them together
-            self.run_send(merge_launches, fanout, drive=False)
-            self.run_recv(merge_launches, fanout, drive=False)
+            self._half(self.send_buckets, merge_launches, fanout, drive=False)
+            self._half(self.recv_buckets, merge_launches, fanout, drive=False)
             self.wire.drive()
         else:
-            self.run_send(merge_launches, fanout)
-            self.run_recv(merge_launches, fanout)
+            self._half(self.send_buckets, merge_launches, fanout, drive=True)
+            self._half(self.recv_buckets, merge_launches, fanout, drive=True)
         if not self.wire.idle():
             raise RuntimeError(f"transfer did not complete; still waiting for a peer: {self.wire.pending()}")
-        for weights in self.target_int8:
-            for weight in weights.values():
-                weight.refresh()
+        self.refresh_int8()
         if synchronize and self.device.type == "cuda":
             torch.cuda.current_stream(self.device).synchronize()
 

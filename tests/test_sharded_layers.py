@@ -11,10 +11,12 @@ import pytest
 import torch
 from torch.distributed.tensor.placement_types import Partial, Replicate, Shard
 
+from etha_amd.comm import LoopbackWire
 from etha_amd.embedding import embedding, embedding_grad
 from etha_amd.experts import grouped_linear, grouped_linear_grad
 from etha_amd.int8 import Int8Weight, int8_linear
 from etha_amd.layout import local_shard
+from etha_amd.tensor_bus.command_queue import Completion
 from etha_amd.world import ReshardJob, TensorSpec
 
 from test_embedding import check_gradient, plain_lookup
@@ -232,6 +234,146 @@ def test_the_bus_takes_the_landing_of_an_8_bit_weight(agent_factory):  # noqa: F
     handlers = run_ranks(body, range(2))
     assert handlers[0].int8_weights == () and handlers[1].int8_weights == (weight,)
     assert agent.batches["b"].recv_buckets[1][0].chunks[0].tensor.data_ptr() == weight.landing.data_ptr()
+    for h in handlers.values():
+        h.close()
+    for c in clients.values():
+        c.close()
+
+
+def count_refreshes(monkeypatch):
+    """Stands in for the conversion, which needs a GPU: notes what the landing held when it was called."""
+    seen = []
+    monkeypatch.setattr(Int8Weight, "refresh", lambda self: seen.append(self.landing.clone()) or self)
+    return seen
+
+
+@pytest.mark.parametrize("how", ["handler", "client", "handler, not blocking", "client, not blocking"])
+def test_every_receive_through_the_bus_converts(agent_factory, monkeypatch, how):  # noqa: F811
+    """Whichever call brings the new weights: what it leaves in the landing is converted once, when it is known to be there."""
+    seen = count_refreshes(monkeypatch)
+    agent, naming = agent_factory(2)
+    weight = Int8Weight(torch.zeros(8, 4))
+    clients = {r: _client(naming, r, connection_timeout=5) for r in range(2)}
+
+    def body(r):
+        names = ("trainer", "inference") if r == 0 else ("inference", "trainer")
+        clients[r].init_pair("w", *names, 1, device_mesh=np.arange(1), placements=(Replicate(),), timeout=10)
+        return clients[r].register_tensors("b", [(torch.ones(8, 4) if r == 0 else weight, "w")], timeout=10)
+
+    handlers = run_ranks(body, range(2))
+
+    class Done:
+        """A command that the agent has finished."""
+
+        def poll(self, timeout):
+            return True
+
+        def recv(self):
+            return "ok", None
+
+        def close(self):
+            pass
+
+    for c in clients.values():
+        c.command_queue.enqueue = lambda command: Completion(Done(), "done")
+    blocking = "not" not in how
+    for k in range(1, 3):
+        weight.landing.fill_(k)
+        who = handlers[1].transfer if how.startswith("handler") else lambda *a, **kw: clients[1].transfer("b", *a, **kw)
+        done = who("recv", blocking=blocking)
+        if not blocking:
+            assert len(seen) == k - 1
+            done.acquire(timeout=5)
+            done.acquire(timeout=5)  # once
+        assert len(seen) == k and bool((seen[-1] == k).all())
+    handlers[0].transfer("send", blocking=True)
+    clients[1].transfer("b", "send", blocking=True)
+    clients[1].transfer("another batch", "recv", blocking=True)
+    assert len(seen) == 2
+    for h in handlers.values():
+        h.close()
+    clients[1].transfer("b", "recv", blocking=True)
+    assert len(seen) == 2, "a closed batch keeps no weights"
+
+
+def test_a_failed_receive_does_not_convert():
+    class Failed:
+        def poll(self, timeout):
+            return True
+
+        def recv(self):
+            return "error", ("ValueError", "no such batch")
+
+    done = Completion(Failed(), "failed")
+    called = []
+    done.then = lambda: called.append(1)
+    with pytest.raises(ValueError, match="no such batch"):
+        done.acquire()
+    done.acquire()
+    assert not called
+
+
+def test_the_halves_of_a_transfer_convert_too(monkeypatch):
+    """run_send and run_recv, called apart: the call behind which nothing is waiting any more converts; run() once."""
+    seen = count_refreshes(monkeypatch)
+    spec = TensorSpec("w", (64, 16), [0, 1], (Shard(0),), [2, 3], (Shard(0),), torch.float32, target_int8=True)
+    job = ReshardJob([spec], device="cpu", bucket_size=256, wire=LoopbackWire("cpu", host_inspection=True))
+    job.wire.on_launch = lambda *a: None
+    job.run_send()
+    assert not seen and not job.wire.idle()
+    job.run_recv()
+    assert len(seen) == 2 and job.wire.idle()  # a target shard each
+    del seen[:]
+    job.run()
+    assert len(seen) == 2
+    # both halves queued, the wire stepped by hand: the caller says when
+    del seen[:]
+    job.run_send(drive=False)
+    job.run_recv(drive=False)
+    assert not seen and not job.wire.idle()
+    job.wire.drive()
+    job.refresh_int8()
+    assert len(seen) == 2
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("pool", ["ring", "resident"])
+def test_the_halves_of_a_transfer_bring_new_values(gpu_device, pool):
+    spec = TensorSpec("w", (96, 640), [0, 1], (Shard(0),), [2], (Replicate(),), torch.float32, torch.bfloat16, seed=1, target_int8=True)
+    job = ReshardJob([spec], device=gpu_device, pool=pool)
+    weight = job.target_int8[0][2]
+    for _ in range(3):
+        for t in job.source_locals[0].values():
+            t.mul_(-1.5)
+        job.run_send()
+        job.run_recv()
+        check_int8_rows(weight.landing, weight.values, weight.scales)
+        assert torch.equal(weight.landing, torch.cat([job.source_locals[0][r] for r in (0, 1)]).bfloat16())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("blocking", [True, False])
+def test_an_8_bit_weight_through_the_clients_own_transfer(gpu_device, agent_factory, blocking):  # noqa: F811
+    agent, naming = agent_factory(2, device=gpu_device)
+    src = torch.randn(40, 96, device=gpu_device)
+    weight = Int8Weight(torch.zeros(40, 96, dtype=torch.bfloat16, device=gpu_device))
+    clients = {r: _client(naming, r, connection_timeout=5) for r in range(2)}
+
+    def body(r):
+        names = ("trainer", "inference") if r == 0 else ("inference", "trainer")
+        clients[r].init_pair("w", *names, 1, device_mesh=np.arange(1), placements=(Replicate(),))
+        return clients[r].register_tensors("b", [(src if r == 0 else weight, "w")])
+
+    handlers = run_ranks(body, range(2))
+    for _ in range(2):
+        src.mul_(-1.5)
+        torch.cuda.synchronize()
+        done = run_ranks(lambda r: clients[r].transfer("b", "send" if r == 0 else "recv", blocking=blocking), range(2))
+        if not blocking:
+            for c in done.values():
+                c.acquire(timeout=30)
+        assert torch.equal(weight.landing, src.bfloat16())
+        check_int8_rows(weight.landing, weight.values, weight.scales)
     for h in handlers.values():
         h.close()
     for c in clients.values():
