@@ -4,6 +4,7 @@
 from __future__ import annotations
 
 import torch
+from torch.autograd.graph import increment_version
 
 from . import _native
 
@@ -97,6 +98,14 @@ def check_out(what: str, out: torch.Tensor, shape, dtypes, *inputs: torch.Tensor
                 if a < hi and lo < b:
                     raise ValueError(f"{what}: out overlaps an input")
     return stride
+
+
+def written(*outs: torch.Tensor | None) -> None:
+    """Tells autograd that the caller's tensors were written: kernels write by address, which it cannot see, and a graph that
+    saved one of them earlier would go on with the new values."""
+    for out in outs:
+        if out is not None:
+            increment_version(out)
 
 
 def refuse_grad(what: str, *inputs: torch.Tensor | None) -> None:

@@ -12,7 +12,7 @@ import torch
 
 from . import _native
 from ._operands import (DTYPE_CODES, TOKEN_CODES, call, check_device, check_out, code_of, readable_rows, refuse_captured_backward,
-                        row_stride)
+                        row_stride, written)
 
 
 def _token_operand(what: str, tokens: torch.Tensor) -> tuple[torch.Tensor, int]:
@@ -31,6 +31,7 @@ def _lookup(tokens, weight, scale, first_row, dtype, out):
         raise ValueError("embedding: the rows of weight have to be contiguous")
     weight_code = code_of("embedding", weight.dtype)
     source, token_code = _token_operand("embedding", tokens)
+    given = out
     if out is None:
         dtype = dtype or weight.dtype
         out_code = code_of("embedding", dtype)
@@ -45,6 +46,7 @@ def _lookup(tokens, weight, scale, first_row, dtype, out):
         device = check_device("embedding", weight, tokens, out)
     call(device, "etha_embedding", source.data_ptr(), token_code, tokens.numel(), weight.data_ptr(),
          weight_code, rows, width, stride, first_row, scale, out.data_ptr(), out_code, out_stride)
+    written(given)
     return out
 
 
@@ -96,6 +98,7 @@ def embedding_grad(grad: torch.Tensor, tokens: torch.Tensor, n_rows: int, *, sca
     grad_code = code_of("embedding_grad", grad.dtype)
     grad, grad_stride = readable_rows(grad)
     source, token_code = _token_operand("embedding_grad", tokens)
+    given = out
     if out is None:
         dtype = dtype or grad.dtype
         out_code = code_of("embedding_grad", dtype)
@@ -113,4 +116,5 @@ def embedding_grad(grad: torch.Tensor, tokens: torch.Tensor, n_rows: int, *, sca
     call(device, "etha_embedding_grad", grad.data_ptr(), grad_code, grad_stride, source.data_ptr(),
          token_code, n_tokens, n_rows, width, first_row, scale, out.data_ptr(), out_code, out_stride, int(accumulate),
          workspace.data_ptr() if nbytes else None, nbytes)
+    written(given)
     return out

@@ -11,7 +11,8 @@ from __future__ import annotations
 import torch
 
 from . import _native
-from ._operands import DTYPE_CODES, MOST_STRIDE, call, check_device, check_out, code_of, readable_rows, refuse_captured_backward
+from ._operands import (DTYPE_CODES, MOST_STRIDE, call, check_device, check_out, code_of, readable_rows, refuse_captured_backward,
+                        written)
 
 _OPERANDS = {torch.bfloat16: _native.BF16, torch.float16: _native.F16}
 
@@ -55,7 +56,7 @@ def _product(what, x, weight, offsets, transposed, out):
     weight, w_stride, w_group = _matrices(what, weight)
     offsets = offsets if offsets.is_contiguous() else offsets.contiguous()
     rows = x.shape[0]
-    fresh = out is None
+    given, fresh = out, out is None
     if not fresh:
         out_stride = check_out(what, out, (rows, cols), DTYPE_CODES, x, weight, offsets)
     device = check_device(what, x, weight, offsets, out)
@@ -64,6 +65,7 @@ def _product(what, x, weight, offsets, transposed, out):
     call(device, "etha_grouped_matmul", source.data_ptr(), _OPERANDS[x.dtype], rows, stride,
          weight.data_ptr(), experts, cols, red, w_stride, w_group, int(transposed), offsets.data_ptr(), out.data_ptr(),
          DTYPE_CODES[out.dtype], out_stride, int(fresh))
+    written(given)
     return out
 
 
@@ -116,6 +118,7 @@ def grouped_linear_grad_weight(grad: torch.Tensor, x: torch.Tensor, offsets: tor
     g, g_stride = readable_rows(grad, MOST_STRIDE)
     r, r_stride = readable_rows(x, MOST_STRIDE)
     offsets = offsets if offsets.is_contiguous() else offsets.contiguous()
+    given = out
     if out is None:
         dtype = dtype or x.dtype
         code_of(what, dtype)
@@ -131,6 +134,7 @@ def grouped_linear_grad_weight(grad: torch.Tensor, x: torch.Tensor, offsets: tor
     call(device, "etha_grouped_matmul_reduce", g.data_ptr(), r.data_ptr(), _OPERANDS[x.dtype], x.shape[0], g_stride, r_stride, experts,
          n, k, offsets.data_ptr(), out.data_ptr(), DTYPE_CODES[out.dtype], out.stride(1), out.stride(0),
          workspace.data_ptr() if nbytes else None, nbytes)
+    written(given)
     return out
 
 

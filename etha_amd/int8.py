@@ -11,7 +11,7 @@ from __future__ import annotations
 import torch
 
 from . import _native
-from ._operands import DTYPE_CODES, MOST_STRIDE, call, check_device, check_out, code_of, readable_rows, refuse_grad
+from ._operands import DTYPE_CODES, MOST_STRIDE, call, check_device, check_out, code_of, readable_rows, refuse_grad, written
 
 INT8_MAX_WIDTH = 131071  # ETHA_INT8_MAX_WIDTH
 
@@ -38,12 +38,14 @@ def quantize_rows(x: torch.Tensor, *, values: torch.Tensor | None = None,
     width = x.shape[-1]
     rows = x.numel() // width if width else x.shape[:-1].numel()
     source, stride = readable_rows(x)
+    given = values, scales
     if values is None:
         values, values_stride = x.new_empty(x.shape, dtype=torch.int8), width
     if scales is None:
         scales = x.new_empty(x.shape[:-1], dtype=torch.float32)
     call(device, "etha_quantize_rows", source.data_ptr(), code, rows, width, stride,
          values.data_ptr(), values_stride, scales.data_ptr())
+    written(*given)
     return values, scales
 
 
@@ -86,12 +88,14 @@ def int8_matmul(x: torch.Tensor, x_scales: torch.Tensor, weight: torch.Tensor, w
     if out is not None:
         out_stride = check_out(what, out, (*x.shape[:-1], channels), DTYPE_CODES, x, x_scales, weight, weight_scales, bias)
     device = check_device(what, x, x_scales, weight, weight_scales, bias, out)
+    given = out
     if out is None:
         code_of(what, dtype)
         out, out_stride = x.new_empty((*x.shape[:-1], channels), dtype=dtype), channels
     call(device, "etha_int8_matmul", source.data_ptr(), x_scales.data_ptr(), rows, stride,
          weight.data_ptr(), weight_scales.data_ptr(), channels, w_stride, width, None if bias is None else bias.data_ptr(),
          out.data_ptr(), DTYPE_CODES[out.dtype], out_stride)
+    written(given)
     return out
 
 
@@ -110,6 +114,7 @@ def int8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scales: torch.Tens
         if dtype is not None and dtype != out.dtype:
             raise ValueError(f"{what}: dtype {dtype} and an out of {out.dtype}")
     device = check_device(what, x, weight, weight_scales, bias, out)
+    given = out
     if out is None:
         dtype = dtype or x.dtype
         code_of(what, dtype)
@@ -119,6 +124,7 @@ def int8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scales: torch.Tens
     call(device, "etha_int8_linear", source.data_ptr(), x_code, rows, stride, weight.data_ptr(),
          weight_scales.data_ptr(), channels, w_stride, width, None if bias is None else bias.data_ptr(), out.data_ptr(),
          DTYPE_CODES[out.dtype], out_stride, workspace.data_ptr() if nbytes else None, nbytes)
+    written(given)
     return out
 
 

@@ -1,0 +1,87 @@
+"""What autograd learns of the operators on local shards: buffers that a call writes, derivatives that it does not have.
+
+On the CPU a stand-in takes the place of the launch: everything asked for here happens on the host.
+"""
+
+import pytest
+import torch
+
+from etha_amd import embedding as embedding_module, experts as experts_module, int8 as int8_module
+from etha_amd.embedding import embedding, embedding_grad
+from etha_amd.experts import grouped_linear, grouped_linear_grad_rows, grouped_linear_grad_weight
+from etha_amd.int8 import Int8Weight, int8_linear, int8_matmul, quantize_rows
+
+
+@pytest.fixture(params=["cpu", pytest.param("gpu", marks=pytest.mark.gpu)])
+def device(request, monkeypatch):
+    if request.param == "gpu":
+        return request.getfixturevalue("gpu_device")
+    for module in (embedding_module, experts_module, int8_module):
+        monkeypatch.setattr(module, "check_device", lambda what, first, *others: 0)
+        monkeypatch.setattr(module, "call", lambda index, name, *args: None)
+    return torch.device("cpu")
+
+
+class Operands:
+    def __init__(self, device):
+        zeros = lambda *shape, dtype=torch.float32: torch.zeros(*shape, dtype=dtype, device=device)
+        self.tokens = zeros(6, dtype=torch.int64)
+        self.table, self.rows = zeros(5, 8), zeros(6, 8)
+        self.x, self.up, self.weight = zeros(6, 8).bfloat16(), zeros(6, 16).bfloat16(), zeros(2, 16, 8).bfloat16()
+        self.offsets = torch.tensor([0, 2, 6], dtype=torch.int32, device=device)
+        self.q, self.w = zeros(6, 8, dtype=torch.int8), zeros(16, 8, dtype=torch.int8)
+        self.row_scales, self.col_scales = zeros(6), zeros(16)
+        self.zeros = zeros
+
+
+# name -> (shape of what it writes, a call that writes it)
+WRITERS = {
+    "embedding": ((6, 8), lambda o, out: embedding(o.tokens, o.table, out=out)),
+    "embedding_grad": ((5, 8), lambda o, out: embedding_grad(o.rows, o.tokens, 5, out=out)),
+    "embedding_grad, accumulate": ((5, 8), lambda o, out: embedding_grad(o.rows, o.tokens, 5, out=out, accumulate=True)),
+    "grouped_linear": ((6, 16), lambda o, out: grouped_linear(o.x, o.weight, o.offsets, out=out)),
+    "grouped_linear_grad_rows": ((6, 8), lambda o, out: grouped_linear_grad_rows(o.up, o.weight, o.offsets, out=out)),
+    "grouped_linear_grad_weight": ((2, 16, 8), lambda o, out: grouped_linear_grad_weight(o.up, o.x, o.offsets, out=out)),
+    "quantize_rows, scales": ((6,), lambda o, out: quantize_rows(o.rows, scales=out)),
+    "int8_matmul": ((6, 16), lambda o, out: int8_matmul(o.q, o.row_scales, o.w, o.col_scales, out=out)),
+    "int8_linear": ((6, 16), lambda o, out: int8_linear(o.rows, o.w, o.col_scales, out=out)),
+}
+
+
+@pytest.mark.parametrize("name", WRITERS)
+def test_a_saved_buffer_that_is_written_again_is_noticed(device, name):
+    """A graph holds the buffer that a call writes: a later backward pass through it must not use the new values."""
+    shape, write = WRITERS[name]
+    o = Operands(device)
+    buffer, p = o.zeros(*shape), o.zeros(*shape).requires_grad_()
+    with torch.no_grad():
+        write(o, buffer)
+    z = (buffer * p).sum()
+    z.backward(retain_graph=True)  # what was written before is no trouble
+    with torch.no_grad():
+        write(o, buffer)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        z.backward()
+
+
+def test_views_and_integers_that_are_written_are_noticed(device):
+    o = Operands(device)
+    wide = o.zeros(6, 20)
+    before = wide._version
+    embedding(o.tokens, o.table, out=wide[:, 3:11])
+    assert wide._version == before + 1
+    values = o.zeros(6, 8, dtype=torch.int8)
+    quantize_rows(o.rows, values=values)
+    assert values._version == 1
+    weight = Int8Weight(o.zeros(16, 8))
+    before = weight.values._version, weight.scales._version, weight.landing._version
+    weight.refresh()
+    assert (weight.values._version, weight.scales._version, weight.landing._version) == (before[0] + 1, before[1] + 1, before[2])
+
+
+def test_inference_tensors_are_written(device):
+    o = Operands(device)
+    with torch.inference_mode():
+        buffer = o.zeros(6, 8)
+        embedding(o.tokens, o.table, out=buffer)
+    embedding(o.tokens, o.table, out=buffer)  # they count no versions
