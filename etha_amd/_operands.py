@@ -4,6 +4,7 @@
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.graph import increment_version
 
 from . import _native
@@ -83,6 +84,7 @@ def check_out(what: str, out: torch.Tensor, shape, dtypes, *inputs: torch.Tensor
         raise ValueError(f"{what}: out is {out.dtype}")
     if out.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{what}: out requires a gradient")
+    refuse_tangent(what, out)
     if out.dim() and out.is_contiguous():
         stride = shape[-1]
     else:
@@ -108,8 +110,18 @@ def written(*outs: torch.Tensor | None) -> None:
             increment_version(out)
 
 
+def refuse_tangent(what: str, *tensors: torch.Tensor | None) -> None:
+    """No operator has a forward-mode derivative, and a result without a tangent would stand for one of zero."""
+    if forward_ad._current_level < 0:  # outside of forward-mode differentiation no tensor has a tangent
+        return
+    for t in tensors:
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise RuntimeError(f"{what} has no forward-mode derivative: pass the primal of its operands")
+
+
 def refuse_grad(what: str, *inputs: torch.Tensor | None) -> None:
     """For operators without a gradient: a silent cut of the graph would train on nothing."""
+    refuse_tangent(what, *inputs)
     for t in inputs:
         if t is not None and t.requires_grad and torch.is_grad_enabled():
             raise RuntimeError(f"{what} has no gradient: call it under torch.no_grad() or detach its inputs")

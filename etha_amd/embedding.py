@@ -12,7 +12,7 @@ import torch
 
 from . import _native
 from ._operands import (DTYPE_CODES, TOKEN_CODES, call, check_device, check_out, code_of, readable_rows, refuse_captured_backward,
-                        row_stride, written)
+                        refuse_tangent, row_stride, written)
 
 
 def _token_operand(what: str, tokens: torch.Tensor) -> tuple[torch.Tensor, int]:
@@ -71,8 +71,9 @@ def embedding(tokens: torch.Tensor, weight: torch.Tensor, *, scale: float = 1.0,
     """``scale * weight[tokens - first_row]`` in ``dtype`` (default: the weight's), zeros for tokens outside the shard.
 
     ``tokens``: int32 or int64, any shape; ``weight``: ``[rows, width]`` in fp32, bf16 or fp16 with contiguous rows.  The
-    product with ``scale`` is formed in fp32 and rounded once.  Differentiable in ``weight`` (not with ``out``).
+    product with ``scale`` is formed in fp32 and rounded once.  Differentiable in ``weight`` (in reverse mode; not with ``out``).
     """
+    refuse_tangent("embedding", weight)
     if weight.requires_grad and torch.is_grad_enabled():
         if out is not None:
             raise ValueError("embedding: out cannot be given where weight requires a gradient")
@@ -88,6 +89,7 @@ def embedding_grad(grad: torch.Tensor, tokens: torch.Tensor, n_rows: int, *, sca
     ``accumulate=True`` the sums are added to ``out`` (micro-batches into one gradient) and rows without a token are not
     touched.  The same inputs give the same bits.  The result is not part of a graph.
     """
+    refuse_tangent("embedding_grad", grad)
     if grad.dim() != tokens.dim() + 1 or grad.shape[:-1] != tokens.shape:
         raise ValueError(f"embedding_grad: grad has shape {tuple(grad.shape)} for tokens of {tuple(tokens.shape)}")
     if n_rows < 0:

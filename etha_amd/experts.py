@@ -12,12 +12,13 @@ import torch
 
 from . import _native
 from ._operands import (DTYPE_CODES, MOST_STRIDE, call, check_device, check_out, code_of, readable_rows, refuse_captured_backward,
-                        written)
+                        refuse_tangent, written)
 
 _OPERANDS = {torch.bfloat16: _native.BF16, torch.float16: _native.F16}
 
 
 def _check(what: str, weight: torch.Tensor | None, offsets: torch.Tensor, *rows: torch.Tensor) -> None:
+    refuse_tangent(what, weight, *rows)
     if offsets.dim() != 1 or offsets.dtype != torch.int32 or offsets.numel() < 1:
         raise ValueError(f"{what}: offsets are {offsets.dtype} {tuple(offsets.shape)}, not int32 [experts + 1]")
     dtype = rows[0].dtype
@@ -89,7 +90,8 @@ def grouped_linear(x: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor,
     """``y[t] = weight[e] @ x[t]`` for the expert ``e`` of row ``t``: ``[rows, out]`` in the type of ``x`` (bf16 or fp16).
 
     Rows of no expert (before ``offsets[0]``, from ``offsets[-1]`` on) are zeros, or left as they are in a given ``out``
-    (which may be fp32).  Sums are held in fp32.  Differentiable in ``x`` and ``weight`` (not with ``out``).
+    (which may be fp32).  Sums are held in fp32.  Differentiable in ``x`` and ``weight`` (in reverse mode; not with
+    ``out``).
     """
     _check("grouped_linear", weight, offsets, x)
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad):

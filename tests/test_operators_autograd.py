@@ -5,6 +5,7 @@ On the CPU a stand-in takes the place of the launch: everything asked for here h
 
 import pytest
 import torch
+import torch.autograd.forward_ad as fwd
 
 from etha_amd import embedding as embedding_module, experts as experts_module, int8 as int8_module
 from etha_amd.embedding import embedding, embedding_grad
@@ -30,7 +31,7 @@ class Operands:
         self.x, self.up, self.weight = zeros(6, 8).bfloat16(), zeros(6, 16).bfloat16(), zeros(2, 16, 8).bfloat16()
         self.offsets = torch.tensor([0, 2, 6], dtype=torch.int32, device=device)
         self.q, self.w = zeros(6, 8, dtype=torch.int8), zeros(16, 8, dtype=torch.int8)
-        self.row_scales, self.col_scales = zeros(6), zeros(16)
+        self.row_scales, self.col_scales, self.bias = zeros(6), zeros(16), zeros(16)
         self.zeros = zeros
 
 
@@ -85,3 +86,53 @@ def test_inference_tensors_are_written(device):
         buffer = o.zeros(6, 8)
         embedding(o.tokens, o.table, out=buffer)
     embedding(o.tokens, o.table, out=buffer)  # they count no versions
+
+
+# name -> (floating-point operands, the call on them); every one of them may carry a tangent
+DERIVATIVES = {
+    "embedding": (("table",), lambda o, t: embedding(o.tokens, t["table"])),
+    "embedding_grad": (("rows",), lambda o, t: embedding_grad(t["rows"], o.tokens, 5)),
+    "grouped_linear": (("x", "weight"), lambda o, t: grouped_linear(t["x"], t["weight"], o.offsets)),
+    "grouped_linear_grad_rows": (("up", "weight"), lambda o, t: grouped_linear_grad_rows(t["up"], t["weight"], o.offsets)),
+    "grouped_linear_grad_weight": (("up", "x"), lambda o, t: grouped_linear_grad_weight(t["up"], t["x"], o.offsets)),
+    "quantize_rows": (("rows",), lambda o, t: quantize_rows(t["rows"])),
+    "int8_matmul": (("row_scales", "col_scales", "bias"),
+                    lambda o, t: int8_matmul(o.q, t["row_scales"], o.w, t["col_scales"], bias=t["bias"])),
+    "int8_linear": (("rows", "col_scales", "bias"), lambda o, t: int8_linear(t["rows"], o.w, t["col_scales"], bias=t["bias"])),
+}
+OPERANDS = [(name, operand) for name, (operands, _) in DERIVATIVES.items() for operand in operands]
+
+
+def operands_of(o, name):
+    return {operand: getattr(o, operand) for operand in DERIVATIVES[name][0]}
+
+
+@pytest.mark.parametrize("name,operand", OPERANDS)
+def test_a_tangent_is_refused(device, name, operand):
+    """No call has a forward-mode derivative: one that dropped the tangent would stand for a derivative of zero."""
+    o = Operands(device)
+    call, given = DERIVATIVES[name][1], operands_of(Operands(device), name)
+    with fwd.dual_level():
+        call(o, given)  # a level alone is no trouble
+        quantize_rows(o.rows, values=o.q, scales=o.row_scales)
+        given[operand] = fwd.make_dual(given[operand], torch.ones_like(given[operand]))
+        with pytest.raises(RuntimeError, match=f"{name} has no forward-mode derivative"):
+            call(o, given)
+        with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):  # which does not switch tangents off
+            call(o, given)
+        if name in ("embedding", "grouped_linear"):  # nor does another operand's gradient
+            given[operand].requires_grad_()
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call(o, given)
+    with pytest.raises(RuntimeError):
+        torch.func.jvp(lambda t: call(o, {**operands_of(o, name), operand: t}), (getattr(o, operand),), (getattr(o, operand),))
+
+
+@pytest.mark.parametrize("name", WRITERS)
+def test_a_tangent_of_the_output_is_refused(device, name):
+    shape, write = WRITERS[name]
+    o = Operands(device)
+    with fwd.dual_level():
+        out = fwd.make_dual(o.zeros(*shape), o.zeros(*shape))
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            write(o, out)
