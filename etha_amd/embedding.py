@@ -12,7 +12,7 @@ import torch
 
 from . import _native
 from ._operands import (DTYPE_CODES, TOKEN_CODES, call, check_device, check_out, code_of, readable_rows, refuse_captured_backward,
-                        refuse_tangent, row_stride, written)
+                        refuse_grad, refuse_tangent, row_stride, written)
 
 
 def _token_operand(what: str, tokens: torch.Tensor) -> tuple[torch.Tensor, int]:
@@ -87,9 +87,10 @@ def embedding_grad(grad: torch.Tensor, tokens: torch.Tensor, n_rows: int, *, sca
 
     ``grad``: the gradient of the result, ``tokens.shape + (width,)``.  Rows without a token become zeros.  With ``out`` and
     ``accumulate=True`` the sums are added to ``out`` (micro-batches into one gradient) and rows without a token are not
-    touched.  The same inputs give the same bits.  The result is not part of a graph.
+    touched.  The same inputs give the same bits.  The result is not part of a graph, so a ``grad`` that requires a
+    gradient is refused.
     """
-    refuse_tangent("embedding_grad", grad)
+    refuse_grad("embedding_grad", grad)
     if grad.dim() != tokens.dim() + 1 or grad.shape[:-1] != tokens.shape:
         raise ValueError(f"embedding_grad: grad has shape {tuple(grad.shape)} for tokens of {tuple(tokens.shape)}")
     if n_rows < 0:

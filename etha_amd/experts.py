@@ -12,7 +12,7 @@ import torch
 
 from . import _native
 from ._operands import (DTYPE_CODES, MOST_STRIDE, call, check_device, check_out, code_of, readable_rows, refuse_captured_backward,
-                        refuse_tangent, written)
+                        refuse_grad, refuse_tangent, written)
 
 _OPERANDS = {torch.bfloat16: _native.BF16, torch.float16: _native.F16}
 
@@ -104,6 +104,7 @@ def grouped_linear(x: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor,
 def grouped_linear_grad_rows(grad: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor, *,
                              out: torch.Tensor | None = None) -> torch.Tensor:
     """Gradient of :func:`grouped_linear` with respect to ``x``: ``grad[t] @ weight[e]``; rows of no expert as there."""
+    refuse_grad("grouped_linear_grad_rows", grad, weight)
     _check("grouped_linear_grad_rows", weight, offsets, grad)
     return _product("grouped_linear_grad_rows", grad, weight, offsets, True, out)
 
@@ -113,6 +114,7 @@ def grouped_linear_grad_weight(grad: torch.Tensor, x: torch.Tensor, offsets: tor
     """Gradient of :func:`grouped_linear` with respect to ``weight``: ``grad[rows of e].T @ x[rows of e]`` for each expert, zeros
     for an expert without rows; in ``dtype`` (default: that of ``x``)."""
     what = "grouped_linear_grad_weight"
+    refuse_grad(what, grad, x)
     _check(what, None, offsets, grad, x)
     if grad.shape[0] != x.shape[0]:
         raise ValueError(f"{what}: {grad.shape[0]} rows of grad and {x.shape[0]} of x")
@@ -143,6 +145,8 @@ def grouped_linear_grad_weight(grad: torch.Tensor, x: torch.Tensor, offsets: tor
 def grouped_linear_grad(grad: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor, *,
                         weight_dtype: torch.dtype | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """Both gradients of :func:`grouped_linear`: of ``x``, and of ``weight`` in ``weight_dtype`` (default: the weight's).  Neither
-    is part of a graph."""
+    is part of a graph, so inputs that require a gradient are refused, as by either of the two: call them under
+    ``torch.no_grad()`` or detach their inputs."""
+    refuse_grad("grouped_linear_grad", grad, x, weight)
     return (grouped_linear_grad_rows(grad, weight, offsets),
             grouped_linear_grad_weight(grad, x, offsets, dtype=weight_dtype or weight.dtype))

@@ -9,7 +9,7 @@ import torch.autograd.forward_ad as fwd
 
 from etha_amd import embedding as embedding_module, experts as experts_module, int8 as int8_module
 from etha_amd.embedding import embedding, embedding_grad
-from etha_amd.experts import grouped_linear, grouped_linear_grad_rows, grouped_linear_grad_weight
+from etha_amd.experts import grouped_linear, grouped_linear_grad, grouped_linear_grad_rows, grouped_linear_grad_weight
 from etha_amd.int8 import Int8Weight, int8_linear, int8_matmul, quantize_rows
 
 
@@ -136,3 +136,26 @@ def test_a_tangent_of_the_output_is_refused(device, name):
         out = fwd.make_dual(o.zeros(*shape), o.zeros(*shape))
         with pytest.raises(RuntimeError, match="forward-mode"):
             write(o, out)
+
+
+@pytest.mark.parametrize("name,operand", [(n, t) for n, t in OPERANDS if n not in ("embedding", "grouped_linear")])
+def test_a_call_without_a_gradient_refuses_to_cut_a_graph(device, name, operand):
+    """One rule for all that have none, the gradient functions among them: operands come detached, or under no_grad."""
+    o = Operands(device)
+    call, given = DERIVATIVES[name][1], operands_of(o, name)
+    given[operand] = given[operand].clone().requires_grad_()
+    with pytest.raises(RuntimeError, match=f"{name} has no gradient"):
+        call(o, given)
+    with torch.no_grad():
+        call(o, given)
+    given[operand] = given[operand].detach()
+    call(o, given)
+
+
+def test_both_gradients_refuse_before_either_runs(device):
+    o = Operands(device)
+    for k in range(3):
+        operands = [o.up, o.x, o.weight]
+        operands[k] = operands[k].clone().requires_grad_()
+        with pytest.raises(RuntimeError, match="grouped_linear_grad has no gradient"):
+            grouped_linear_grad(*operands, o.offsets)
