@@ -14,7 +14,7 @@ import numpy as np
 from .build import LIB_PATH
 
 ETHA_MAX_NDIM = 8
-ABI_VERSION = 7
+ABI_VERSION = 8
 LAUNCH_UNORDERED = 1  # ETHA_LAUNCH_UNORDERED
 SEG_PACK, SEG_UNPACK, SEG_REDUCE_PACK, SEG_SELFCOPY = 0, 1, 2, 3  # ETHA_SEG_*
 MAX_SEGMENTS = 16
@@ -161,6 +161,8 @@ _SIGNATURES = {
     "etha_grouped_matmul_reduce_workspace": (c_int, [c_uint64, c_uint64, c_uint64, c_uint64, POINTER(c_uint64)]),
     "etha_grouped_matmul_reduce": (c_int, [c_void_p, c_void_p, c_uint32, c_uint64, c_int64, c_int64, c_uint64, c_uint64, c_uint64,
                                            c_void_p, c_void_p, c_uint32, c_int64, c_int64, c_void_p, c_uint64, c_void_p]),
+    "etha_product_kernel": (c_int, [c_uint32, c_uint32, c_void_p, c_int64, c_void_p, c_int64, c_int64, c_uint64, c_uint64, c_uint64,
+                                    c_uint64, POINTER(c_uint32), POINTER(c_int)]),
 }
 
 _lib = None
@@ -446,6 +448,19 @@ def grouped_matmul_reduce_workspace(rows: int, n_groups: int, out_rows: int, out
     _check("etha_grouped_matmul_reduce_workspace",
            lib().etha_grouped_matmul_reduce_workspace(rows, n_groups, out_rows, out_cols, byref(out)))
     return out.value
+
+
+PRODUCT_INT8, PRODUCT_ROWS, PRODUCT_ROWS_T, PRODUCT_REDUCE = 0, 1, 2, 3
+PRODUCT_KERNELS = ("short", "few 16", "few 32", "few 64", "tile 32", "tile 128", "tile 256")  # ETHA_PRODUCT_*
+
+
+def product_kernel(product: int, dtype: int, p: tuple, q: tuple, rows: int, cols: int, red: int, n_groups: int = 0) -> tuple[str, bool]:
+    """Kernel of a product of these sizes, and whether its operands go straight into LDS (see ``etha_product_kernel``);
+    ``p`` and ``q``: address, row stride and, for ``q``, group stride."""
+    kernel, direct = c_uint32(), c_int()
+    _check("etha_product_kernel", lib().etha_product_kernel(product, dtype, p[0], p[1], q[0], q[1], q[2] if len(q) > 2 else 0, rows, cols,
+                                                            red, n_groups, byref(kernel), byref(direct)))
+    return PRODUCT_KERNELS[kernel.value], bool(direct.value)
 
 
 def ipc_open(handle_bytes: bytes) -> int:

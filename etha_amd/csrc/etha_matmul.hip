@@ -975,11 +975,14 @@ uint64_t row_tiles_of(const MatmulArgs& a, uint32_t kind, int bm) {
   return (a.rows - groups) / bm + groups;
 }
 
+// Workgroups of a launch: with 512 work-items each, half of what a grid may have.
+constexpr uint64_t kMostBlocks = 1u << 22;
+
 template <typename E, uint32_t KIND, typename D, typename S, template <typename> class STAGE>
 int launch_matmul(const char* what, const MatmulArgs& a, void* stream) {
   const uint64_t row_tiles = row_tiles_of(a, KIND, S::BM);
   const uint64_t col_tiles = ((uint64_t)a.cols + S::BN - 1) / S::BN, blocks = row_tiles * col_tiles;
-  if (blocks >= 1ull << 22) return fail(ETHA_ERR_UNSUPPORTED, "%s: the product is too large for one call", what);
+  if (blocks >= kMostBlocks) return fail(ETHA_ERR_UNSUPPORTED, "%s: the product is too large for one call", what);
   if (!blocks) return ETHA_OK;
   hipLaunchKernelGGL((etha_matmul_kernel<E, KIND, D, S, STAGE>), dim3((uint32_t)blocks, a.splits > 1 ? a.splits : 1), dim3(S::kThreads), 0, (hipStream_t)stream, a);
   return launched("etha_matmul_kernel");
@@ -993,7 +996,7 @@ int launch_shape(const char* what, const MatmulArgs& a, bool direct, void* strea
 template <typename E, uint32_t KIND, typename D, typename SX, int MT>
 int launch_few(const char* what, const FewArgs& few, void* stream) {
   const uint64_t blocks = row_tiles_of(few.m, KIND, MT * 16) * (((uint64_t)few.m.cols + kFewCols - 1) / kFewCols);
-  if (blocks >= 1ull << 22) return fail(ETHA_ERR_UNSUPPORTED, "%s: the product is too large for one call", what);
+  if (blocks >= kMostBlocks) return fail(ETHA_ERR_UNSUPPORTED, "%s: the product is too large for one call", what);
   hipLaunchKernelGGL((etha_few_rows_kernel<E, KIND, D, SX, MT>), dim3((uint32_t)blocks), dim3(kFewThreads), 0, (hipStream_t)stream, few);
   return launched("etha_few_rows_kernel");
 }
@@ -1020,70 +1023,88 @@ double tile_cost(const MatmulArgs& a, uint32_t kind, int es, const TileCost& t) 
   return us;
 }
 
+// The kernel that a product takes (ETHA_PRODUCT_*).
+uint32_t choose_kernel(const MatmulArgs& a, uint32_t kind, int es, bool direct) {
+  const uint64_t p_row = (uint64_t)(kind == kGroupReduce ? a.rows : a.red) * es;
+  const uint64_t q_row = (uint64_t)(kind == kGroupReduce || kind == kGroupRowsT ? a.cols : a.red) * es;
+  if (!direct && (p_row < 16 || q_row < 16)) return ETHA_PRODUCT_SHORT;
+  if (kind == kGroupReduce) {
+    // the large tile wherever there are enough of them for every CU, also for few rows, where all there is to do is writing
+    // the results (16 rows, 8 x [3584, 4096]: 53 us, 63 us with the middle one)
+    const uint64_t tiles = row_tiles_of(a, kind, ShapeL::BM) * (((uint64_t)a.cols + ShapeL::BN - 1) / ShapeL::BN);
+    return a.splits < 2 && tiles >= 192 ? ETHA_PRODUCT_TILE_256 : ETHA_PRODUCT_TILE_128;
+  }
+  const double none = 1e30;
+  const bool few = kind != kGroupRowsT;
+  const TileCost shapes[6] = {
+      few ? TileCost{16, kFewCols, 512, 2, 11, 6000} : TileCost{16, kFewColsT, 512, 2, 7, 6000},
+      {32, kFewCols, 512, 2, 11, 6000},
+      {64, kFewCols, 256, 2, 11, 6000},
+      {ShapeS::BM, ShapeS::BN, 512, 3, 11, 4600},
+      {ShapeM::BM, ShapeM::BN, 512, 4, 11, 5200},
+      {ShapeL::BM, ShapeL::BN, 256, 8, 11, 4600},
+  };
+  static const uint32_t kernels[6] = {ETHA_PRODUCT_FEW_16, ETHA_PRODUCT_FEW_32, ETHA_PRODUCT_FEW_64,
+                                      ETHA_PRODUCT_TILE_32, ETHA_PRODUCT_TILE_128, ETHA_PRODUCT_TILE_256};
+  double cost[6];
+  for (int i = 0; i < 6; i++) {
+    cost[i] = tile_cost(a, kind, es, shapes[i]);
+    if (row_tiles_of(a, kind, shapes[i].bm) * (((uint64_t)a.cols + shapes[i].bn - 1) / shapes[i].bn) >= kMostBlocks)
+      cost[i] += none;  // more than a launch takes: only if no shape fits, which the launch then refuses
+  }
+  if (!few) cost[1] = cost[2] = 2 * none;
+  if (!few && (p_row < 16 || q_row < 16)) cost[0] = 2 * none;  // its loads begin 16 bytes before the end of a row
+  int best = 0;
+  for (int i = 1; i < 6; i++)
+    if (cost[i] < cost[best]) best = i;
+  return kernels[best];
+}
+
 template <typename E, uint32_t KIND, typename D>
 int shaped_matmul(const char* what, const MatmulArgs& a, bool direct, void* stream) {
-  const uint64_t p_row = (uint64_t)(KIND == kGroupReduce ? a.rows : a.red) * E::kEs;
-  const uint64_t q_row = (uint64_t)(KIND == kGroupReduce || KIND == kGroupRowsT ? a.cols : a.red) * E::kEs;
-  if (!direct && (p_row < 16 || q_row < 16)) {
+  const uint32_t kernel = choose_kernel(a, KIND, E::kEs, direct);
+  if (kernel == ETHA_PRODUCT_SHORT) {
     const uint64_t blocks = ((KIND == kGroupReduce ? a.n_groups : 1ull) * a.rows * a.cols + 255) / 256;
     hipLaunchKernelGGL((etha_matmul_short_kernel<E, KIND, D>), dim3((uint32_t)(blocks < 1u << 20 ? blocks : 1u << 20)), dim3(256), 0,
                        (hipStream_t)stream, a);
     return launched("etha_matmul_short_kernel");
   }
+  if (kernel == ETHA_PRODUCT_TILE_256) return launch_shape<E, KIND, D, ShapeL>(what, a, direct, stream);
   if constexpr (KIND == kGroupReduce) {
-    // the large tile wherever there are enough of them for every CU, also for few rows, where all there is to do is writing
-    // the results (16 rows, 8 x [3584, 4096]: 53 us, 63 us with the middle one)
-    const uint64_t tiles = row_tiles_of(a, KIND, ShapeL::BM) * (((uint64_t)a.cols + ShapeL::BN - 1) / ShapeL::BN);
-    if (a.splits < 2 && tiles >= 192) return launch_shape<E, KIND, D, ShapeL>(what, a, direct, stream);
     return launch_shape<E, KIND, D, ShapeM>(what, a, direct, stream);
   } else {
-    double cost[6];
-    const double none = 1e30;
-    constexpr bool few = KIND != kGroupRowsT;
-    const TileCost shapes[6] = {
-        few ? TileCost{16, kFewCols, 512, 2, 11, 6000} : TileCost{16, kFewColsT, 512, 2, 7, 6000},
-        {32, kFewCols, 512, 2, 11, 6000},
-        {64, kFewCols, 256, 2, 11, 6000},
-        {ShapeS::BM, ShapeS::BN, 512, 3, 11, 4600},
-        {ShapeM::BM, ShapeM::BN, 512, 4, 11, 5200},
-        {ShapeL::BM, ShapeL::BN, 256, 8, 11, 4600},
-    };
-    for (int i = 0; i < 6; i++) cost[i] = tile_cost(a, KIND, E::kEs, shapes[i]);
-    if (!few) cost[1] = cost[2] = none;
-    if (!few && (p_row < 16 || q_row < 16)) cost[0] = none;  // its loads begin 16 bytes before the end of a row
-    int best = 0;
-    for (int i = 1; i < 6; i++)
-      if (cost[i] < cost[best]) best = i;
-    if constexpr (few) {
+    if constexpr (KIND != kGroupRowsT) {
       FewArgs args = {};
       args.m = a;
-      if (best == 0) return launch_few<E, KIND, D, void, 1>(what, args, stream);
-      if (best == 1) return launch_few<E, KIND, D, void, 2>(what, args, stream);
-      if (best == 2) return launch_few<E, KIND, D, void, 4>(what, args, stream);
-    }
-    if constexpr (KIND == kGroupRowsT) {
-      if (best == 0) {
+      if (kernel == ETHA_PRODUCT_FEW_16) return launch_few<E, KIND, D, void, 1>(what, args, stream);
+      if (kernel == ETHA_PRODUCT_FEW_32) return launch_few<E, KIND, D, void, 2>(what, args, stream);
+      if (kernel == ETHA_PRODUCT_FEW_64) return launch_few<E, KIND, D, void, 4>(what, args, stream);
+    } else {
+      if (kernel == ETHA_PRODUCT_FEW_16) {
         const uint64_t blocks = row_tiles_of(a, KIND, 16) * (((uint64_t)a.cols + kFewColsT - 1) / kFewColsT);
-        if (blocks >= 1ull << 22) return fail(ETHA_ERR_UNSUPPORTED, "%s: the product is too large for one call", what);
+        if (blocks >= kMostBlocks) return fail(ETHA_ERR_UNSUPPORTED, "%s: the product is too large for one call", what);
         hipLaunchKernelGGL((etha_few_rows_transposed_kernel<E, D>), dim3((uint32_t)blocks), dim3(kFewThreads), 0, (hipStream_t)stream, a);
         return launched("etha_few_rows_transposed_kernel");
       }
     }
-    if (best == 5) return launch_shape<E, KIND, D, ShapeL>(what, a, direct, stream);
-    if (best == 4) return launch_shape<E, KIND, D, ShapeM>(what, a, direct, stream);
+    if (kernel == ETHA_PRODUCT_TILE_128) return launch_shape<E, KIND, D, ShapeM>(what, a, direct, stream);
     return launch_shape<E, KIND, D, ShapeS>(what, a, direct, stream);
   }
 }
 
+bool takes_direct(const MatmulArgs& a, uint32_t kind, int es) {
+  const uint64_t k_bytes = (uint64_t)a.red * es;
+  return is_direct(a.p, a.p_stride, 0, k_bytes, kind == kGroupReduce, a.rows) &&
+         is_direct(a.q, a.q_stride, a.q_group_stride, k_bytes, kind == kGroupReduce || kind == kGroupRowsT, a.cols);
+}
+
 template <typename E, uint32_t KIND>
 int run_matmul(const char* what, const MatmulArgs& a, uint32_t out_dtype, void* stream) {
-  constexpr bool kTransP = KIND == kGroupReduce, kTransQ = KIND == kGroupReduce || KIND == kGroupRowsT;
   if (a.p_stride < 0 || a.q_stride < 0 || a.p_stride > kMostStride || a.q_stride > kMostStride)
     return fail(ETHA_ERR_UNSUPPORTED, "%s: rows have to lie at most %u bytes apart", what, kMostStride);
   const uint64_t k_bytes = (uint64_t)a.red * E::kEs;
   if (KIND != kGroupReduce && k_bytes > 1u << 30) return fail(ETHA_ERR_UNSUPPORTED, "%s: sums over at most 2^30 bytes of a row", what);
-  const bool direct = is_direct(a.p, a.p_stride, 0, k_bytes, kTransP, a.rows) &&
-                      is_direct(a.q, a.q_stride, a.q_group_stride, k_bytes, kTransQ, a.cols);
+  const bool direct = takes_direct(a, KIND, E::kEs);
   if (out_dtype == ETHA_F32) return shaped_matmul<E, KIND, F32>(what, a, direct, stream);
   if (out_dtype == ETHA_BF16) return shaped_matmul<E, KIND, BF16>(what, a, direct, stream);
   return shaped_matmul<E, KIND, F16>(what, a, direct, stream);
@@ -1098,7 +1119,7 @@ bool is_out(uint32_t dtype) { return dtype == ETHA_F32 || dtype == ETHA_BF16 || 
 // always is (14336 x 4096: 14.4 us, 16.5 us).
 bool is_few(uint64_t rows, uint64_t cols, uint64_t width) {
   const uint64_t padded = (width + 127) / 128 * 128;
-  if (rows > kFewConverted || rows * padded > kFewLds) return false;
+  if (rows > kFewConverted || rows * padded > kFewLds || (cols + kFewCols - 1) / kFewCols >= kMostBlocks) return false;
   return rows == 1 || (rows * padded * ((cols + 4095) / 4096) <= kFewLds && (cols <= 8192 || padded <= 1024) &&
                        (rows <= kFewTogether || padded <= 2048));
 }
@@ -1155,6 +1176,32 @@ int etha_int8_matmul(const int8_t* x, const float* x_scale, uint64_t rows, int64
   a.col_scale = w_scale;
   a.bias = bias;
   return run_matmul<ElemI8, kPlain>("etha_int8_matmul", a, out_dtype, stream);
+}
+
+int etha_product_kernel(uint32_t product, uint32_t dtype, const void* p, int64_t p_stride, const void* q, int64_t q_stride,
+                        int64_t q_group_stride, uint64_t rows, uint64_t cols, uint64_t red, uint64_t n_groups, uint32_t* kernel,
+                        int* direct) {
+  if (!kernel || !direct) return fail(ETHA_ERR_INVALID, "etha_product_kernel: null result");
+  if (product > kGroupReduce || (product == kPlain ? dtype != ETHA_I8 : dtype != ETHA_BF16 && dtype != ETHA_F16))
+    return fail(ETHA_ERR_INVALID, "etha_product_kernel: no such product");
+  const int rc = check_sizes("etha_product_kernel", rows, cols, red, (1ull << 31) - 1);
+  if (rc != ETHA_OK) return rc;
+  if (n_groups > 1u << 16 || !rows || !cols) return fail(ETHA_ERR_INVALID, "etha_product_kernel: nothing is launched for these sizes");
+  const int es = product == kPlain ? 1 : 2;
+  MatmulArgs a = {};
+  a.p = (const char*)p;
+  a.q = (const char*)q;
+  a.p_stride = p_stride * es;
+  a.q_stride = q_stride * es;
+  a.q_group_stride = q_group_stride * es;
+  a.rows = (uint32_t)rows;
+  a.cols = (uint32_t)cols;
+  a.red = (uint32_t)red;
+  a.n_groups = (uint32_t)n_groups;
+  if (product == kGroupReduce) a.splits = reduce_splits(red, n_groups, rows, cols);
+  *direct = takes_direct(a, product, es);
+  *kernel = choose_kernel(a, product, es, *direct != 0);
+  return ETHA_OK;
 }
 
 int etha_int8_linear_workspace(uint64_t rows, uint64_t cols, uint64_t width, uint64_t* bytes) {

@@ -32,7 +32,7 @@
 extern "C" {
 #endif
 
-#define ETHA_ABI_VERSION 7
+#define ETHA_ABI_VERSION 8
 #define ETHA_MAX_NDIM 8
 
 /* status codes */
@@ -400,6 +400,22 @@ int etha_grouped_matmul_reduce(const void* grad, const void* x, uint32_t dtype, 
                                uint64_t n_groups, uint64_t out_rows, uint64_t out_cols, const int32_t* offsets, void* out,
                                uint32_t out_dtype, int64_t out_stride, int64_t out_group_stride, void* workspace,
                                uint64_t workspace_bytes, void* stream);
+
+/*
+ * For inspection: the kernel that a product of these sizes takes, and whether its operands go straight into LDS.  `product`
+ * is 0 for etha_int8_matmul, 1 and 2 for etha_grouped_matmul (w as it lies, w transposed), 3 for etha_grouped_matmul_reduce,
+ * whose out_rows, out_cols and rows are rows, cols and red here.  p and q are the operands' addresses, which are not read.
+ */
+#define ETHA_PRODUCT_SHORT 0u    /* rows shorter than 16 bytes: a work-item an element */
+#define ETHA_PRODUCT_FEW_16 1u   /* a few rows against the matrices, 16, 32 or 64 at a time */
+#define ETHA_PRODUCT_FEW_32 2u
+#define ETHA_PRODUCT_FEW_64 3u
+#define ETHA_PRODUCT_TILE_32 4u  /* tiles of 32 x 64, 128 x 128, 256 x 256 */
+#define ETHA_PRODUCT_TILE_128 5u
+#define ETHA_PRODUCT_TILE_256 6u
+int etha_product_kernel(uint32_t product, uint32_t dtype, const void* p, int64_t p_stride, const void* q, int64_t q_stride,
+                        int64_t q_group_stride, uint64_t rows, uint64_t cols, uint64_t red, uint64_t n_groups, uint32_t* kernel,
+                        int* direct);
 
 #ifdef __cplusplus
 }
