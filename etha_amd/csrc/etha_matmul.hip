@@ -199,8 +199,11 @@ struct Operand {
 __device__ inline uint32_t lds_address(const char* p) { return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) char*)p; }
 
 // Straight from memory into LDS, 16 bytes a lane: for operands whose rows start at 16-byte addresses and, k-contiguous
-// ones, hold whole 16-byte pieces of k.  The buffer descriptor ends with the operand tile's last byte, so that whatever
-// the tile reaches over reads as zero.  The loads write no registers; the kernel waits for them by count.
+// ones, hold whole 16-byte pieces of k.  The buffer descriptor ends with the operand tile's last word, so that whatever
+// the tile reaches over reads as zero.  It has to be the whole word: memory is checked against the end word by word, and of
+// one that lies across it nothing arrives, the last element of an odd width among it.  The other half of that word lies in
+// the same 16 bytes of memory, and belongs to a column whose results are dropped.  The loads write no registers; the kernel
+// waits for them by count.
 template <typename OP>
 struct DirectStage {
   static constexpr bool kDirect = true;
@@ -216,6 +219,7 @@ struct DirectStage {
     stride = (uint32_t)row_stride;
     left = OP::kTrans ? (int64_t)((int)red - 1) * row_stride + (int64_t)n_rows * 2
                       : (int64_t)((int)n_rows - 1) * row_stride + (int64_t)red * OP::kEs;
+    left = (left + 3) & ~(int64_t)3;
     #pragma unroll
     for (int i = 0; i < OP::kPer; i++) {
       const uint32_t slot = threadIdx.x + i * OP::kThreads;

@@ -192,3 +192,15 @@ def test_a_product_of_very_many_rows_or_columns(gpu_device, rows, cols):
             check_product(got[part], x[part], xs[part], w, ws, None)
         else:
             check_product(got[:, part], x, xs, w[part], ws[part], None)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("over", range(1, 8))
+@pytest.mark.parametrize("product,kernel,rows,cols,red,experts", [c for c in CASES if c[0] >= nat.PRODUCT_ROWS_T and c[1] != "few 16"])
+def test_widths_that_are_no_whole_pieces(gpu_device, product, kernel, rows, cols, red, experts, over):
+    """Operands that lie transposed go straight into LDS also where their rows end within a piece of 16 bytes, or within 4:
+    the last row's last piece reaches over the operand's end."""
+    gen = torch.Generator(device=gpu_device).manual_seed(over)
+    rows = rows // 8 * 8 + over if product == nat.PRODUCT_REDUCE else rows
+    cols = cols // 8 * 8 + over
+    check_values(gen, gpu_device, product, kernel, rows, cols, red, experts, torch.bfloat16, lambda n: ceil_to(n, 8), 0, True)
