@@ -242,10 +242,15 @@ struct DirectStage {
     base += step;
     left -= step;
   }
+  // m0, where the load's place in LDS stands, is named as written: nothing else in these kernels uses it, and whatever a
+  // compiler may make of them has to set it anew.  (The warning is about registers that are not kept across the statement.)
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
   __device__ void part(int i) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
-                 :: "s"(to + i * OP::kThreads * 16), "v"(at[i] | outside), "s"(rsrc) : "memory");
+                 :: "s"(to + i * OP::kThreads * 16), "v"(at[i] | outside), "s"(rsrc) : "memory", "m0");
   }
+#pragma clang diagnostic pop
 };
 
 // n bytes (0 to 16) dropped at the low end, zeros in at the high end
