@@ -215,7 +215,7 @@ struct GradArgs {
   float* partial;        // [chunk][2][width]
   uint64_t n, width;
   int64_t grad_stride, out_stride;
-  uint32_t n_rows, chunk, n_chunks, n_cols, sum_blocks;
+  uint32_t n_rows, chunk, n_chunks, n_cols, sum_blocks, zero_blocks;
   uint32_t accumulate;
   float scale;
 };
@@ -293,16 +293,17 @@ __global__ __launch_bounds__(kGradWaves* kWave) void etha_embedding_grad_kernel(
   constexpr int N = grad_vec<S>();
   const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   if (blockIdx.x >= a.sum_blocks) {  // rows without a token
-    const uint64_t row0 = (uint64_t)(blockIdx.x - a.sum_blocks) * kZeroRows;
-    const bool empty = lane < kZeroRows && row0 + lane < a.n_rows && !a.used[row0 + lane];
-    uint64_t todo = __ballot(empty);
-    constexpr int M = 16 / (int)sizeof(typename D::bits);
-    const float zero[M] = {};
-    for (uint32_t r = wave; r < kZeroRows; r += kGradWaves)
-      if ((todo >> r) & 1) {
-        typename D::bits* p = (typename D::bits*)a.out + (int64_t)(row0 + r) * a.out_stride;
-        for (uint64_t c = lane * M; c < a.width; c += 64 * M) store_f32<D, M, true>(p + c, zero, (int64_t)(a.width - c));
-      }
+    for (uint64_t row0 = (uint64_t)(blockIdx.x - a.sum_blocks) * kZeroRows; row0 < a.n_rows; row0 += (uint64_t)a.zero_blocks * kZeroRows) {
+      const bool empty = lane < kZeroRows && row0 + lane < a.n_rows && !a.used[row0 + lane];
+      uint64_t todo = __ballot(empty);
+      constexpr int M = 16 / (int)sizeof(typename D::bits);
+      const float zero[M] = {};
+      for (uint32_t r = wave; r < kZeroRows; r += kGradWaves)
+        if ((todo >> r) & 1) {
+          typename D::bits* p = (typename D::bits*)a.out + (int64_t)(row0 + r) * a.out_stride;
+          for (uint64_t c = lane * M; c < a.width; c += 64 * M) store_f32<D, M, true>(p + c, zero, (int64_t)(a.width - c));
+        }
+    }
     return;
   }
   const uint64_t unit = (uint64_t)blockIdx.x * kGradWaves + wave;
@@ -347,8 +348,9 @@ __global__ __launch_bounds__(kGradWaves* kWave) void etha_embedding_grad_kernel(
   else write_row<D, N>(a, cur, c, acc);
 }
 
-// Few tokens: no sort and one launch.  A workgroup owns 16 rows and 64 vectors of columns; each wave picks the places of
-// its 4 rows' tokens out of all tokens, in their order, and adds their rows up.
+// Few tokens: no sort and one launch.  A workgroup owns 16 rows (and further ones where there are more than a grid takes) and
+// 64 vectors of columns; each wave picks the places of its 4 rows' tokens out of all tokens, in their order, and adds their
+// rows up.
 constexpr uint32_t kFewTokens = 512, kFewTokenRows = 4;
 
 struct FewGradArgs {
@@ -365,40 +367,41 @@ __global__ __launch_bounds__(kGradWaves* kWave) void etha_embedding_grad_few_ker
   const GradArgs& a = few.g;
   __shared__ uint16_t s_list[kGradWaves][kFewTokenRows][kFewTokens];
   const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const uint32_t row0 = (blockIdx.x * kGradWaves + wave) * kFewTokenRows;
   const Columns<N> c(((uint64_t)blockIdx.y * 64 + lane) * N, a.width);
   uint32_t row[kSteps];
   #pragma unroll
   for (uint32_t i = 0; i < kSteps; i++) row[i] = i * 64 + lane < a.n ? local_row(few.tokens, few.wide, i * 64 + lane, few.first, a.n_rows) : a.n_rows;
-  uint32_t count[kFewTokenRows] = {};
-  #pragma unroll
-  for (uint32_t i = 0; i < kSteps; i++) {
-    if (i * 64 >= a.n) break;
+  for (uint32_t row0 = (blockIdx.x * kGradWaves + wave) * kFewTokenRows; row0 < a.n_rows; row0 += gridDim.x * (kGradWaves * kFewTokenRows)) {
+    uint32_t count[kFewTokenRows] = {};
     #pragma unroll
-    for (uint32_t r = 0; r < kFewTokenRows; r++) {
-      const bool mine = row[i] == row0 + r && row[i] < a.n_rows;
-      const uint64_t mask = __ballot(mine);
-      if (mine) s_list[wave][r][count[r] + __popcll(mask & ((1ull << lane) - 1))] = (uint16_t)(i * 64 + lane);
-      count[r] += (uint32_t)__popcll(mask);
-    }
-  }
-  #pragma unroll
-  for (uint32_t r = 0; r < kFewTokenRows; r++) {
-    if (row0 + r >= a.n_rows || (a.accumulate && !count[r])) continue;
-    float acc[N] = {};
-    for (uint32_t i = 0; i < count[r]; i += kFewAhead) {
-      u32x4 raw[kFewAhead];
-      load_rows<S, N>(raw, a, c, count[r] - i, [&](uint32_t u) { return (uint32_t)s_list[wave][r][i + u]; });
+    for (uint32_t i = 0; i < kSteps; i++) {
+      if (i * 64 >= a.n) break;
       #pragma unroll
-      for (uint32_t u = 0; u < kFewAhead; u++) {
-        if (i + u >= count[r]) break;
-        float v[N];
-        raw_to_f32<S>(v, raw[u]);
-        #pragma unroll
-        for (int e = 0; e < N; e++) acc[e] += v[e];
+      for (uint32_t r = 0; r < kFewTokenRows; r++) {
+        const bool mine = row[i] == row0 + r && row[i] < a.n_rows;
+        const uint64_t mask = __ballot(mine);
+        if (mine) s_list[wave][r][count[r] + __popcll(mask & ((1ull << lane) - 1))] = (uint16_t)(i * 64 + lane);
+        count[r] += (uint32_t)__popcll(mask);
       }
     }
-    write_row<D, N>(a, row0 + r, c, acc);
+    #pragma unroll
+    for (uint32_t r = 0; r < kFewTokenRows; r++) {
+      if (row0 + r >= a.n_rows || (a.accumulate && !count[r])) continue;
+      float acc[N] = {};
+      for (uint32_t i = 0; i < count[r]; i += kFewAhead) {
+        u32x4 raw[kFewAhead];
+        load_rows<S, N>(raw, a, c, count[r] - i, [&](uint32_t u) { return (uint32_t)s_list[wave][r][i + u]; });
+        #pragma unroll
+        for (uint32_t u = 0; u < kFewAhead; u++) {
+          if (i + u >= count[r]) break;
+          float v[N];
+          raw_to_f32<S>(v, raw[u]);
+          #pragma unroll
+          for (int e = 0; e < N; e++) acc[e] += v[e];
+        }
+      }
+      write_row<D, N>(a, row0 + r, c, acc);
+    }
   }
 }
 
@@ -572,6 +575,9 @@ int check_gradient_tokens(const char* what, uint64_t n_tokens, uint64_t n_rows) 
   return ETHA_OK;
 }
 
+// Workgroups that sum, and that write rows of zeros: with 256 work-items each, together in a grid of fewer than 2^32.
+constexpr uint32_t kMostGradBlocks = 1u << 23;
+
 // Column blocks, chunk length and workspace of a gradient call: a rule on sizes alone.
 struct GradPlan {
   uint32_t n_cols, chunk, n_chunks;
@@ -696,8 +702,9 @@ int etha_embedding_grad(const void* grad, uint32_t grad_dtype, int64_t grad_stri
   if (n_tokens <= kFewTokens) {
     const FewGradArgs few = {g, tokens, first_row, token_dtype == ETHA_I64};
     const uint64_t per = 64 * (16 / es);
-    const dim3 grid((uint32_t)((n_rows + kGradWaves * kFewTokenRows - 1) / (kGradWaves * kFewTokenRows)), (uint32_t)((width + per - 1) / per));
-    if (grid.x >= 1u << 24 || grid.y > 65535) return fail(ETHA_ERR_UNSUPPORTED, "etha_embedding_grad: too many rows or columns");
+    dim3 grid((uint32_t)((n_rows + kGradWaves * kFewTokenRows - 1) / (kGradWaves * kFewTokenRows)), (uint32_t)((width + per - 1) / per));
+    if (grid.y > 65535) return fail(ETHA_ERR_UNSUPPORTED, "etha_embedding_grad: too many columns");
+    if (grid.x > kMostGradBlocks) grid.x = kMostGradBlocks;  // which then go round
     with_type(grad_dtype, [&](auto s) {
       with_type(out_dtype, [&](auto d) {
         hipLaunchKernelGGL((etha_embedding_grad_few_kernel<decltype(s), decltype(d)>), grid, dim3(kGradWaves * kWave), 0,
@@ -725,14 +732,14 @@ int etha_embedding_grad(const void* grad, uint32_t grad_dtype, int64_t grad_stri
     g.n_chunks = p.n_chunks;
     g.n_cols = p.n_cols;
     const uint64_t blocks = ((uint64_t)p.n_chunks * p.n_cols + kGradWaves - 1) / kGradWaves;
-    if (blocks > 1u << 23) return fail(ETHA_ERR_UNSUPPORTED, "etha_embedding_grad: too many tokens for this width");
+    if (blocks > kMostGradBlocks) return fail(ETHA_ERR_UNSUPPORTED, "etha_embedding_grad: too many tokens for this width");
     g.sum_blocks = (uint32_t)blocks;
   }
   const uint64_t zero_blocks = accumulate ? 0 : (n_rows + kZeroRows - 1) / kZeroRows;
-  if (g.sum_blocks + zero_blocks >= 1u << 24) return fail(ETHA_ERR_UNSUPPORTED, "etha_embedding_grad: too many rows");
+  g.zero_blocks = (uint32_t)(zero_blocks < kMostGradBlocks ? zero_blocks : kMostGradBlocks - 1);  // which then go round
   with_type(grad_dtype, [&](auto s) {
     with_type(out_dtype, [&](auto d) {
-      hipLaunchKernelGGL((etha_embedding_grad_kernel<decltype(s), decltype(d)>), dim3((uint32_t)(g.sum_blocks + zero_blocks)),
+      hipLaunchKernelGGL((etha_embedding_grad_kernel<decltype(s), decltype(d)>), dim3(g.sum_blocks + g.zero_blocks),
                          dim3(kGradWaves * kWave), 0, (hipStream_t)stream, g);
     });
   });

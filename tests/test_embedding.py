@@ -362,3 +362,22 @@ def test_captured_backward_is_refused(gpu_device):
         x.add_(1)
     graph.replay()
     refuse_captured_backward("embedding")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tokens,rows,width,dtype", [(700, (1 << 26) + 5, 1, torch.float32), (40, (1 << 28) + 21, 2, torch.bfloat16)])
+def test_gradient_of_more_rows_than_a_grid_takes(gpu_device, tokens, rows, width, dtype):
+    gen = torch.Generator(device=gpu_device).manual_seed(rows)
+    ids = torch.randint(0, rows, (tokens,), generator=gen, device=gpu_device)
+    ids[:4] = torch.tensor([0, rows - 1, rows - 1, rows // 2], device=gpu_device)
+    grad = (torch.rand(tokens, width, generator=gen, device=gpu_device) + 1).to(dtype)
+    out = torch.full((rows, width), 3.0, dtype=dtype, device=gpu_device)
+    embedding_grad(grad, ids, rows, out=out)
+    there = ids.unique()
+    assert int((out != 0).any(1).sum()) == there.numel()  # all others are zeros
+    small = torch.searchsorted(there, ids)
+    check_gradient(out[there], grad, small, there.numel(), 1.0, 0)
+    before = out[there].clone()
+    embedding_grad(grad, ids, rows, out=out, accumulate=True)
+    assert int((out != 0).any(1).sum()) == there.numel()
+    check_gradient(out[there], grad, small, there.numel(), 1.0, 0, before=before)
