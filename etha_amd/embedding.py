@@ -8,6 +8,8 @@ collapses.  :func:`embedding_grad` is the gradient of that shard: each row's tok
 
 from __future__ import annotations
 
+import operator
+
 import torch
 
 from . import _native
@@ -20,6 +22,13 @@ def _token_operand(what: str, tokens: torch.Tensor) -> tuple[torch.Tensor, int]:
     if code is None:
         raise ValueError(f"{what}: tokens are {tokens.dtype}; int32 and int64 are supported")
     return (tokens if tokens.is_contiguous() else tokens.contiguous()), code
+
+
+def _first_row(what: str, first_row) -> int:
+    first_row = operator.index(first_row)
+    if not -(1 << 63) <= first_row < 1 << 63:
+        raise ValueError(f"{what}: first_row {first_row} has more than 64 bits")
+    return first_row
 
 
 def _lookup(tokens, weight, scale, first_row, dtype, out):
@@ -77,8 +86,8 @@ def embedding(tokens: torch.Tensor, weight: torch.Tensor, *, scale: float = 1.0,
     if weight.requires_grad and torch.is_grad_enabled():
         if out is not None:
             raise ValueError("embedding: out cannot be given where weight requires a gradient")
-        return _Embedding.apply(tokens, weight, float(scale), int(first_row), dtype)
-    return _lookup(tokens, weight, scale, first_row, dtype, out)
+        return _Embedding.apply(tokens, weight, float(scale), _first_row("embedding", first_row), dtype)
+    return _lookup(tokens, weight, float(scale), _first_row("embedding", first_row), dtype, out)
 
 
 def embedding_grad(grad: torch.Tensor, tokens: torch.Tensor, n_rows: int, *, scale: float = 1.0, first_row: int = 0,
@@ -97,6 +106,7 @@ def embedding_grad(grad: torch.Tensor, tokens: torch.Tensor, n_rows: int, *, sca
         raise ValueError(f"embedding_grad: {n_rows} rows")
     if accumulate and out is None:
         raise ValueError("embedding_grad: accumulate needs an out")
+    scale, first_row = float(scale), _first_row("embedding_grad", first_row)
     width, n_tokens = grad.shape[-1], tokens.numel()
     grad_code = code_of("embedding_grad", grad.dtype)
     grad, grad_stride = readable_rows(grad)

@@ -5,6 +5,7 @@ some grouping: each of its n additions rounds a partial sum that is at most A = 
 products with scale and the value added to (accumulate) add one rounding of 2^-24 each, the result's type half a step.
 """
 
+import numpy as np
 import pytest
 import torch
 
@@ -381,3 +382,29 @@ def test_gradient_of_more_rows_than_a_grid_takes(gpu_device, tokens, rows, width
     embedding_grad(grad, ids, rows, out=out, accumulate=True)
     assert int((out != 0).any(1).sum()) == there.numel()
     check_gradient(out[there], grad, small, there.numel(), 1.0, 0, before=before)
+
+
+@pytest.mark.parametrize("graph", [False, True])
+def test_scale_and_first_row_of_any_number_type(monkeypatch, graph):
+    """The same numbers are taken with and without a graph, and none is wrapped around."""
+    from etha_amd import embedding as module
+
+    seen = []
+    monkeypatch.setattr(module, "check_device", lambda what, first, *others: 0)
+    monkeypatch.setattr(module, "call", lambda index, name, *args: seen.append(args))
+    weight, tokens = torch.zeros(8, 4).requires_grad_(graph), torch.zeros(3, dtype=torch.int64)
+    for scale in (2.0, 2, np.float32(2), np.float64(2), torch.tensor(2.0)):
+        for first in (3, np.int64(3), torch.tensor(3)):
+            embedding(tokens, weight, scale=scale, first_row=first)
+            embedding_grad(torch.zeros(3, 4), tokens, 8, scale=scale, first_row=first)
+    for args in seen:
+        first, scale = (args[8], args[9])
+        assert type(first) is int and type(scale) is float and (first, scale) == (3, 2.0)
+    for call in (lambda **k: embedding(tokens, weight, **k), lambda **k: embedding_grad(torch.zeros(3, 4), tokens, 8, **k)):
+        call(first_row=-2 ** 63)
+        call(first_row=2 ** 63 - 1)
+        for first in (2 ** 63, -2 ** 63 - 1, 2 ** 64):
+            with pytest.raises(ValueError, match="first_row"):
+                call(first_row=first)
+        with pytest.raises(TypeError):
+            call(first_row=1.5)
