@@ -77,10 +77,11 @@ __global__ __launch_bounds__(256) void etha_embedding_kernel(const LookupArgs a)
 // a workgroup owns every 2^groups_log2-th row (frequent tokens lie close together) and looks through all tokens, a wave
 // through a run of them.  It counts those of each of its rows, wave by wave, and those of the workgroups before it, which
 // says where its own begin, and notes which they are; then every wave puts its tokens where the counts say.  Lanes whose
-// tokens have the same row find each other with one ballot per bit.  What bounds it is the looking, some 10 instructions for
-// 64 tokens: 57984 tokens of 21716 rows 20 us, 6965 of 6676 rows 7 us (a radix sort of two passes, with four launches, took
-// 29 us and the gaps between them; one in a single workgroup 17 us for the latter; runs of rows instead of every 256th, with
-// the tokens looked through twice, 57 us for the former).
+// tokens have the same row find each other with one ballot per bit.  57984 tokens of 21716 rows 20 us, 6965 of 6676 rows 7 us
+// (a radix sort of two passes, with four launches, took 29 us and the gaps between them; one in a single workgroup 17 us for
+// the latter; runs of rows instead of every 256th, with the tokens looked through twice, 57 us for the former).  The looking,
+// some 10 instructions for 64 tokens, would take about 4 of those 20 us; how the rest is shared by clearing, scans and placing
+// has not been measured.
 constexpr uint32_t kSortThreads = 1024, kSortWaves = kSortThreads / kWave, kSortNoted = 1024;
 constexpr int kSortBinsLog2 = 10;
 constexpr int kSortGroupsLog2 = 8;
@@ -253,7 +254,8 @@ __device__ inline void load_rows(u32x4 (&raw)[K], const GradArgs& a, const Colum
 
 // Stored through the caches, unlike the rows of zeros: a wave here writes 1 KB of one row, its neighbours the rest at other
 // times, and the lines are put together in L2 (65536 tokens of 4096 into 128256 rows 321 us, 343 us around the caches; 4 tokens
-// into 20480 x 2809 fp32 34 us, 70 us).
+// into 20480 x 2809 fp32 34 us, 70 us).  (These and the following figures: calls with one set of inputs, over and over; the
+// first of them takes 334 us where the inputs change from call to call.)
 template <typename D, int N>
 __device__ inline void write_row(const GradArgs& a, uint32_t row, const Columns<N>& c, float (&acc)[N]) {
   if (!c.inside) return;
@@ -591,7 +593,10 @@ GradPlan grad_plan(uint64_t n, uint64_t n_rows, uint64_t width, int es) {
   p.n_cols = (uint32_t)((width + per - 1) / per);
   // chunks of 128 places, shorter while there would be fewer waves than the chip holds a few of per SIMD (16 places where that
   // is still less than two waves a SIMD: 6965 tokens of 76 columns 23 us, 28 us with 32; 57984 of 128 columns 56 us, 48 us with
-  // 32), longer where the pieces of rows that cross chunks would need more than 2048 places in the workspace
+  // 32); such chunks make fewer than 8192 waves, so their pieces need at most 32 MB of workspace.  Chunks of 128 get longer where
+  // there would be more than 2048 of them.  What the call takes does not jump there, though the number of waves does: 524160
+  // tokens of 512 columns (8190 chunks of 64) 807 us, 524544 (2050 chunks of 256) 780 us; 262016 of 1024 columns 427 us, 262400
+  // 410 us.
   uint64_t chunk = 128;
   while (chunk > 32 && (n + chunk - 1) / chunk * p.n_cols < 4096) chunk >>= 1;
   if (chunk == 32 && (n + 15) / 16 * p.n_cols < 2048) chunk = 16;
@@ -616,8 +621,12 @@ void quantize_with(const QuantArgs& a, hipStream_t stream) {
 // Part of a wave or a wave a row while the row fits its registers (narrow rows: 45913 of 102 in bf16 6 us, 36 us with a wave),
 // else a workgroup a row, always with little more room than the row needs (64128 rows of 4096 in fp32: 215 us with room for
 // 4096, some 15 us more with room for 8192).  16-bit rows go further in a wave: 49268 of 832 31 us with 32 lanes, 33 us with 64;
-// 23040 of 2496 36 us with a wave, 48 us with a workgroup; 32768 of 2700 59 us, 71 us; 64128 of 4096 143 us, 157 us, but 8192 of
-// 4096 28 us, 25 us.  fp32 does not: 49268 of 832 38 us with 32 lanes, 36 us; 8246 of 2453 22.3 us with a wave, 20.7 us.
+// 23040 of 2496 36 us with a wave, 48 us with a workgroup; 32768 of 2700 59 us, 71 us.  From 3585 to 4096 that depends on the
+// rows.  bf16, 3600 wide, a wave and a workgroup: 8192 rows 27.7 and 23.5 us, 16384 43.2 and 41.3, 24576 59.1 and 59.4, 32768
+// 75.2 and 77.7, 64128 137 and 148 us; fp16: 24576 rows 56.3 and 53.7 us, 32768 71.0 and 69.8, 49152 101.5 and 102.4, 64128 130.3
+// and 131.8 us; 4096 wide alike.  One cut for both types, at 32768 rows, is within 6 % of the better one wherever it was measured
+// (farthest: fp16, 32768 of 3848, 75.5 and 71.6 us).  fp32 does not go further in a wave: 49268 of 832 38 us with 32 lanes, 36 us;
+// 8246 of 2453 22.3 us with a wave, 20.7 us.
 int quantize_launch(const QuantArgs& a, uint32_t dtype, hipStream_t stream) {
   with_type(dtype, [&](auto s) {
     typedef decltype(s) S;

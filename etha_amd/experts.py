@@ -3,7 +3,8 @@
 ``weight`` is ``[experts, out, in]``; rows ``offsets[e] .. offsets[e + 1]`` of ``x`` (sorted by expert) belong to expert ``e``.
 ``offsets`` stays on the device: sizes of a batch are never waited for.  A rank that holds a range of the experts
 (``Shard(0)``) passes that range of the offsets; column- and row-parallel shards (``Shard(1)``, ``Shard(2)``) pass their own
-part of ``out`` or ``in``, the latter's results being the members of a ``Partial("sum")``.
+part of ``out`` or ``in``, the latter's results being the members of a ``Partial("sum")`` (rounded to the type of ``x``; fp32
+members come by an ``out`` of that type).
 """
 
 from __future__ import annotations

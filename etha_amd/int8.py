@@ -76,7 +76,8 @@ def int8_matmul(x: torch.Tensor, x_scales: torch.Tensor, weight: torch.Tensor, w
     """``(x * x_scales[..., None]) @ (weight * weight_scales[:, None]).T + bias`` of 8-bit operands, in ``dtype``.
 
     ``x``: int8 ``[..., width]``; ``weight``: int8 ``[channels, width]``; scales and ``bias`` fp32.  The sum over the integers
-    is exact (``width`` up to 131071); scales and bias are applied in fp32 and rounded once.
+    is exact (``width`` up to 131071).  The rest is fp32: the sum is rounded to it, the two scales are multiplied, and their
+    product is applied to the sum, with the bias in one fused operation; then comes the result's type.
     """
     what = "int8_matmul"
     if x.dtype != torch.int8:
@@ -131,7 +132,11 @@ def int8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scales: torch.Tens
 class Int8Weight:
     """A weight in 8 bits that a transfer fills: the transfer writes ``landing`` (``[..., channels, width]`` in fp32, bf16 or
     fp16), :meth:`refresh` converts it into ``values`` (int8) and ``scales`` (fp32, one for each channel), which keep their
-    addresses, so that captured graphs read the new weights."""
+    addresses, so that captured graphs read the new weights.
+
+    The landing stays for the next transfer, whose plan holds its address: such a weight needs 3 or 5 bytes an element.  What
+    it saves is what a product reads.
+    """
 
     def __init__(self, landing: torch.Tensor):
         if landing.dim() < 2:

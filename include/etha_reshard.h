@@ -326,7 +326,7 @@ int etha_ipc_close(void* opened_ptr);
  *  - tensors are given by address and strides in elements of their own type; the last dimension is contiguous; rows
  *    may start at any multiple of the element size.  Types are ETHA_F32, ETHA_BF16 and ETHA_F16 unless said otherwise.
  *    Operands of products have rows at most 8 MiB apart.
- *  - sums are held in fp32 (32-bit integers for 8-bit products) and rounded once.
+ *  - sums are held in fp32 and rounded once to the result's type (those of 8-bit products in 32-bit integers, then fp32).
  *  - results do not depend on timing: the same call on the same values gives the same bits.
  *  - launches are asynchronous on `stream` of the current device and can be captured into a graph; nothing is allocated.
  *    An output must not overlap an input.
@@ -363,8 +363,9 @@ int etha_quantize_rows(const void* x, uint32_t dtype, uint64_t rows, uint64_t wi
                        int64_t values_stride, float* scales, void* stream);
 
 /*
- * Product of 8-bit rows with a scale each: out[m,n] = x_scale[m] * w_scale[n] * sum_k x[m,k] * w[n,k] + bias[n] (bias:
- * fp32, may be NULL; added in one fused operation).  The sum is exact; width is at most ETHA_INT8_MAX_WIDTH, so that it stays within 32 bits.
+ * Product of 8-bit rows with a scale each: out[m,n] = (x_scale[m] * w_scale[n]) * sum_k x[m,k] * w[n,k] + bias[n] (bias:
+ * fp32, may be NULL; added in one fused operation).  The sum is exact; width is at most ETHA_INT8_MAX_WIDTH, so that it stays
+ * within 32 bits.  It is rounded to fp32, as the product of the scales is, before the two are multiplied.
  */
 #define ETHA_INT8_MAX_WIDTH 131071u
 int etha_int8_matmul(const int8_t* x, const float* x_scale, uint64_t rows, int64_t x_stride, const int8_t* w, const float* w_scale,
