@@ -77,10 +77,10 @@ __global__ __launch_bounds__(256) void etha_embedding_kernel(const LookupArgs a)
 // a workgroup owns every 2^groups_log2-th row (frequent tokens lie close together) and looks through all tokens, a wave
 // through a run of them.  It counts those of each of its rows, wave by wave, and those of the workgroups before it, which
 // says where its own begin, and notes which they are; then every wave puts its tokens where the counts say.  Lanes whose
-// tokens have the same row find each other with one ballot per bit.  57984 tokens of 21716 rows 20 us, 6965 of 6676 rows 7 us
+// tokens have the same row find each other with one ballot per bit.  57984 tokens of 21716 rows 22 us, 6965 of 6676 rows 7 us
 // (a radix sort of two passes, with four launches, took 29 us and the gaps between them; one in a single workgroup 17 us for
 // the latter; runs of rows instead of every 256th, with the tokens looked through twice, 57 us for the former).  The looking,
-// some 10 instructions for 64 tokens, would take about 4 of those 20 us; how the rest is shared by clearing, scans and placing
+// some 10 instructions for 64 tokens, would take about 4 of those 22 us; how the rest is shared by clearing, scans and placing
 // has not been measured.
 constexpr uint32_t kSortThreads = 1024, kSortWaves = kSortThreads / kWave, kSortNoted = 1024;
 constexpr int kSortBinsLog2 = 10;
