@@ -58,7 +58,8 @@ class BatchHandler:
 
     def transfer(self, transfer_type: Literal["send", "recv"], blocking: bool = False, timeout: float = 30.0) -> Completion:
         """As the client's ``transfer``."""
-        return self.client._transfer(self.batch_id, transfer_type, f"batch_{self.batch_id}_{transfer_type}", blocking, timeout)
+        return self.client._transfer(self.batch_id, transfer_type, f"batch_{self.batch_id}_{transfer_type}", blocking, timeout,
+                                     self.int8_weights)
 
     def refresh_int8(self) -> None:
         """Convert the batch's 8-bit weights from what the last transfer brought (no counterpart in the reference), on the
@@ -175,13 +176,13 @@ class TensorBusClient:
                  timeout: float = 30.0) -> Completion:
         """A ``recv`` also converts the batch's 8-bit weights, on the stream that is current when its completion is
         acquired: within this call if it blocks, else in the returned completion's ``acquire``."""
-        return self._transfer(batch_id, transfer_type, batch_id, blocking, timeout)
+        return self._transfer(batch_id, transfer_type, batch_id, blocking, timeout, self._int8_weights.get(batch_id, ()))
 
-    def _transfer(self, batch_id: str, transfer_type: str, context_id: str, blocking: bool, timeout: float) -> Completion:
-        int8_weights = self._int8_weights.get(batch_id) if transfer_type == "recv" else None
+    def _transfer(self, batch_id: str, transfer_type: str, context_id: str, blocking: bool, timeout: float,
+                  int8_weights: tuple[Int8Weight, ...]) -> Completion:
         return self._execute_command_with_semaphore(
             Transfer(batch_id=batch_id, transfer_type=transfer_type), "transfer", context_id=context_id, blocking=blocking,
-            timeout=timeout, then=(lambda: _refresh(int8_weights)) if int8_weights else None)
+            timeout=timeout, then=(lambda: _refresh(int8_weights)) if int8_weights and transfer_type == "recv" else None)
 
     def query_transfer_signal(self, batch_id: str, blocking: bool = True, timeout: float = 30.0) -> bool:
         msg = QueryStatus(batch_id=batch_id, state_name="transfer_signal")

@@ -244,23 +244,26 @@ class ReshardJob:
 
     # ------------------------------------------------------------------------------------------
     def run_send(self, merge_launches: bool = False, fanout: int = 1, drive: bool = True) -> None:
-        """The senders' half of a transfer.  If nothing is waiting for a peer behind it, targets in 8 bits are converted;
-        who steps the wire otherwise (``drive=False``, a peer process) calls :meth:`refresh_int8` when it is idle."""
+        """The senders' half of a transfer.  If nothing of this job is waiting for a peer behind it, targets in 8 bits are
+        converted; who steps the wire otherwise (``drive=False``, a peer process) calls :meth:`refresh_int8` when it is done."""
         self._half(self.send_buckets, merge_launches, fanout, drive)
-        self._refresh_if_idle()
+        self._refresh_if_done()
 
     def run_recv(self, merge_launches: bool = False, fanout: int = 1, drive: bool = True) -> None:
         """The receivers' half of a transfer; targets in 8 bits as in :meth:`run_send`."""
         self._half(self.recv_buckets, merge_launches, fanout, drive)
-        self._refresh_if_idle()
+        self._refresh_if_done()
 
     def _half(self, lists: dict[int, list], merge_launches: bool, fanout: int, drive: bool) -> None:
         for buckets in lists.values():
             bucket_comm(buckets, self.max_in_flight, wire=self.wire, merge_launches=merge_launches, synchronize=False,
                         fanout=fanout, drive=drive)
 
-    def _refresh_if_idle(self) -> None:
-        if any(self.target_int8) and self.wire.idle():
+    def _refresh_if_done(self) -> None:
+        if not any(self.target_int8):
+            return
+        # of this job alone: others may share the wire
+        if not any(self.wire.in_progress(buckets) for lists in (self.send_buckets, self.recv_buckets) for buckets in lists.values()):
             self.refresh_int8()
 
     def refresh_int8(self) -> None:

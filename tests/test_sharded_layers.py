@@ -16,6 +16,7 @@ from etha_amd.embedding import embedding, embedding_grad
 from etha_amd.experts import grouped_linear, grouped_linear_grad
 from etha_amd.int8 import Int8Weight, int8_linear
 from etha_amd.layout import local_shard
+from etha_amd.tensor_bus.client import BatchHandler, TensorBusClient
 from etha_amd.tensor_bus.command_queue import Completion
 from etha_amd.world import ReshardJob, TensorSpec
 
@@ -378,3 +379,47 @@ def test_an_8_bit_weight_through_the_clients_own_transfer(gpu_device, agent_fact
         h.close()
     for c in clients.values():
         c.close()
+
+
+def test_another_job_on_the_wire_does_not_hold_up_the_conversion(monkeypatch):
+    seen = count_refreshes(monkeypatch)
+    wire = LoopbackWire("cpu", host_inspection=True)
+    wire.on_launch = lambda *a: None
+    job, other = (ReshardJob([TensorSpec("w", (64, 16), [n, n + 1], (Shard(0),), [n + 2, n + 3], (Shard(0),), torch.float32, target_int8=n == 0)],
+                             device="cpu", bucket_size=256, wire=wire) for n in (0, 4))
+    other.run_send()
+    job.run_send()
+    assert not seen
+    job.run_recv()
+    assert len(seen) == 2 and not wire.idle()
+    other.run_recv()
+    assert len(seen) == 2 and wire.idle()
+
+
+def test_a_handler_converts_the_weights_that_it_was_given(monkeypatch):
+    """Also one that was made with them, and not by its client's registration."""
+    seen = count_refreshes(monkeypatch)
+    weight = Int8Weight(torch.zeros(8, 4))
+
+    class Client:
+        _int8_weights = {}
+        agent_rank = 0
+        _transfer = TensorBusClient._transfer
+        _execute_command_with_semaphore = TensorBusClient._execute_command_with_semaphore
+
+        class command_queue:
+            @staticmethod
+            def enqueue(command):
+                class Done:
+                    poll = staticmethod(lambda timeout: True)
+                    recv = staticmethod(lambda: ("ok", None))
+                    close = staticmethod(lambda: None)
+
+                return Completion(Done(), "done")
+
+    client = Client()
+    handler = BatchHandler(client, "b", ["w"], (weight,))
+    handler.transfer("send", blocking=True)
+    assert not seen
+    handler.transfer("recv", blocking=True)
+    assert len(seen) == 1
