@@ -76,6 +76,19 @@ def _byte_range(t: torch.Tensor) -> tuple[int, int]:
     return t.data_ptr() + lo * es, t.data_ptr() + (hi + 1) * es
 
 
+def _interleaved(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether ``a`` and ``b`` are columns of their own of rows that lie at one distance, as those of one wide buffer: modulo
+    that distance, no byte of one then lies where one of the other does."""
+    if not a.dim() or not b.dim():
+        return False
+    step_a, step_b = row_stride(a), row_stride(b)
+    if not step_a or not step_b or step_a * a.element_size() != step_b * b.element_size():
+        return False
+    apart = step_a * a.element_size()
+    behind = (b.data_ptr() - a.data_ptr()) % apart
+    return a.shape[-1] * a.element_size() <= behind and behind + b.shape[-1] * b.element_size() <= apart
+
+
 def check_out(what: str, out: torch.Tensor, shape, dtypes, *inputs: torch.Tensor | None) -> int:
     """Checks an output that the caller passes; returns its row stride."""
     if out.shape != shape:
@@ -97,7 +110,7 @@ def check_out(what: str, out: torch.Tensor, shape, dtypes, *inputs: torch.Tensor
         for t in inputs:
             if t is not None and t.numel():
                 a, b = _byte_range(t)
-                if a < hi and lo < b:
+                if a < hi and lo < b and not _interleaved(t, out):
                     raise ValueError(f"{what}: out overlaps an input")
     return stride
 
