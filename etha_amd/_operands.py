@@ -115,12 +115,10 @@ def check_out(what: str, out: torch.Tensor, shape, dtypes, *inputs: torch.Tensor
     return stride
 
 
-def written(*outs: torch.Tensor | None) -> None:
-    """Tells autograd that the caller's tensors were written: kernels write by address, which it cannot see, and a graph that
-    saved one of them earlier would go on with the new values."""
-    for out in outs:
-        if out is not None:
-            increment_version(out)
+def written(out: torch.Tensor) -> None:
+    """Tells autograd that a tensor of the caller's was written: kernels write by address, which it cannot see, and a graph that
+    saved it earlier would go on with the new values."""
+    increment_version(out)
 
 
 def refuse_tangent(what: str, *tensors: torch.Tensor | None) -> None:
@@ -134,7 +132,8 @@ def refuse_tangent(what: str, *tensors: torch.Tensor | None) -> None:
 
 def refuse_grad(what: str, *inputs: torch.Tensor | None) -> None:
     """For operators without a gradient: a silent cut of the graph would train on nothing."""
-    refuse_tangent(what, *inputs)
+    if forward_ad._current_level >= 0:
+        refuse_tangent(what, *inputs)
     for t in inputs:
         if t is not None and t.requires_grad and torch.is_grad_enabled():
             raise RuntimeError(f"{what} has no gradient: call it under torch.no_grad() or detach its inputs")

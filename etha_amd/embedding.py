@@ -25,7 +25,8 @@ def _token_operand(what: str, tokens: torch.Tensor) -> tuple[torch.Tensor, int]:
 
 
 def _first_row(what: str, first_row) -> int:
-    first_row = operator.index(first_row)
+    if type(first_row) is not int:
+        first_row = operator.index(first_row)
     if not -(1 << 63) <= first_row < 1 << 63:
         raise ValueError(f"{what}: first_row {first_row} has more than 64 bits")
     return first_row
@@ -55,7 +56,8 @@ def _lookup(tokens, weight, scale, first_row, dtype, out):
         device = check_device("embedding", weight, tokens, out)
     call(device, "etha_embedding", source.data_ptr(), token_code, tokens.numel(), weight.data_ptr(),
          weight_code, rows, width, stride, first_row, scale, out.data_ptr(), out_code, out_stride)
-    written(given)
+    if given is not None:
+        written(given)
     return out
 
 
@@ -129,5 +131,6 @@ def embedding_grad(grad: torch.Tensor, tokens: torch.Tensor, n_rows: int, *, sca
     call(device, "etha_embedding_grad", grad.data_ptr(), grad_code, grad_stride, source.data_ptr(),
          token_code, n_tokens, n_rows, width, first_row, scale, out.data_ptr(), out_code, out_stride, int(accumulate),
          workspace.data_ptr() if nbytes else None, nbytes)
-    written(given)
+    if given is not None:
+        written(given)
     return out

@@ -67,7 +67,8 @@ def _product(what, x, weight, offsets, transposed, out):
     call(device, "etha_grouped_matmul", source.data_ptr(), _OPERANDS[x.dtype], rows, stride,
          weight.data_ptr(), experts, cols, red, w_stride, w_group, int(transposed), offsets.data_ptr(), out.data_ptr(),
          DTYPE_CODES[out.dtype], out_stride, int(fresh))
-    written(given)
+    if given is not None:
+        written(given)
     return out
 
 
@@ -139,7 +140,8 @@ def grouped_linear_grad_weight(grad: torch.Tensor, x: torch.Tensor, offsets: tor
     call(device, "etha_grouped_matmul_reduce", g.data_ptr(), r.data_ptr(), _OPERANDS[x.dtype], x.shape[0], g_stride, r_stride, experts,
          n, k, offsets.data_ptr(), out.data_ptr(), DTYPE_CODES[out.dtype], out.stride(1), out.stride(0),
          workspace.data_ptr() if nbytes else None, nbytes)
-    written(given)
+    if given is not None:
+        written(given)
     return out
 
 

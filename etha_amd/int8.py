@@ -45,7 +45,9 @@ def quantize_rows(x: torch.Tensor, *, values: torch.Tensor | None = None,
         scales = x.new_empty(x.shape[:-1], dtype=torch.float32)
     call(device, "etha_quantize_rows", source.data_ptr(), code, rows, width, stride,
          values.data_ptr(), values_stride, scales.data_ptr())
-    written(*given)
+    for out in given:
+        if out is not None:
+            written(out)
     return values, scales
 
 
@@ -96,7 +98,8 @@ def int8_matmul(x: torch.Tensor, x_scales: torch.Tensor, weight: torch.Tensor, w
     call(device, "etha_int8_matmul", source.data_ptr(), x_scales.data_ptr(), rows, stride,
          weight.data_ptr(), weight_scales.data_ptr(), channels, w_stride, width, None if bias is None else bias.data_ptr(),
          out.data_ptr(), DTYPE_CODES[out.dtype], out_stride)
-    written(given)
+    if given is not None:
+        written(given)
     return out
 
 
@@ -125,7 +128,8 @@ def int8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scales: torch.Tens
     call(device, "etha_int8_linear", source.data_ptr(), x_code, rows, stride, weight.data_ptr(),
          weight_scales.data_ptr(), channels, w_stride, width, None if bias is None else bias.data_ptr(), out.data_ptr(),
          DTYPE_CODES[out.dtype], out_stride, workspace.data_ptr() if nbytes else None, nbytes)
-    written(given)
+    if given is not None:
+        written(given)
     return out
 
 
